@@ -53,6 +53,13 @@
  *   marian_hip_candidate_argmax  select_token over a lexical shortlist's candidates
  *                              (shortlist.rs:150-198)
  *   marian_hip_positions       sinusoidal_positions crates/marian-model/src/position.rs:5-21
+ * Op-level entry points without a counterpart in the reference, for one decode
+ * step of many requests in a pre-norm stack (each request with its own adapter
+ * and its own sampling settings):
+ *   marian_hip_residual_rms_norm  residual addition, RMS norm, int8 rows
+ *   marian_hip_q8_linear_lora  a Q8 layer with each row's own low-rank adapter
+ *   marian_hip_sample_logits, marian_hip_sample_candidates  temperature, top-k,
+ *                              top-p and min-p sampling from given numbers
  * The op-level entry points that need intermediate device buffers keep them
  * in library scratch, one set per (device, stream), kept until the process
  * ends: calls on different streams do not share it, and calls on one stream
@@ -79,10 +86,12 @@
 extern "C" {
 #endif
 
-#define MARIAN_HIP_ABI_VERSION 4 /* 2: marian_hip_attention takes head_dim;
+#define MARIAN_HIP_ABI_VERSION 5 /* 2: marian_hip_attention takes head_dim;
                                     3: the Transformer-SSRU engine, shortlisted translate;
                                     4: warmup, reserve, validate_batch, stats
-                                       launched_steps and allocations */
+                                       launched_steps and allocations;
+                                    5: residual_rms_norm, q8_linear_lora, sample_logits,
+                                       sample_candidates */
 
 enum {
   MARIAN_HIP_OK = 0,
@@ -448,6 +457,48 @@ int marian_hip_residual_layer_norm(const float* x, const float* r, const float* 
                                    const float* bias, int64_t rows, int64_t dim, float* out,
                                    int8_t* q, float* a, int* err, void* stream);
 
+/* Root-mean-square norm with the residual's addition and int8 rows (no
+ * counterpart in the reference): s = x + r (fp32), y = s / sqrt(mean(s^2) + eps)
+ * * scale, a[m] = 127 / max|y[m,:]| (1 for a zero row), q = clamp(rne(y a), -127,
+ * 127).  The mean and y are computed in 64 bits and rounded once, so results do
+ * not depend on the launch; a and q are what marian_hip_quantize_rows makes of y.
+ * x and r (r may be NULL: s = x) are fp32 rows, or bfloat16 with in_bf16 != 0, ldx
+ * and ldr values apart, at any value-aligned address.  dim 1 to 16384, eps > 0.
+ * sum (s, the residual stream), out (y) and q with a are contiguous rows, each
+ * optional, but one of out and q must be given.  fp32 outputs may be x or r
+ * themselves when those are fp32 rows dim apart; other overlaps are refused.
+ * err (device int, may be NULL) is set to 1 when a y is not finite. */
+int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int64_t ldr,
+                                 const float* scale, float eps, int64_t rows, int64_t dim,
+                                 int in_bf16, float* sum, float* out, int8_t* q, float* a, int* err,
+                                 void* stream);
+
+/* marian_hip_q8_linear with each row's own low-rank adapter (no counterpart in
+ * the reference), s = slot_of_row[m]:
+ *   out[m] = (relu of) acc * (1/(xa[m] w_mult)) + bias + lora_scale[s] * B_s (A_s x[m])
+ * A row with a negative slot has no adapter.  lora_a [slots, max_rank, K] and
+ * lora_b [slots, N, max_rank] hold bfloat16 values; slot s uses its first
+ * lora_rank[s] (0 to max_rank) rows of A and columns of B, the rest is not used.
+ * max_rank is a multiple of 8 up to 128, K a multiple of 64.  A slot at or past
+ * `slots`, or a rank out of range, sets *err (device int, may be NULL) to 1 and
+ * counts as no adapter; a row's result does not depend on other rows' adapters.
+ * x (fp32 [M, K]) is always given, it is what the adapters read; xq / xa are its
+ * codes and multipliers (both or neither: then the call quantizes x, and a
+ * non-finite x sets *err).  The adapters' products are sums of fp32 with exact bf16
+ * weights.  out may share memory with x (not with xq, nor with the
+ * weights).  x, xq, w, lora_a, lora_b and workspace must be 16-byte aligned.
+ * workspace: device memory of marian_hip_q8_linear_lora_workspace bytes that no
+ * other call uses meanwhile, or NULL for library scratch.  A call captured into
+ * a graph must bring one (the graph owns it for its life). */
+int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa, int64_t M, int64_t K,
+                              const int8_t* w, const float* w_mult, const float* bias, int64_t N, int relu,
+                              const uint16_t* lora_a, const uint16_t* lora_b, const float* lora_scale,
+                              const int32_t* lora_rank, int64_t slots, int64_t max_rank,
+                              const int32_t* slot_of_row, float* out_f32, void* workspace,
+                              size_t workspace_bytes, int* err, void* stream);
+/* Bytes of workspace of a call with these sizes (has_xq: xq / xa are given). */
+int marian_hip_q8_linear_lora_workspace(int64_t M, int64_t K, int64_t max_rank, int has_xq, size_t* bytes);
+
 /* Variable-length attention: query row i belongs to sequence seq_of_row[i]
  * and attends over key rows [cu_k[s], cu_k[s+1]); max_keys bounds every range
  * (at most 4096); heads <= 16 of width head_dim (64, or 48 as in the
@@ -489,6 +540,40 @@ int marian_hip_candidate_argmax(const int8_t* xq, const float* xa, int64_t M, in
                                 int64_t V, const uint32_t* cand, const uint32_t* cand_offsets,
                                 int64_t max_cands, int32_t* token, float* logits, int* err,
                                 void* stream);
+
+/* One id per row of logits, drawn with given numbers (no counterpart in the
+ * reference, which is greedy).  Row m is logits[m * ld .. + V), fp32, or bfloat16
+ * with in_bf16 != 0, at any value-aligned address; NaN and -inf ids are never
+ * drawn (the generation mask of marian_hip_vocab_argmax's logits).  Per row, each
+ * array may be NULL: temperature (>= 0; NULL 1; 0 takes the maximum), top_k (NULL
+ * or <= 0: no limit), top_p (>= 0; NULL or >= 1: no limit), min_p (0 to 1; NULL 0);
+ * u in [0, 1).  With ids ordered by logit, equal logits by lower id first, and
+ * p ~ exp(logit / temperature): top_k keeps the first k, top_p of those the
+ * shortest prefix (at least one id) with top_p of their mass, min_p of those the
+ * ids with p >= min_p * max(p).  token[m] is the first kept id in ascending order
+ * whose running kept mass exceeds u of the kept mass; logprob[m] (optional) the
+ * logarithm of its share of the kept mass.  Masses are multiples of 2^-44 of the
+ * maximum's, and their sums exact: ids below 2^-45 of it are never drawn, and a
+ * row's result does not depend on the launch or on other rows.  A row of only
+ * -inf and NaN gets id 0 and logprob -inf.  A setting or u out of range sets *err
+ * (device int, may be NULL) to 1, and the row's maximum is taken.
+ * V up to 524288, rows up to 1048576.  Nothing is allocated. */
+int marian_hip_sample_logits(const void* logits, int64_t ld, int64_t rows, int64_t V, int in_bf16,
+                             const float* temperature, const int32_t* top_k, const float* top_p,
+                             const float* min_p, const float* u, int32_t* token, float* logprob,
+                             int* err, void* stream);
+
+/* The same over per-row candidate lists, as marian_hip_candidate_argmax scores
+ * them: row m's fp32 logits are logits[cand_offsets[m] .. cand_offsets[m+1]), for
+ * the ids at the same places of cand (ascending), and token[m] is one of those.
+ * max_cands (up to 524288) bounds every list's length: a longer list sets *err and
+ * only its first max_cands are looked at.  An empty list gives token -1 and
+ * logprob -inf; decreasing offsets set *err and count as an empty list. */
+int marian_hip_sample_candidates(const float* logits, const uint32_t* cand, const uint32_t* cand_offsets,
+                                 int64_t rows, int64_t max_cands, const float* temperature,
+                                 const int32_t* top_k, const float* top_p, const float* min_p,
+                                 const float* u, int32_t* token, float* logprob, int* err,
+                                 void* stream);
 
 /* marian_hip_vocab_argmax without any device allocation.  No counterpart in
  * the reference: it is for callers that cannot allocate device memory (code

@@ -121,6 +121,32 @@ hipError_t launch_linear_f32(const GemmArgs& g, const Epilogue& e, hipStream_t s
 // Picks the kernel by M (host-known M only).
 hipError_t launch_gemm_store(const GemmArgs& g, const Epilogue& e, hipStream_t s);
 
+// Low-rank adapters beside a Q8 layer: out[m] = (relu of) Q8(x[m]) + scale[s]
+// b[s] (a[s] x[m]) for s = slot_of_row[m] (negative: no adapter), from fp32 rows x
+// [M, K].  a [slots, max_rank, K] and b [slots, N, max_rank] are bf16; slot s uses
+// its first rank[s] rows of a and columns of b.  launch_lora_down fills t
+// (lora_scratch_bytes) with the rows' products with a; launch_lora_linear
+// computes the layer from the quantized rows in `base` and t.
+constexpr int kLoraMaxRank = 128;  // and a multiple of 8
+struct LoraArgs {
+  const float* x = nullptr;
+  int64_t M = 0;
+  int K = 0, N = 0;
+  const uint16_t* a = nullptr;
+  const uint16_t* b = nullptr;
+  const float* scale = nullptr;
+  const int32_t* rank = nullptr;
+  int slots = 0, max_rank = 0;
+  const int32_t* slot_of_row = nullptr;
+  float* t = nullptr;
+  int relu = 0;
+  float* out = nullptr;  // [M, N]
+  int* err = nullptr;    // set to 1 on a slot or rank out of range (the row then has no adapter)
+};
+size_t lora_scratch_bytes(int64_t M, int max_rank);
+hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s);
+hipError_t launch_lora_linear(const GemmArgs& base, const LoraArgs& g, hipStream_t s);
+
 hipError_t launch_quantize_rows(const float* x, int64_t ldx, int rows, const int* rows_dev,
                                 int cols, int8_t* q, int64_t ldq, float* a, int* err,
                                 hipStream_t s);
@@ -132,6 +158,28 @@ hipError_t launch_residual_ln(const float* y, const float* r, const float* g, co
                               int rows, const int* rows_dev, int d, float* out, int8_t* q,
                               float* a, int* err, hipStream_t s, float qmult = 0.0f,
                               bool fast = false);
+
+// Residual addition, root-mean-square norm and int8 rows: s = x + r (r
+// optional), y = s / sqrt(mean(s^2) + eps) * scale, each row's multiplier
+// a = 127 / max|y| and codes q.  x and r are fp32 or bf16 rows ldx / ldr values
+// apart; sum (s), out (y), q and a are contiguous and each optional (q needs a).
+constexpr int kRmsMaxDim = 16384;
+struct RmsArgs {
+  const void* x = nullptr;
+  const void* r = nullptr;
+  int64_t ldx = 0, ldr = 0;
+  const float* scale = nullptr;
+  float eps = 0.0f;
+  int bf16 = 0;
+  int64_t rows = 0;
+  int dim = 0;
+  float* sum = nullptr;
+  float* out = nullptr;
+  int8_t* q = nullptr;
+  float* a = nullptr;
+  int* err = nullptr;  // set to 1 on a non-finite y
+};
+hipError_t launch_rms_norm(const RmsArgs& g, hipStream_t s);
 
 // Quantization with one static activation multiplier for every row (a[row] =
 // mult); rejects a multiplier that is not finite and positive.
@@ -449,6 +497,30 @@ struct CandArgs {
 int cand_groups(int max_cands);
 bool cand_ln_supported(int K);
 hipError_t launch_cand_argmax(const CandArgs& c, hipStream_t s);
+
+// One drawn id per row of logits (fp32 or bf16): row r is logits[r * ld .. + V),
+// or with off the list logits[off[r] .. off[r + 1]) of ids cand[...] (at most V
+// of them).  Settings per row, each array optional: temperature (1; 0: the
+// maximum), top_k (0: no limit), top_p (1), min_p (0); u in [0, 1).
+constexpr int kSampleMaxRows = 1 << 20;
+constexpr int kSampleMaxIds = 1 << 19;  // sums of 2^44 stay below 2^63; groups of 512 ids
+struct SampleArgs {
+  const void* logits = nullptr;
+  int64_t ld = 0;
+  int bf16 = 0;
+  const uint32_t* cand = nullptr;
+  const uint32_t* off = nullptr;
+  int rows = 0, V = 0;
+  const float* temperature = nullptr;
+  const int32_t* top_k = nullptr;
+  const float* top_p = nullptr;
+  const float* min_p = nullptr;
+  const float* u = nullptr;
+  int32_t* token = nullptr;
+  float* logprob = nullptr;  // optional
+  int* err = nullptr;        // set to 1 on a setting out of range (the row's maximum is drawn)
+};
+hipError_t launch_sample(const SampleArgs& g, hipStream_t s);
 
 // Reduces argmax partials to token ids (op-level argmax).
 // Records the message marian_hip_last_op_error returns on this thread.

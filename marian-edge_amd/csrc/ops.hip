@@ -35,8 +35,8 @@ int op_status(hipError_t e, const char* what) {
 // Sets live until the process ends (a stream that is destroyed leaves its
 // set behind).
 struct OpScratch {
-  void* p[3] = {nullptr, nullptr, nullptr};
-  size_t cap[3] = {0, 0, 0};
+  void* p[4] = {nullptr, nullptr, nullptr, nullptr};
+  size_t cap[4] = {0, 0, 0, 0};
 };
 std::mutex g_scratch_mu;
 std::map<std::pair<int, uintptr_t>, OpScratch> g_scratch;
@@ -166,6 +166,36 @@ int linear_op(const float* x, float act, const int8_t* xq, const float* xa, int6
   return op_status(launch_gemm_store(g, e, s), what);
 }
 
+// Records why a call is refused.
+int refuse(const char* what) {
+  g_op_error = what;
+  return MARIAN_HIP_ERR_INVALID_INPUT;
+}
+
+// Whether `stream` is recording a graph (the default stream cannot).
+bool capturing(hipStream_t s) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  return s && hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+}
+
+// Workspace of the adapter layer: the rows' products with the adapters, then,
+// when the call quantizes x itself, the codes and multipliers.
+struct LoraWorkspace {
+  size_t codes, mults, bytes;  // offsets, total
+};
+LoraWorkspace lora_workspace(int64_t M, int64_t K, int64_t max_rank, bool has_xq) {
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  LoraWorkspace w;
+  w.codes = up(lora_scratch_bytes(M, (int)max_rank));
+  w.mults = w.codes + (has_xq ? 0 : up((size_t)M * K));
+  w.bytes = w.mults + (has_xq ? 0 : up((size_t)M * 4));
+  return w;
+}
+bool lora_sizes_ok(int64_t M, int64_t K, int64_t max_rank) {
+  return M >= 0 && M <= INT32_MAX && K > 0 && K <= INT32_MAX && K % 64 == 0 && max_rank > 0 &&
+         max_rank <= kLoraMaxRank && max_rank % 8 == 0;
+}
+
 bool vocab_args_ok(const int8_t* xq, const float* xa, int64_t M, int64_t K, const int8_t* emb,
                    const float* emb_mult, const float* bias, int64_t V, const int32_t* token) {
   return xq && xa && emb && emb_mult && bias && token && M >= 0 && K > 0 && K % 64 == 0 &&
@@ -231,6 +261,168 @@ int marian_hip_residual_layer_norm(const float* x, const float* r, const float* 
   return op_status(launch_residual_ln(x, r, scale, bias, (int)rows, nullptr, (int)dim, out, q, a,
                                       err, (hipStream_t)stream),
                    "residual_layer_norm");
+}
+
+int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int64_t ldr,
+                                 const float* scale, float eps, int64_t rows, int64_t dim,
+                                 int in_bf16, float* sum, float* out, int8_t* q, float* a, int* err,
+                                 void* stream) {
+  if (!x || !scale || rows < 0 || rows > INT32_MAX || dim <= 0 || dim > kRmsMaxDim || ldx < dim ||
+      (r && ldr < dim) || !(eps > 0.0f) || !std::isfinite(eps))
+    return refuse("residual_rms_norm: sizes, strides or eps out of range, or x or scale missing");
+  if (!out && !q) return refuse("residual_rms_norm: neither out nor q is given");
+  if (!q != !a) return refuse("residual_rms_norm: q and a go together");
+  // Outputs may be x or r themselves (fp32 rows dim apart), and share no other memory.
+  const size_t n = (size_t)rows * dim, vb = in_bf16 ? 2 : 4;
+  const struct { const void* p; size_t bytes; bool same; } ins[] = {
+      {x, rows ? ((size_t)(rows - 1) * ldx + dim) * vb : 0, !in_bf16 && ldx == dim},
+      {r, rows ? ((size_t)(rows - 1) * ldr + dim) * vb : 0, !in_bf16 && ldr == dim},
+      {scale, (size_t)dim * 4, false}};
+  const struct { const void* p; size_t bytes; bool f32; } outs[] = {
+      {sum, n * 4, true}, {out, n * 4, true}, {q, n, false}, {a, (size_t)rows * 4, false}};
+  for (int i = 0; i < 4; ++i) {
+    for (const auto& in : ins)
+      if (overlap(outs[i].p, outs[i].bytes, in.p, in.bytes) && !(outs[i].f32 && in.same && outs[i].p == in.p))
+        return refuse("residual_rms_norm: an output overlaps an input");
+    for (int k = 0; k < i; ++k)
+      if (overlap(outs[i].p, outs[i].bytes, outs[k].p, outs[k].bytes))
+        return refuse("residual_rms_norm: two outputs overlap");
+  }
+  RmsArgs g;
+  g.x = x;
+  g.r = r;
+  g.ldx = ldx;
+  g.ldr = ldr;
+  g.scale = scale;
+  g.eps = eps;
+  g.bf16 = in_bf16 ? 1 : 0;
+  g.rows = rows;
+  g.dim = (int)dim;
+  g.sum = sum;
+  g.out = out;
+  g.q = q;
+  g.a = a;
+  g.err = err;
+  return op_status(launch_rms_norm(g, (hipStream_t)stream), "residual_rms_norm");
+}
+
+int marian_hip_q8_linear_lora_workspace(int64_t M, int64_t K, int64_t max_rank, int has_xq, size_t* bytes) {
+  if (!bytes || !lora_sizes_ok(M, K, max_rank)) return refuse("q8_linear_lora_workspace: sizes out of range");
+  *bytes = lora_workspace(M, K, max_rank, has_xq).bytes;
+  return MARIAN_HIP_OK;
+}
+
+int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa, int64_t M, int64_t K,
+                              const int8_t* w, const float* w_mult, const float* bias, int64_t N, int relu,
+                              const uint16_t* lora_a, const uint16_t* lora_b, const float* lora_scale,
+                              const int32_t* lora_rank, int64_t slots, int64_t max_rank,
+                              const int32_t* slot_of_row, float* out_f32, void* workspace,
+                              size_t workspace_bytes, int* err, void* stream) {
+  if (!lora_sizes_ok(M, K, max_rank) || N <= 0 || N > INT32_MAX || slots <= 0 || slots > INT32_MAX)
+    return refuse("q8_linear_lora: sizes out of range");
+  if (!x || !w || !w_mult || !bias || !lora_a || !lora_b || !lora_scale || !lora_rank || !slot_of_row || !out_f32 ||
+      !xq != !xa)
+    return refuse("q8_linear_lora: a tensor is missing");
+  if (((uintptr_t)x | (uintptr_t)xq | (uintptr_t)w | (uintptr_t)lora_a | (uintptr_t)lora_b | (uintptr_t)workspace) % 16)
+    return refuse("q8_linear_lora: x, xq, w, lora_a, lora_b and workspace must be 16-byte aligned");
+  if (M == 0) return MARIAN_HIP_OK;
+  hipStream_t s = (hipStream_t)stream;
+  const LoraWorkspace ws = lora_workspace(M, K, max_rank, xq != nullptr);
+  if (workspace) {
+    if (workspace_bytes < ws.bytes) return refuse("q8_linear_lora: the workspace is too small");
+  } else {
+    // A graph would go on using scratch that a later call may replace.
+    if (capturing(s)) return refuse("q8_linear_lora: a call that is captured into a graph needs a workspace");
+    workspace = op_scratch(3, ws.bytes, s);
+    if (!workspace) return op_status(hipErrorOutOfMemory, "q8_linear_lora scratch");
+  }
+  LoraArgs l;
+  l.x = x;
+  l.M = M;
+  l.K = (int)K;
+  l.N = (int)N;
+  l.a = lora_a;
+  l.b = lora_b;
+  l.scale = lora_scale;
+  l.rank = lora_rank;
+  l.slots = (int)slots;
+  l.max_rank = (int)max_rank;
+  l.slot_of_row = slot_of_row;
+  l.t = (float*)workspace;
+  l.relu = relu;
+  l.out = out_f32;
+  l.err = err;
+  int8_t* q = (int8_t*)workspace + ws.codes;
+  float* a = (float*)((char*)workspace + ws.mults);
+  int rc;
+  if (!xq) {
+    rc = op_status(launch_quantize_rows(x, K, (int)M, nullptr, (int)K, q, K, a, err, s), "q8_linear_lora");
+    if (rc) return rc;
+    xq = q;
+    xa = a;
+  }
+  rc = op_status(launch_lora_down(l, s), "q8_linear_lora down");
+  if (rc) return rc;
+  GemmArgs g;
+  g.A = xq;
+  g.a = xa;
+  g.lda = K;
+  g.M = (int)M;
+  g.K = (int)K;
+  g.W = w;
+  g.wmult = w_mult;
+  g.bias = bias;
+  g.N = (int)N;
+  return op_status(launch_lora_linear(g, l, s), "q8_linear_lora");
+}
+
+int marian_hip_sample_logits(const void* logits, int64_t ld, int64_t rows, int64_t V, int in_bf16,
+                             const float* temperature, const int32_t* top_k, const float* top_p,
+                             const float* min_p, const float* u, int32_t* token, float* logprob,
+                             int* err, void* stream) {
+  if (!logits || !u || !token) return refuse("sample_logits: logits, u or token is missing");
+  if (rows < 0 || rows > kSampleMaxRows || V <= 0 || V > kSampleMaxIds || ld < V)
+    return refuse("sample_logits: sizes out of range");
+  SampleArgs g;
+  g.logits = logits;
+  g.ld = ld;
+  g.bf16 = in_bf16 ? 1 : 0;
+  g.rows = (int)rows;
+  g.V = (int)V;
+  g.temperature = temperature;
+  g.top_k = top_k;
+  g.top_p = top_p;
+  g.min_p = min_p;
+  g.u = u;
+  g.token = token;
+  g.logprob = logprob;
+  g.err = err;
+  return op_status(launch_sample(g, (hipStream_t)stream), "sample_logits");
+}
+
+int marian_hip_sample_candidates(const float* logits, const uint32_t* cand, const uint32_t* cand_offsets,
+                                 int64_t rows, int64_t max_cands, const float* temperature,
+                                 const int32_t* top_k, const float* top_p, const float* min_p,
+                                 const float* u, int32_t* token, float* logprob, int* err,
+                                 void* stream) {
+  if (!logits || !cand || !cand_offsets || !u || !token) return refuse("sample_candidates: a tensor is missing");
+  if (rows < 0 || rows > kSampleMaxRows || max_cands <= 0 || max_cands > kSampleMaxIds)
+    return refuse("sample_candidates: sizes out of range");
+  SampleArgs g;
+  g.logits = logits;
+  g.cand = cand;
+  g.off = cand_offsets;
+  g.rows = (int)rows;
+  g.V = (int)max_cands;
+  g.temperature = temperature;
+  g.top_k = top_k;
+  g.top_p = top_p;
+  g.min_p = min_p;
+  g.u = u;
+  g.token = token;
+  g.logprob = logprob;
+  g.err = err;
+  return op_status(launch_sample(g, (hipStream_t)stream), "sample_candidates");
 }
 
 int marian_hip_attention(const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,

@@ -125,6 +125,54 @@ def residual_layer_norm(x, r, scale, bias, out, q=None, a=None, err=None, stream
         "residual_layer_norm")
 
 
+def residual_rms_norm(x, r, scale, eps: float, total=None, out=None, q=None, a=None, bf16: bool = False, ldx=None,
+                      ldr=None, err=None, stream=None) -> None:
+    """marian_hip_residual_rms_norm: total = x + r, out its root-mean-square norm,
+    q / a out's int8 rows and multipliers; r None: the norm of x alone."""
+    rows, dim = x.shape[0], scale.shape[0]
+    _lib.check(_lib.load().marian_hip_residual_rms_norm(
+        x.ptr, ldx or x.shape[1], _p(r), ldr or (r.shape[1] if r is not None else 0), scale.ptr, eps, rows, dim,
+        int(bf16), _p(total), _p(out), _p(q), _p(a), _p(err), stream), "residual_rms_norm")
+
+
+def q8_linear_lora(x, w, mult, bias, lora_a, lora_b, lora_scale, lora_rank, slot_of_row, out, relu: bool = False,
+                   xq=None, xa=None, workspace=None, err=None, stream=None) -> None:
+    """marian_hip_q8_linear_lora: lora_a [slots, max_rank, K] and lora_b [slots, N,
+    max_rank] hold bfloat16 values (as uint16).  workspace: a byte buffer of
+    q8_linear_lora_workspace bytes, needed when the call is captured into a graph."""
+    M, K = x.shape
+    slots, max_rank = lora_a.shape[0], lora_a.shape[1]
+    _lib.check(_lib.load().marian_hip_q8_linear_lora(
+        x.ptr, _p(xq), _p(xa), M, K, w.ptr, mult.ptr, bias.ptr, w.shape[0], int(relu), lora_a.ptr, lora_b.ptr,
+        lora_scale.ptr, lora_rank.ptr, slots, max_rank, slot_of_row.ptr, out.ptr, _p(workspace),
+        workspace.nbytes if workspace is not None else 0, _p(err), stream), "q8_linear_lora")
+
+
+def q8_linear_lora_workspace(M: int, K: int, max_rank: int, quantized: bool) -> int:
+    """Bytes of workspace of q8_linear_lora (quantized: with xq and xa)."""
+    n = C.c_size_t(0)
+    _lib.check(_lib.load().marian_hip_q8_linear_lora_workspace(M, K, max_rank, int(quantized), C.byref(n)),
+               "q8_linear_lora_workspace")
+    return n.value
+
+
+def sample_logits(logits, u, token, temperature=None, top_k=None, top_p=None, min_p=None, logprob=None,
+                  bf16: bool = False, ids=None, err=None, stream=None) -> None:
+    """marian_hip_sample_logits; ids: the row's ids when fewer than its stride."""
+    rows, ld = logits.shape
+    _lib.check(_lib.load().marian_hip_sample_logits(
+        logits.ptr, ld, rows, ids or ld, int(bf16), _p(temperature), _p(top_k), _p(top_p), _p(min_p), u.ptr, token.ptr,
+        _p(logprob), _p(err), stream), "sample_logits")
+
+
+def sample_candidates(logits, cand, cand_offsets, max_cands: int, u, token, temperature=None, top_k=None, top_p=None,
+                      min_p=None, logprob=None, err=None, stream=None) -> None:
+    """marian_hip_sample_candidates: the logits that candidate_argmax wrote, drawn from."""
+    _lib.check(_lib.load().marian_hip_sample_candidates(
+        logits.ptr, cand.ptr, cand_offsets.ptr, cand_offsets.shape[0] - 1, int(max_cands), _p(temperature), _p(top_k),
+        _p(top_p), _p(min_p), u.ptr, token.ptr, _p(logprob), _p(err), stream), "sample_candidates")
+
+
 def attention(q, k, v, seq_of_row, cu, out, heads: int, max_keys: int, ldq=None, ldkv=None,
               ldo=None, bf16: bool = False, packed_self: bool = True, head_dim: int = 64,
               stream=None) -> None:
