@@ -125,9 +125,11 @@ hipError_t launch_gemm_store(const GemmArgs& g, const Epilogue& e, hipStream_t s
 // b[s] (a[s] x[m]) for s = slot_of_row[m] (negative: no adapter), from fp32 rows x
 // [M, K].  a [slots, max_rank, K] and b [slots, N, max_rank] are bf16; slot s uses
 // its first rank[s] rows of a and columns of b.  launch_lora_down fills t
-// (lora_scratch_bytes) with the rows' products with a; launch_lora_linear
-// computes the layer from the quantized rows in `base` and t.
+// (lora_scratch_bytes) with the rows' products with a, and quantizes the rows into
+// xq / xa when those are given; launch_lora_linear computes the layer from the
+// quantized rows in `base` and t.
 constexpr int kLoraMaxRank = 128;  // and a multiple of 8
+constexpr int kLoraMaxN = (1 << 20) - 1;  // a tile's output rows stay within 32-bit buffer offsets
 struct LoraArgs {
   const float* x = nullptr;
   int64_t M = 0;
@@ -138,14 +140,23 @@ struct LoraArgs {
   const int32_t* rank = nullptr;
   int slots = 0, max_rank = 0;
   const int32_t* slot_of_row = nullptr;
-  float* t = nullptr;
+  // Few rows: fp32 [M, max_rank]; many: the values' three bf16 parts [M, 3, lora_ldt].
+  void* t = nullptr;
+  int8_t* xq = nullptr;
+  float* xa = nullptr;
   int relu = 0;
   float* out = nullptr;  // [M, N]
   int* err = nullptr;    // set to 1 on a slot or rank out of range (the row then has no adapter)
 };
+constexpr int lora_ldt(int max_rank) { return (max_rank + 15) / 16 * 16; }
+// Whether M rows count as few: each row its own adapter (below), else tiles of
+// rows that mostly share one.
+bool lora_few_rows(int64_t M);
 size_t lora_scratch_bytes(int64_t M, int max_rank);
 hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s);
 hipError_t launch_lora_linear(const GemmArgs& base, const LoraArgs& g, hipStream_t s);
+// The tile GEMM with the adapters' second products in its epilogue (many rows).
+hipError_t launch_gemm_tile_lora(const GemmArgs& g, const LoraArgs& l, hipStream_t s);
 
 hipError_t launch_quantize_rows(const float* x, int64_t ldx, int rows, const int* rows_dev,
                                 int cols, int8_t* q, int64_t ldq, float* a, int* err,

@@ -318,7 +318,7 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
                               const int32_t* lora_rank, int64_t slots, int64_t max_rank,
                               const int32_t* slot_of_row, float* out_f32, void* workspace,
                               size_t workspace_bytes, int* err, void* stream) {
-  if (!lora_sizes_ok(M, K, max_rank) || N <= 0 || N > INT32_MAX || slots <= 0 || slots > INT32_MAX)
+  if (!lora_sizes_ok(M, K, max_rank) || N <= 0 || N > kLoraMaxN || slots <= 0 || slots > INT32_MAX)
     return refuse("q8_linear_lora: sizes out of range");
   if (!x || !w || !w_mult || !bias || !lora_a || !lora_b || !lora_scale || !lora_rank || !slot_of_row || !out_f32 ||
       !xq != !xa)
@@ -348,20 +348,17 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
   l.slots = (int)slots;
   l.max_rank = (int)max_rank;
   l.slot_of_row = slot_of_row;
-  l.t = (float*)workspace;
+  l.t = workspace;
   l.relu = relu;
   l.out = out_f32;
   l.err = err;
-  int8_t* q = (int8_t*)workspace + ws.codes;
-  float* a = (float*)((char*)workspace + ws.mults);
-  int rc;
   if (!xq) {
-    rc = op_status(launch_quantize_rows(x, K, (int)M, nullptr, (int)K, q, K, a, err, s), "q8_linear_lora");
-    if (rc) return rc;
-    xq = q;
-    xa = a;
+    l.xq = (int8_t*)workspace + ws.codes;
+    l.xa = (float*)((char*)workspace + ws.mults);
+    xq = l.xq;
+    xa = l.xa;
   }
-  rc = op_status(launch_lora_down(l, s), "q8_linear_lora down");
+  const int rc = op_status(launch_lora_down(l, s), "q8_linear_lora down");
   if (rc) return rc;
   GemmArgs g;
   g.A = xq;

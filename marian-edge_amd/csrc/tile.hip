@@ -5,6 +5,7 @@
 // b_n with optional ReLU, i32 copy and statically quantized copy.
 #include "device_common.h"
 #include "kernels.h"
+#include "lora_device.h"
 #include <algorithm>
 #include <type_traits>
 
@@ -12,6 +13,7 @@ namespace mh {
 namespace {
 
 typedef int v16i __attribute__((ext_vector_type(16)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------------------
 // One workgroup of WM x WN waves per BM x BN output tile, each wave a grid of
@@ -175,9 +177,83 @@ __device__ __forceinline__ void tile_store(const GemmArgs& g, const Epilogue& e,
   }
 }
 
-template <int BM, int BN, int WM, int WN, int PF, bool RELU, bool EXTRA, bool WIDE>
-__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(BM > 128 ? 2 : WM * WN / 2)))
-void k_gemm_tile(GemmArgs g, Epilogue e, int tiles_n, int tiles, int stream) {
+// tile_store of fp32 outputs with the adapters' second products added: y + B_s t,
+// t (the first products) as three bf16 parts.  v_mfma_f32_32x32x16_bf16 takes rows
+// and columns l % 32 from lane l, k 8 (l / 32) .. + 8, and its results lie where the
+// int8 blocks' do.  Each distinct slot of a block's 32 rows is one product with all
+// rows' t; rows of other slots do not take it.
+template <int BM, int MB, int NB, bool RELU>
+__device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e, const LoraArgs& l,
+                                           const v16i (&acc)[MB][NB], const float* sAm, const float (&wm)[NB],
+                                           const float (&bi)[NB], bool ok, int m0, int n0, int wr, int wc) {
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+#pragma unroll
+  for (int k = 0; k < NB; ++k) ok &= recip_factor(wm[k]);
+  ok = __all(ok);
+  const float* sm = sAm + wr + 4 * half;
+  const int rows = min(BM, g.M - m0), ldt = lora_ldt(l.max_rank);
+  const __amdgpu_buffer_rsrc_t out = tile_rows(e.out, m0 * e.ldo, e.ldo, rows, 4);
+  const uint32_t ldb = (uint32_t)e.ldo * 4;
+#pragma unroll
+  for (int i = 0; i < MB; ++i) {
+    const int r0 = m0 + wr + 32 * i, row = min(r0 + (lane & 31), g.M - 1);
+    const RowAdapter ad = row_adapter(l, r0 + (lane & 31) < g.M ? l.slot_of_row[row] : -1, nullptr);
+    const uint16_t* t = (const uint16_t*)l.t + (int64_t)row * 3 * ldt + 8 * half;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int n = n0 + wc + k * 32 + (lane & 31);
+      const uint16_t* b = l.b + (int64_t)min(n, g.N - 1) * l.max_rank;
+      float y[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 a4 = *(const float4*)(sm + i * 32 + 8 * q);
+        const float av[4] = {a4.x, a4.y, a4.z, a4.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float inv = ok ? recip_exact(av[c] * wm[k]) : dequant_scale(av[c], wm[k]);
+          y[4 * q + c] = dequant_apply(acc[i][k][4 * q + c], inv, bi[k]);
+        }
+      }
+      uint32_t todo = (uint32_t)__ballot(ad.rank > 0);
+      while (todo) {
+        const int lead = __builtin_ctz(todo);
+        const int slot = __builtin_amdgcn_readlane(ad.slot, lead), rank = __builtin_amdgcn_readlane(ad.rank, lead);
+        const uint32_t mine = (uint32_t)__ballot(ad.slot == slot && ad.rank > 0);
+        todo &= ~mine;
+        const uint16_t* bs = b + (int64_t)slot * g.N * l.max_rank;
+        v16f p;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = 0.0f;
+        for (int k0 = 0; k0 < rank; k0 += 16) {
+          const int at = k0 + 8 * half;
+          bf8 w = *(const bf8*)(bs + min(at, l.max_rank - 8));
+          if (k0 + 16 > rank) w = first_values(w, min(max(rank - at, 0), 8));
+#pragma unroll
+          for (int c = 2; c >= 0; --c)
+            p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf8*)(t + c * ldt + k0), w, p, 0, 0, 0);
+        }
+        const uint32_t m = mine >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] += (m >> (8 * (r >> 2) + (r & 3))) & 1 ? p[r] : 0.0f;
+      }
+      uint32_t off = n < g.N ? (uint32_t)(wr + 4 * half + 32 * i) * ldb + (uint32_t)n * 4 : 0x80000000u;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float v = y[4 * q + c];
+          if (RELU) v = v > 0.0f ? v : 0.0f;
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), out, off, 0, 0);
+          off += (c == 3 ? 5u : 1u) * ldb;
+        }
+    }
+  }
+}
+
+// lora_store with ADAPTERS, else tile_store.
+template <int BM, int BN, int WM, int WN, int PF, bool RELU, bool EXTRA, bool WIDE, bool ADAPTERS>
+__device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epilogue& e, int tiles_n, int tiles, int stream,
+                                          const LoraArgs& l) {
   constexpr int NT = WM * WN * 64;
   constexpr int MB = BM / WM / 32, NB = BN / WN / 32;  // 32x32 blocks per wave
   constexpr int AP = BM * 8 / NT, BP = BN * 8 / NT;    // 16-byte pieces per thread and chunk
@@ -302,10 +378,25 @@ void k_gemm_tile(GemmArgs g, Epilogue e, int tiles_n, int tiles, int stream) {
     bool ok = true;
 #pragma unroll
     for (int i = 0; i < BM; i += 64) ok &= recip_factor(sAm[tpar][i + lane]);
-    tile_store<BM, MB, NB, RELU, EXTRA, WIDE>(g, e, acc, sAm[tpar], wm, bi, ok, m0, n0, wr, wc, stream);
+    if constexpr (ADAPTERS)
+      lora_store<BM, MB, NB, RELU>(g, e, l, acc, sAm[tpar], wm, bi, ok, m0, n0, wr, wc);
+    else
+      tile_store<BM, MB, NB, RELU, EXTRA, WIDE>(g, e, acc, sAm[tpar], wm, bi, ok, m0, n0, wr, wc, stream);
     m0 = m1;
     n0 = n1;
   }
+}
+
+template <int BM, int BN, int WM, int WN, int PF, bool RELU, bool EXTRA, bool WIDE>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(BM > 128 ? 2 : WM * WN / 2)))
+void k_gemm_tile(GemmArgs g, Epilogue e, int tiles_n, int tiles, int stream) {
+  gemm_tile<BM, BN, WM, WN, PF, RELU, EXTRA, WIDE, false>(g, e, tiles_n, tiles, stream, LoraArgs{});
+}
+
+template <int BM, int BN, int WM, int WN, int PF, bool RELU>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(BM > 128 ? 2 : WM * WN / 2)))
+void k_gemm_tile_lora(GemmArgs g, Epilogue e, int tiles_n, int tiles, LoraArgs l) {
+  gemm_tile<BM, BN, WM, WN, PF, RELU, false, false, true>(g, e, tiles_n, tiles, 0, l);
 }
 
 // ---------------------------------------------------------------------------
@@ -520,6 +611,29 @@ hipError_t launch_gemm_tile(const GemmArgs& g, const Epilogue& e, hipStream_t s)
   const bool one_round = tiles(128, 128) >= 224 && tiles(128, 128) <= 256;
   if (one_round || (int64_t)g.M * g.N >= 224 * 128 * 128) return launch_tile<128, 128, 2, 4, 2>(g, e, 1 << 30, s);
   return launch_tile<64, 64, 2, 2, 2>(g, e, 1024, s);
+}
+
+namespace {
+template <int BM, int BN, int WM, int WN, int PF>
+hipError_t launch_tile_lora(const GemmArgs& g, const LoraArgs& l, int max_wgs, hipStream_t s) {
+  const int64_t tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  if (tiles > (int64_t)INT32_MAX / 2) return hipErrorInvalidValue;
+  const int grid = (int)std::min<int64_t>((tiles + 7) / 8 * 8, max_wgs);
+  Epilogue e;
+  e.out = l.out;
+  e.ldo = g.N;
+  auto kern = l.relu ? k_gemm_tile_lora<BM, BN, WM, WN, PF, true> : k_gemm_tile_lora<BM, BN, WM, WN, PF, false>;
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(WM * WN * 64), 0, s, g, e, (int)tiles_n, (int)tiles, l);
+  return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_gemm_tile_lora(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
+  if (g.K <= 0 || g.K % 64 || g.N <= 0 || g.N > kLoraMaxN || g.lda % 16) return hipErrorInvalidValue;
+  if (g.M <= 0) return hipSuccess;
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
+  if (tiles(128, 128) >= 224) return launch_tile_lora<128, 128, 2, 4, 2>(g, l, 1 << 30, s);
+  return launch_tile_lora<64, 64, 2, 2, 2>(g, l, 1024, s);
 }
 
 static int64_t f32_tiles(const GemmArgs& g, int bn) {
