@@ -514,7 +514,7 @@ hipError_t launch_cand_argmax(const CandArgs& c, hipStream_t s);
 // of them).  Settings per row, each array optional: temperature (1; 0: the
 // maximum), top_k (0: no limit), top_p (1), min_p (0); u in [0, 1).
 constexpr int kSampleMaxRows = 1 << 20;
-constexpr int kSampleMaxIds = 1 << 19;  // sums of 2^44 stay below 2^63; groups of 512 ids
+constexpr int kSampleMaxIds = 1 << 19;  // sums of 2^44 stay below 2^63; 2048 groups of 256 ids
 struct SampleArgs {
   const void* logits = nullptr;
   int64_t ld = 0;
