@@ -71,28 +71,8 @@ __device__ __forceinline__ uint64_t mass_of_steps(Octave o, const double* exp2) 
   return (uint64_t)__double_as_longlong(p + 0x1p52) & 0x000FFFFFFFFFFFFFull;
 }
 
-// DPP move that leaves 0 in the lanes it does not write.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp0(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t dpp0(uint64_t v) {
-  return ((uint64_t)dpp0<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | dpp0<CTRL, ROWS>((uint32_t)v);
-}
-// Inclusive prefix sums over the wave.
-template <class V>
-__device__ __forceinline__ V wave_scan(V v) {
-  v += dpp0<0x111, 0xF>(v);  // row_shr:1
-  v += dpp0<0x112, 0xF>(v);  // row_shr:2
-  v += dpp0<0x114, 0xF>(v);  // row_shr:4
-  v += dpp0<0x118, 0xF>(v);  // row_shr:8
-  v += dpp0<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-  v += dpp0<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
-// wave_scan of masses in 12 additions, the lanes moved by the additions themselves
-// (the compiler moves them first: 36 instructions).  A lane's result is read by the
+// Inclusive prefix sums over the wave, in 12 additions that move the lanes
+// themselves (the compiler moves them first: 36 instructions).  A lane's result is read by the
 // next step two instructions later, as the hardware asks.
 __device__ __forceinline__ uint64_t wave_scan_mass(uint64_t v) {
   uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
@@ -136,13 +116,11 @@ template <int T, int IDS>
 struct SampleLds {
   static constexpr int NW = T / 64, SEGS = (IDS ? IDS : kSampleMaxIds) / 256;
   float val[IDS ? IDS : 4];  // the row, each value written and read by one thread
-  union {
-    uint64_t mass[kBins];
-    uint32_t cnt[kBins];
-  };
+  uint64_t hist[kBins];      // masses or counts
   double exp2[32];
   uint64_t seg[SEGS];  // kept mass of every 256 consecutive ids
-  uint64_t pair[kList], weight[kList], before[kList];
+  ulonglong2 entry[kList];  // the list: pair, weight
+  uint64_t before[kList];
   uint64_t wsum[NW];
   float wmax[NW];
   int found, best;
@@ -150,21 +128,25 @@ struct SampleLds {
   uint64_t lo, hi, found_before, border;
 };
 
-// The first of h's kBins at which the running sum reaches need(sum of all), and
-// the running sum before it; bin -1: none.  Called with h complete (a barrier
-// before); on return h may be written again.
+// The first of the kBins of L.hist at which the running sum reaches need(sum of
+// all), and the running sum before it; bin -1: none.  Called with the histogram
+// complete but for a barrier; it is zero again on return, but for a barrier.
 struct Found {
   int bin;
   uint64_t before, total;
 };
-template <int T, class Lds, class V, class Need>
-__device__ __forceinline__ Found locate(Lds& L, const V* h, Need&& need_of) {
+template <int T, class Lds, class Need>
+__device__ __forceinline__ Found locate(Lds& L, Need&& need_of) {
   constexpr int B = kBins / T, NW = T / 64;
   const int t = threadIdx.x, w = t >> 6;
-  V c[B];
+  wg_lds_barrier();
+  uint64_t c[B];
 #pragma unroll
-  for (int i = 0; i < B; ++i) c[i] = h[t * B + i] + (i ? c[i - 1] : (V)0);
-  uint64_t s = wave_scan(c[B - 1]);
+  for (int i = 0; i < B; ++i) {
+    c[i] = L.hist[t * B + i] + (i ? c[i - 1] : 0ull);
+    L.hist[t * B + i] = 0;
+  }
+  uint64_t s = wave_scan_mass(c[B - 1]);
   if ((t & 63) == 63) L.wsum[w] = s;
   if (t == 0) {
     L.found = -1;
@@ -184,7 +166,7 @@ __device__ __forceinline__ Found locate(Lds& L, const V* h, Need&& need_of) {
   const uint64_t need = need_of(total);
 #pragma unroll
   for (int i = 0; i < B; ++i) {
-    const uint64_t before = s + (i ? c[i - 1] : (V)0);
+    const uint64_t before = s + (i ? c[i - 1] : 0ull);
     if (before < need && need <= s + c[i]) {
       L.found = t * B + i;
       L.found_before = before;
@@ -194,27 +176,15 @@ __device__ __forceinline__ Found locate(Lds& L, const V* h, Need&& need_of) {
   return {__builtin_amdgcn_readfirstlane(L.found), L.found_before, total};
 }
 
-// Sum over the workgroup; two barriers.
-template <int T, class Lds>
-__device__ __forceinline__ uint64_t block_sum(Lds& L, uint64_t v) {
-  v = wave_scan(v);
-  wg_lds_barrier();  // earlier sums are read
-  if ((threadIdx.x & 63) == 63) L.wsum[threadIdx.x >> 6] = v;
-  wg_lds_barrier();
-  uint64_t s = 0;
-#pragma unroll
-  for (int i = 0; i < T / 64; ++i) s += L.wsum[i];
-  return s;
-}
-
 // One workgroup of T threads per row.  Thread t holds ids 4(jT + t) + c, so that
-// a wave's 256 values of one j are consecutive ids: the final draw sums those,
-// finds the group that the number falls into, and one wave scans its 256.  A row
-// of up to IDS ids is read from memory once and kept in LDS, each thread its own
-// values; IDS = 0: each pass reads memory again.  One compute unit works on a row,
-// so instructions per id and pass are what bounds it, and the passes are rolled
-// loops: unrolled (values and masses in registers) they outgrow the instruction
-// cache and took longer.
+// a wave's 256 values of one j (a slot) are consecutive ids: the final draw sums
+// those, finds the group that the number falls into, and one wave scans its 256.
+// A row of up to IDS ids is read from memory once and kept in LDS, each thread its
+// own values; IDS = 0: each pass reads memory again.  One compute unit works on a
+// row, so instructions per id and pass are what bounds it, and, as every
+// instruction is fetched once per row, the size of the code: the passes are rolled
+// loops and the stages below share one piece of code (unrolled, with values
+// and masses in registers, they took half as long again).
 //
 // Few ids to draw from (at most kList ids in the row, or a top-k of which at most
 // kList ids can be part): all of them in a list, compared pairwise.  The k-th
@@ -226,6 +196,8 @@ __device__ __forceinline__ uint64_t block_sum(Lds& L, uint64_t v) {
 // every id of that bin against every other.  A bin of more than kList ids (many
 // equal logits) is cut again by (logit, id) pairs, kBins ways a time, until few
 // are left.
+enum Stage { LIST_ALL, LIST_TOP, BORDER_K, BORDER_P, DRAW, DRAWN };
+
 template <int T, int IDS, bool BF16>
 __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   constexpr int NW = T / 64, NJ = IDS / (4 * T);  // slots of four ids per thread
@@ -264,40 +236,36 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     return;
   }
 
-  // ---- the row's values at ids 4 slot + c: -inf for NaN and past the row ----
+  // ---- the row's values: -inf for NaN and past the row ----
+  // Of this wave's slots, `full` lie inside the row and `slots` begin there.
+  const int w0 = 256 * wave;
+  const int full = n >= w0 + 256 ? (n - w0 - 256) / (4 * T) + 1 : 0, slots = n > w0 ? (n - w0 - 1) / (4 * T) + 1 : 0;
   bool only_inf = false;  // the maximum is infinite: those ids alone, as if of logit 0
-  auto load4 = [&](int slot) -> f4v {  // as stored; the row's last values once more past it
+  auto value = [&](int id) -> float { return BF16 ? bf16_to_f32(((const uint16_t*)base)[id]) : ((const float*)base)[id]; };
+  auto load4 = [&](int j) -> f4v {  // a slot inside the row
     f4v v;
-    if (n >= 4) {
-      const int at = min(4 * slot, n - 4);
-      if constexpr (BF16) {
-        const h4u h = *(const h4u*)((const uint16_t*)base + at);
+    if constexpr (BF16) {
+      const h4u h = *(const h4u*)((const uint16_t*)base + 4 * (j * T + t));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = bf16_to_f32(h[c]);
-      } else {
-        const f4u f = *(const f4u*)((const float*)base + at);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = f[c];
-      }
+      for (int c = 0; c < 4; ++c) v[c] = bf16_to_f32(h[c]);
     } else {
+      const f4u f = *(const f4u*)((const float*)base + 4 * (j * T + t));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int at = min(c, n - 1);
-        v[c] = BF16 ? bf16_to_f32(((const uint16_t*)base)[at]) : ((const float*)base)[at];
-      }
+      for (int c = 0; c < 4; ++c) v[c] = f[c];
     }
     return v;
   };
-  auto clean4 = [&](int slot, f4v v) -> f4v {
-    if (__any(4 * slot + 4 > n)) {  // the row's end is inside or before this slot
-      const int sh = n >= 4 ? max(0, 4 * slot - (n - 4)) : 0;
-      const float v1 = v[1], v2 = v[2], v3 = v[3];
-      v[0] = sh == 0 ? v[0] : sh == 1 ? v1 : sh == 2 ? v2 : v3;
-      v[1] = sh == 0 ? v1 : sh == 1 ? v2 : v3;
-      v[2] = sh == 0 ? v2 : v3;
+  auto last4 = [&](int j) -> f4v {  // the slot that the row ends in
+    f4v v;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = 4 * slot + c < n ? v[c] : -INFINITY;
+    for (int c = 0; c < 4; ++c) {
+      const int id = 4 * (j * T + t) + c;
+      v[c] = value(min(id, n - 1));
+      v[c] = id < n ? v[c] : -INFINITY;
     }
+    return v;
+  };
+  auto clean = [&](f4v v) -> f4v {
 #pragma unroll
     for (int c = 0; c < 4; ++c) v[c] = fmaxf(v[c], -INFINITY);
     if (only_inf) {
@@ -306,26 +274,34 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     }
     return v;
   };
-  const int nj = (n + 4 * T - 1) / (4 * T);
-  // f(j, first id, four values) for every slot of this thread, from memory with
-  // BATCH loads in flight.
+  // f(j, first id, four values) for this thread's slots, from memory, the next
+  // BATCH slots requested before BATCH are worked on.
   auto each_read = [&](auto&& f) {
     constexpr int BATCH = IDS ? NJ : 4;
-    for (int j0 = 0; j0 < nj; j0 += BATCH) {
-      f4v v[BATCH];
+    if (full > 0) {
+      f4v v[BATCH], next[BATCH];
 #pragma unroll
-      for (int b = 0; b < BATCH; ++b) v[b] = load4((j0 + b) * T + t);
+      for (int b = 0; b < BATCH; ++b) v[b] = load4(min(b, full - 1));
+      for (int j0 = 0; j0 < full; j0 += BATCH) {
+        if constexpr (IDS == 0) {
 #pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        if (j0 + b >= nj) break;
-        f(j0 + b, 4 * ((j0 + b) * T + t), clean4((j0 + b) * T + t, v[b]));
+          for (int b = 0; b < BATCH; ++b) next[b] = load4(min(j0 + BATCH + b, full - 1));
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+          if (j0 + b < full) f(j0 + b, 4 * ((j0 + b) * T + t), clean(v[b]));
+        if constexpr (IDS == 0) {
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) v[b] = next[b];
+        }
       }
     }
+    if (slots > full) f(full, 4 * (full * T + t), clean(last4(full)));
   };
   auto each = [&](auto&& f) {
     if constexpr (IDS > 0) {
 #pragma unroll 1
-      for (int j = 0; j < nj; ++j) f(j, 4 * (j * T + t), *(const f4v*)(L.val + 4 * (j * T + t)));
+      for (int j = 0; j < slots; ++j) f(j, 4 * (j * T + t), *(const f4v*)(L.val + 4 * (j * T + t)));
     } else {
       each_read(f);
     }
@@ -341,9 +317,13 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     const float m = wave_max(tmax);
     if (lane == 0) L.wmax[wave] = m;
   }
-  if (t == 0) L.best = 0x7FFFFFFF;
+  if (t == 0) {
+    L.best = 0x7FFFFFFF;
+    L.listed = 0;
+  }
   if (t < 32) L.exp2[t] = kExp2[t];
-  for (int b = t; b < kBins; b += T) L.mass[b] = 0;
+  for (int b = t; b < kBins; b += T) L.hist[b] = 0;
+  for (int s = t; s < SampleLds<T, IDS>::SEGS; s += T) L.seg[s] = 0;
   wg_lds_barrier();
   float lmax = L.wmax[0];
 #pragma unroll
@@ -354,7 +334,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   }
   if (!valid || temp == 0.0f || top_k == 1 || top_p == 0.0f) {  // the maximum's lowest id
     int best = 0x7FFFFFFF;
-    if (tmax == lmax)
+    if (__any(tmax == lmax))
       each([&](int, int i, f4v v) {
 #pragma unroll
         for (int c = 3; c >= 0; --c) best = v[c] == lmax ? min(best, i + c) : best;
@@ -391,9 +371,6 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   auto need_u = [&](uint64_t total) -> uint64_t {
     return __umul64hi(total, (uint64_t)(uint32_t)(u * 0x1p32f) << 32) + 1;
   };
-  auto share = [&](float v, uint64_t total) -> float {
-    return (float)(octave(v) * 0.6931471805599453 - log(ldexp((double)total, -kMassBits)));
-  };
   const bool by_k = top_k > 0 && top_k < n, by_p = top_p < 1.0f;
   // The least logit that min-p keeps, by its order key: steps of 1, 2, 4 ... from
   // where rounding apart it should be, then halves of what the last one jumped over.
@@ -420,101 +397,9 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     least_v = order_logit((uint32_t)hi);
   }
 
-  // Adds ids of bins [first, last] with pairs in [lo, hi] to the list, as long as it has room.
-  auto gather = [&](int first, int last, uint64_t lo, uint64_t hi, bool range, auto&& also) {
-    const float least = least_of(last), most = first ? most_of(first) : INFINITY;
-    each([&](int, int i, f4v v) {
-      bool in[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) in[c] = (v[c] >= least) & (v[c] <= most);
-      if (!__any((in[0] | in[1]) | (in[2] | in[3]))) return;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (!in[c]) continue;
-        const int b = bin_of(v[c]);
-        if (b < first || b > last || !also(v[c], i + c)) continue;
-        const uint64_t p = pair_of(v[c], (uint32_t)(i + c));
-        if (p < lo || p > hi) continue;
-        const uint32_t at = lds_add(&L.listed, 1u);
-        if (at < (uint32_t)kList) L.pair[at] = p;
-        if (range) {
-          __hip_atomic_fetch_min(&L.lo, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          __hip_atomic_fetch_max(&L.hi, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
-      }
-    });
-    wg_lds_barrier();
-  };
-  // For the list's entry of this thread's place (t % kList): the sum of weight over
-  // the entries that come before it, in L.before.  T / kList groups of threads share
-  // the entries.  The weights are complete but for a barrier, and the sums on return.
-  auto sum_before = [&](uint32_t listed, auto&& comes_before) {
-    if (t < kList) L.before[t] = 0;
-    wg_lds_barrier();
-    const uint32_t at = t % kList;
-    if (at < listed) {
-      uint64_t s = 0;
-#pragma unroll 4
-      for (uint32_t i = t / kList; i < listed; i += T / kList) s += comes_before(L.pair[i]) ? L.weight[i] : 0ull;
-      if (s) lds_add(&L.before[at], s);
-    }
-    wg_lds_barrier();
-  };
-
-  // ---- few ids: a list of them ----
-  bool few = n <= kList;
-  if (few || (by_k && top_k <= kList * 3 / 4)) {
-    int last = kLastBin;
-    if (few) {
-      if (t == 0) L.listed = 0;
-      wg_lds_barrier();
-    } else {
-      const int b = bin_of(tmax);
-      if (b <= kLastBin) lds_add(&L.cnt[b], 1u);
-      wg_lds_barrier();
-      const Found f = locate<T>(L, L.cnt, [&](uint64_t) { return (uint64_t)top_k; });
-      for (int z = t; z < kBins; z += T) L.mass[z] = 0;
-      few = f.bin >= 0;
-      last = f.bin;
-    }
-    if (few) {
-      gather(0, last, 0, ~0ull, false, [](float, int) { return true; });
-      few = L.listed <= (uint32_t)kList;
-    }
-    if (few) {
-      const uint32_t listed = L.listed, at = t % kList;
-      const uint64_t mine = L.pair[min(at, listed - 1)];
-      const bool own = t < (int)listed;  // one thread per entry
-      const float v = pair_logit(mine);
-      const uint64_t m = own ? mass_of(v) : 0ull;
-      bool keep = own;
-      if (by_k) {
-        if (own) L.weight[t] = 1;
-        sum_before(listed, [&](uint64_t p) { return p > mine; });
-        keep = own && L.before[at] < (uint64_t)top_k;
-        wg_lds_barrier();
-      }
-      if (by_p) {
-        if (own) L.weight[t] = keep ? m : 0ull;
-        const uint64_t need = need_p(block_sum<T>(L, keep ? m : 0ull));
-        sum_before(listed, [&](uint64_t p) { return p > mine; });
-        keep = keep && L.before[at] < need;
-        wg_lds_barrier();
-      }
-      keep = keep && v >= least_v;
-      if (own) L.weight[t] = keep ? m : 0ull;
-      const uint64_t total = block_sum<T>(L, keep ? m : 0ull), need = need_u(total);
-      sum_before(listed, [&](uint64_t p) { return (uint32_t)p > (uint32_t)mine; });  // lower ids
-      if (keep && L.before[at] < need && need <= L.before[at] + m) finish(pair_id(mine), share(v, total));
-      return;
-    }
-    wg_lds_barrier();
-  }
-
-  // ---- the borders: ids kept are those at or before (border_v, border_id) ----
+  // Ids kept are those at or before (border_v, border_id).
   float border_v = -INFINITY;
   int border_id = 0x7FFFFFFF;
-  auto kept = [&](float v, int id) -> bool { return (v > border_v) | ((v == border_v) & (id <= border_id)); };
   // f(j, octaves and masses of the kept ids), for every slot; slots without any are left out
   auto each_mass = [&](auto&& f) {
     const bool all = border_v == -INFINITY;
@@ -545,136 +430,225 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     });
   };
 
-  // top-k, then top-p: one piece of code for both.
+  int drawn = -1;  // in the thread that holds it: the id, its logit, the kept mass
+  float drawn_v = 0.0f;
+  uint64_t drawn_of = 0;
+  int stage = n <= kList ? LIST_ALL : !by_k ? (by_p ? BORDER_P : DRAW) : top_k <= kList * 3 / 4 ? LIST_TOP : BORDER_K;
 #pragma unroll 1
-  for (int stage = by_k ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
-    const bool count = stage == 0;
-    auto need_of = [&](uint64_t total) { return count ? (uint64_t)top_k : need_p(total); };
-    Found f;
-    if (count) {
-      each([&](int, int, f4v v) {
+  while (stage < DRAW) {
+    // ---- the list: of the stage's bins, of a part of one when it is crowded ----
+    int first = 0, last = kLastBin, shift = -1;  // shift: of a part's number
+    uint64_t need = 0, lo = 0, hi = ~0ull;       // pairs looked at
+#pragma unroll 1
+    for (;;) {
+      if (stage != LIST_ALL) {
+        if (shift >= 0) {
+          each([&](int, int i, f4v v) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int b = bin_of(v[c]);
-          if (b <= kLastBin) lds_add(&L.cnt[b], 1u);
+            for (int c = 0; c < 4; ++c) {
+              const uint64_t p = pair_of(v[c], (uint32_t)(i + c));
+              if (p >= lo && p <= hi) lds_add(&L.hist[(hi - p) >> shift], stage == BORDER_P ? mass_of(v[c]) : (uint64_t)1);
+            }
+          });
+        } else if (stage == LIST_TOP) {
+          const int b = bin_of(tmax);
+          if (b <= kLastBin) lds_add(&L.hist[b], (uint64_t)1);
+        } else if (stage == BORDER_K) {
+          each([&](int, int, f4v v) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int b = bin_of(v[c]);
+              if (b <= kLastBin) lds_add(&L.hist[b], (uint64_t)1);
+            }
+          });
+        } else {
+          each_mass([&](int, const Octave (&o)[4], const uint64_t (&m)[4]) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (m[c]) lds_add(&L.hist[-o[c].steps], m[c]);
+          });
         }
-      });
-      wg_lds_barrier();
-      f = locate<T>(L, L.cnt, need_of);
-    } else {
-      each_mass([&](int, const Octave (&o)[4], const uint64_t (&m)[4]) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (m[c]) lds_add(&L.mass[-o[c].steps], m[c]);
-      });
-      wg_lds_barrier();
-      f = locate<T>(L, L.mass, need_of);
-    }
-    for (int b = t; b < kBins; b += T) L.mass[b] = 0;  // for the next histogram
-    if (f.bin < 0) {  // fewer ids with mass than the count asks for
-      wg_lds_barrier();
-      continue;
-    }
-    uint64_t need = need_of(f.total) - f.before;  // within the bin
-    auto weigh = [&](float v) -> uint64_t { return count ? 1ull : mass_of(v); };
-    gather(f.bin, f.bin, 0, ~0ull, true, kept);
-    if (L.listed > (uint32_t)kList) {
-      uint64_t lo = L.lo, hi = L.hi;
-      do {  // kBins parts of [lo, hi] at a time: a part of one pair at the end
-        const uint64_t span = hi - lo;
-        const int shift = max(0, 64 - 11 - __builtin_clzll(span | 1));
+        const Found f = locate<T>(L, [&](uint64_t total) {
+          return shift >= 0 ? need : stage == BORDER_P ? need_p(total) : (uint64_t)top_k;
+        });
+        if (shift >= 0) {
+          hi -= (uint64_t)f.bin << shift;
+          lo = umax64(lo, hi - ((1ull << shift) - 1));
+        } else {
+          need = stage == BORDER_P ? need_p(f.total) : (uint64_t)top_k;
+          last = f.bin;
+          first = stage == LIST_TOP ? 0 : f.bin;
+        }
+        need -= f.before;
+      }
+      if (last >= 0) {
+        const float least = least_of(last), most = first ? most_of(first) : INFINITY;
         each([&](int, int i, f4v v) {
+          bool in[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) in[c] = (v[c] >= least) & (v[c] <= most);
+          if (!__any((in[0] | in[1]) | (in[2] | in[3]))) return;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
+            if (!in[c]) continue;
+            const int b = bin_of(v[c]);
             const uint64_t p = pair_of(v[c], (uint32_t)(i + c));
-            if (p >= lo && p <= hi) lds_add(&L.mass[(hi - p) >> shift], weigh(v[c]));
+            if (b < first || b > last || p < lo || p > hi || p < pair_of(border_v, (uint32_t)border_id)) continue;
+            const uint32_t at = lds_add(&L.listed, 1u);
+            if (at < (uint32_t)kList) L.entry[at].x = p;
+            if (shift < 0 && stage >= BORDER_K) {  // the range of all, should they be too many
+              __hip_atomic_fetch_min(&L.lo, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+              __hip_atomic_fetch_max(&L.hi, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
           }
         });
-        wg_lds_barrier();
-        const Found z = locate<T>(L, L.mass, [&](uint64_t) { return need; });
-        need -= z.before;
-        hi -= (uint64_t)z.bin << shift;
-        lo = umax64(lo, hi - ((1ull << shift) - 1));
-        for (int b = t; b < kBins; b += T) L.mass[b] = 0;
-        gather(f.bin, f.bin, lo, hi, false, kept);
-      } while (L.listed > (uint32_t)kList);
+      }
+      wg_lds_barrier();
+      if (last < 0 || L.listed <= (uint32_t)kList || stage == LIST_TOP) break;
+      if (shift < 0) {
+        lo = L.lo;
+        hi = L.hi;
+      }
+      shift = max(0, 64 - 11 - __builtin_clzll((hi - lo) | 1));  // kBins parts of [lo, hi]
     }
-    const uint32_t listed = L.listed, at = t % kList;
-    const uint64_t mine = L.pair[min(at, listed - 1)];
-    uint64_t w = 0;
-    if (t < (int)listed) {
-      w = weigh(pair_logit(mine));
-      L.weight[t] = w;
+    const uint32_t listed = L.listed;
+    if (last < 0 || listed > (uint32_t)kList) {  // too few ids with mass for top_k, too many for the list
+      stage = stage == LIST_TOP ? BORDER_K : by_p ? BORDER_P : DRAW;
+      continue;
     }
-    sum_before(listed, [&](uint64_t p) { return p > mine; });
-    if (t < (int)listed && L.before[at] < need && need <= L.before[at] + w) L.border = mine;
-    wg_lds_barrier();
-    border_v = pair_logit(L.border);
-    border_id = pair_id(L.border);
+
+    // ---- its entries against each other: 64, 128 or 256 threads take one entry each, and
+    // as many groups of them as there are share the comparisons ----
+    const int lg = listed <= 64 ? 6 : listed <= 128 ? 7 : 8;
+    static_assert(kList == 256, "groups of up to 256 threads");
+    const uint32_t at = t & ((1 << lg) - 1), groups = T >> lg;
+    const uint64_t mine = L.entry[min(at, listed - 1)].x;
+    const float v = pair_logit(mine);
+    const uint64_t m = mass_of(v);
+    const bool own = t < (int)listed;  // one thread per entry
+    bool keep = own, hit = false;
+    int pass = stage == BORDER_P || (stage == LIST_ALL && !by_k) ? 1 : 0;  // 0: count, 1: mass, 2: draw
+    const int end = stage >= BORDER_K ? pass : 2;
+#pragma unroll 1
+    for (; pass <= end; ++pass) {
+      if (pass == 1 && !by_p) continue;
+      if (pass == 2) keep = keep && v >= least_v;
+      const uint64_t w = !keep ? 0ull : pass ? m : 1ull;
+      const uint64_t ws = wave_scan_mass(w);
+      if (lane == 63) L.wsum[wave] = ws;
+      if (own) L.entry[t].y = w;
+      if (t < kList) L.before[t] = 0;
+      wg_lds_barrier();
+      uint64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < kList / 64; ++i) sum += L.wsum[i];
+      if (stage < BORDER_K) need = pass == 0 ? (uint64_t)top_k : pass == 1 ? need_p(sum) : need_u(sum);
+      const uint64_t mask = pass == 2 ? 0xFFFFFFFFull : ~0ull;  // the draw goes by id alone
+      if (at < listed) {
+        uint64_t s = 0;
+#pragma unroll 4
+        for (uint32_t i = t >> lg; i < listed; i += groups) {
+          const ulonglong2 e = L.entry[i];
+          s += (e.x & mask) > (mine & mask) ? e.y : 0ull;
+        }
+        if (s) lds_add(&L.before[at], s);
+      }
+      wg_lds_barrier();
+      const uint64_t before = L.before[at];
+      hit = keep && before < need && need <= before + w;  // the sum reaches need here
+      keep = keep && before < need;
+      drawn_of = sum;
+      wg_lds_barrier();
+    }
+    if (stage < BORDER_K) {
+      if (hit) {
+        drawn = pair_id(mine);
+        drawn_v = v;
+      }
+      stage = DRAWN;
+    } else {
+      if (hit) L.border = mine;
+      wg_lds_barrier();
+      border_v = pair_logit(L.border);
+      border_id = pair_id(L.border);
+      stage = stage == BORDER_K && by_p ? BORDER_P : DRAW;
+    }
   }
 
   // ---- the draw: kept mass of every 256 consecutive ids, then one id ----
-  if (least_v > border_v) {
-    border_v = least_v;
-    border_id = 0x7FFFFFFF;
-  }
-  for (int b = t; b < (IDS ? nj * NW : kBins); b += T) L.seg[b] = 0;
-  wg_lds_barrier();
-  each_mass([&](int j, const Octave (&)[4], const uint64_t (&m)[4]) {
-    const uint64_t s = wave_scan_mass((m[0] + m[1]) + (m[2] + m[3]));
-    if (lane == 63) L.seg[j * NW + wave] = s;
-  });
-  wg_lds_barrier();
-  int seg = -1;
-  uint64_t before = 0, total;
-  if constexpr (IDS > 0) {  // each wave finds the group by itself
-    constexpr int PER = (SampleLds<T, IDS>::SEGS + 63) / 64;
-    const int segs = nj * NW;
-    uint64_t c[PER];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int s = lane * PER + k;
-      c[k] = (s < segs ? L.seg[s] : 0ull) + (k ? c[k - 1] : 0ull);
+  if (stage == DRAW) {
+    if (least_v > border_v) {
+      border_v = least_v;
+      border_id = 0x7FFFFFFF;
     }
-    const uint64_t upto = wave_scan(c[PER - 1]);
-    total = lane_u64(upto, 63);
-    const uint64_t need = need_u(total);
+    each_mass([&](int j, const Octave (&)[4], const uint64_t (&m)[4]) {
+      const uint64_t s = wave_scan_mass((m[0] + m[1]) + (m[2] + m[3]));
+      if (lane == 63) L.seg[j * NW + wave] = s;
+    });
+    wg_lds_barrier();
+    // Each wave finds the group by itself, 64 PER sums at a time.
+    constexpr int PER = IDS ? (SampleLds<T, IDS>::SEGS + 63) / 64 : 8;
+    const int segs = (n + 255) / 256;
+    uint64_t total = 0, before = 0, need = 0;
+    int seg = -1;
+#pragma unroll 1
+    for (int find = 0; find < 2; ++find) {
+      uint64_t run = 0;
+#pragma unroll 1
+      for (int s0 = 0; s0 < segs && seg < 0; s0 += 64 * PER) {
+        uint64_t c[PER];
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const uint64_t b = upto - c[PER - 1] + (k ? c[k - 1] : 0ull);
-      const uint64_t who = __ballot(b < need && need <= upto - c[PER - 1] + c[k]);
-      if (who) {
-        seg = __builtin_ctzll(who) * PER + k;
-        before = lane_u64(b, __builtin_ctzll(who));
+        for (int k = 0; k < PER; ++k) {
+          const int s = s0 + lane * PER + k;
+          c[k] = (s < segs ? L.seg[s] : 0ull) + (k ? c[k - 1] : 0ull);
+        }
+        const uint64_t upto = run + wave_scan_mass(c[PER - 1]);
+        if (find) {
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const uint64_t b = upto - c[PER - 1] + (k ? c[k - 1] : 0ull);
+            const uint64_t who = __ballot(b < need && need <= upto - c[PER - 1] + c[k]);
+            if (who) {
+              seg = s0 + __builtin_ctzll(who) * PER + k;
+              before = lane_u64(b, __builtin_ctzll(who));
+            }
+          }
+        }
+        run = lane_u64(upto, 63);
+      }
+      if (!find) {
+        total = run;
+        need = need_u(total);
       }
     }
-  } else {
-    const Found f = locate<T>(L, L.seg, need_u);
-    seg = f.bin;
-    before = f.before;
-    total = f.total;
-  }
-  if (wave == seg % NW) {  // the wave that holds the group
-    const int slot = seg * 64 + lane;
-    f4v v;
-    if constexpr (IDS > 0)
-      v = *(const f4v*)(L.val + 4 * slot);
-    else
-      v = clean4(slot, load4(slot));
-    uint64_t m[4];
+    if (wave == seg % NW) {  // the wave that holds the group
+      const int j = seg / NW, i = 4 * (j * T + t);
+      f4v v;
+      if constexpr (IDS > 0)
+        v = *(const f4v*)(L.val + i);
+      else
+        v = clean(j < full ? load4(j) : last4(j));
+      uint64_t m[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      v[c] = kept(v[c], 4 * slot + c) ? v[c] : -INFINITY;
-      m[c] = mass_of(v[c]);
-    }
-    const uint64_t own = m[0] + m[1] + m[2] + m[3], need = need_u(total);
-    uint64_t run = before + wave_scan(own) - own;
+      for (int c = 0; c < 4; ++c) {
+        const bool in = (v[c] > border_v) | ((v[c] == border_v) & (i + c <= border_id));
+        m[c] = in ? mass_of(v[c]) : 0ull;
+      }
+      const uint64_t own = (m[0] + m[1]) + (m[2] + m[3]);
+      uint64_t run = before + wave_scan_mass(own) - own;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (run < need && need <= run + m[c]) finish(4 * slot + c, share(v[c], total));
-      run += m[c];
+      for (int c = 0; c < 4; ++c) {
+        if (run < need && need <= run + m[c]) {
+          drawn = i + c;
+          drawn_v = v[c];
+        }
+        run += m[c];
+      }
+      drawn_of = total;
     }
   }
+  if (drawn >= 0)
+    finish(drawn, (float)(octave(drawn_v) * 0.6931471805599453 - log(ldexp((double)drawn_of, -kMassBits))));
 }
 
 template <int T, int IDS>
