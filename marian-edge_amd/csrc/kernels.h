@@ -140,7 +140,7 @@ struct LoraArgs {
   const int32_t* rank = nullptr;
   int slots = 0, max_rank = 0;
   const int32_t* slot_of_row = nullptr;
-  // Few rows: fp32 [M, max_rank]; many: the values' three bf16 parts [M, 3, lora_ldt].
+  // Few rows: fp32 [M, max_rank]; many: the values' three bf16 parts in operand order.
   void* t = nullptr;
   int8_t* xq = nullptr;
   float* xa = nullptr;

@@ -260,81 +260,112 @@ __global__ __launch_bounds__(NW * 64) void k_lora_rows(GemmArgs g, LoraArgs l) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows, first product: 16 rows per workgroup, its four waves split K in
+// Many rows, first product: 16 rows per workgroup, its eight waves split K in
 // chunks of 32, RT tiles of 16 ranks.  v_mfma_f32_16x16x32_bf16: lane l holds k
 // 8 (l / 16) .. + 8 of x's row l % 16 and of A's row l % 16, and of the result
-// column (rank) l % 16, rows 4 (l / 16) + r.
+// column (rank) l % 16, rows 4 (l / 16) + r.  A wave reads and splits its x once, 512
+// columns of the row at a time, and multiplies it with each slot of the tile.
 // ---------------------------------------------------------------------------
 constexpr int kDownRows = 16;
+constexpr int kDownWaves = 8;
+constexpr int kDownChunks = 2;  // chunks of a wave held at once
 
 template <int RT>
-__global__ __launch_bounds__(256) void k_lora_down_tile(LoraArgs g) {
+__global__ __launch_bounds__(kDownWaves * 64) void k_lora_down_tile(LoraArgs g) {
   touch_kernargs<sizeof(LoraArgs)>();
   constexpr int LDS_LD = 16 * RT + 1;
-  __shared__ float sT[4][kDownRows * LDS_LD];
+  __shared__ float sT[kDownWaves][kDownRows * LDS_LD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t m0 = (int64_t)blockIdx.x * kDownRows;
   const int K = g.K, kq = 8 * (lane >> 4), chunks = K >> 5;
   const int64_t row = m0 + (lane & 15) < g.M ? m0 + (lane & 15) : g.M - 1;
   const float* x = g.x + row * K + kq;
+  f4v x0[kDownChunks], x1[kDownChunks];
+  auto load_x = [&](int c0) {  // past K: the last chunk again
+#pragma unroll
+    for (int u = 0; u < kDownChunks; ++u) {
+      const int c = min(c0 + kDownWaves * u, chunks - 1);
+      x0[u] = *(const f4v*)(x + 32 * c);
+      x1[u] = *(const f4v*)(x + 32 * c + 4);
+    }
+  };
+  load_x(wave);
   const RowAdapter ad = row_adapter(g, m0 + (lane & 15) < g.M ? g.slot_of_row[row] : -1, g.err);
+  const uint32_t with = (uint32_t)__ballot(ad.rank > 0) & 0xFFFFu;  // rows with an adapter
   f4v sum[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) sum[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-  uint32_t todo = (uint32_t)__ballot(ad.rank > 0) & 0xFFFFu;
-  while (todo) {  // the tile's slots, one after another
-    const int lead = __builtin_ctz(todo);
-    const int slot = __builtin_amdgcn_readlane(ad.slot, lead), rank = __builtin_amdgcn_readlane(ad.rank, lead);
-    const uint32_t mine = (uint32_t)__ballot(ad.slot == slot && ad.rank > 0) & 0xFFFFu;
-    todo &= ~mine;
-    const uint16_t* a[RT];
+  for (int c0 = wave; with && c0 < chunks; c0 += kDownWaves * kDownChunks) {
+    bf8 p[kDownChunks][3];
+    for (uint32_t todo = with; todo;) {  // the tile's slots, one after another
+      const int lead = __builtin_ctz(todo);
+      const int slot = __builtin_amdgcn_readlane(ad.slot, lead), rank = __builtin_amdgcn_readlane(ad.rank, lead);
+      const uint32_t mine = (uint32_t)__ballot(ad.slot == slot && ad.rank > 0) & 0xFFFFu;
+      const uint16_t* a = g.a + (int64_t)slot * g.max_rank * K + kq;
+      f4v acc[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-      a[t] = g.a + ((int64_t)slot * g.max_rank + min(16 * t + (lane & 15), rank - 1)) * K + kq;
-    f4v acc[RT];
+      for (int t = 0; t < RT; ++t) acc[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+      // At most eight weight operands in flight.
+      constexpr int AT = RT > 8 / kDownChunks ? 8 / kDownChunks : RT;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) acc[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = wave; c < chunks; c += 4) {
-      const f4v x0 = *(const f4v*)(x + 32 * c), x1 = *(const f4v*)(x + 32 * c + 4);
-      bf8 w[RT];
+      for (int t0 = 0; t0 < RT; t0 += AT) {
+        bf8 w[kDownChunks][AT];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) w[t] = *(const bf8*)(a[t] + 32 * c);
-      bf8 p[3];
-      split3(x0, x1, p);
+        for (int u = 0; u < kDownChunks; ++u)
+#pragma unroll
+          for (int t = 0; t < AT; ++t)
+            w[u][t] = *(const bf8*)(a + (int64_t)min(16 * (t0 + t) + (lane & 15), rank - 1) * K +
+                                    32 * min(c0 + kDownWaves * u, chunks - 1));
+        if (t0 == 0 && todo == with) {
+#pragma unroll
+          for (int u = 0; u < kDownChunks; ++u) split3(x0[u], x1[u], p[u]);
+          if (c0 + kDownWaves * kDownChunks < chunks) load_x(c0 + kDownWaves * kDownChunks);
+        }
+#pragma unroll
+        for (int u = 0; u < kDownChunks; ++u)
+          if (c0 + kDownWaves * u < chunks)  // uniform
+#pragma unroll
+            for (int t = 0; t < AT; ++t)
+#pragma unroll
+              for (int i = 2; i >= 0; --i)
+                acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[u][i], w[u][t], acc[t0 + t], 0, 0, 0);
+      }
+      const float gain = g.scale[slot];
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int i = 2; i >= 0; --i) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[i], w[t], acc[t], 0, 0, 0);
+        for (int r = 0; r < 4; ++r)
+          if (((mine >> (4 * (lane >> 4) + r)) & 1) && 16 * t + (lane & 15) < rank)
+            sum[t][r] += acc[t][r] * gain;
+      todo &= ~mine;
     }
-    const float gain = g.scale[slot];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (((mine >> (4 * (lane >> 4) + r)) & 1) && 16 * t + (lane & 15) < rank) sum[t][r] = acc[t][r] * gain;
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) sT[wave][(4 * (lane >> 4) + r) * LDS_LD + 16 * t + (lane & 15)] = sum[t][r];
   wg_lds_barrier();
-  const int ldt = 16 * RT;
-  for (int i = tid; i < kDownRows * ldt / 2; i += 256) {
-    const int r = i / (ldt / 2), c = i % (ldt / 2) * 2;
-    float v[2];
+  // Eight ranks of a row per thread: the waves' sums, split, one 16-byte store a part.
+  const int ldt = lora_ldt(g.max_rank);
+  for (int i = tid; i < kDownRows * 2 * RT; i += kDownWaves * 64) {
+    const int r = i % kDownRows, c = i / kDownRows * 8;
+    if (c >= ldt) break;
+    f4v v[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 8; ++h) {
       const float* s = &sT[0][r * LDS_LD + c + h];
       constexpr int W = kDownRows * LDS_LD;
-      v[h] = (s[0] + s[W]) + (s[2 * W] + s[3 * W]);
-    }
-    if (m0 + r < g.M && c < lora_ldt(g.max_rank)) {
-      uint32_t p[3];
-      split3_pair(v[0], v[1], p);
-      uint16_t* out = (uint16_t*)g.t + (m0 + r) * 3 * lora_ldt(g.max_rank) + c;
+      float d = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *(uint32_t*)(out + (int64_t)k * lora_ldt(g.max_rank)) = p[k];
+      for (int w = 0; w < kDownWaves; ++w) d += s[w * W];
+      v[h >> 2][h & 3] = d;
     }
+    bf8 p[3];
+    split3(v[0], v[1], p);
+    const int64_t m = m0 + r;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      *(bf8*)((uint16_t*)g.t + lora_t_index(m >> 5, k, c >> 4, (int)(m & 31) + 32 * ((c >> 3) & 1), ldt)) = p[k];
   }
 }
 
@@ -342,7 +373,9 @@ __global__ __launch_bounds__(256) void k_lora_down_tile(LoraArgs g) {
 
 bool lora_few_rows(int64_t M) { return M <= 320; }
 
-size_t lora_scratch_bytes(int64_t M, int max_rank) { return (size_t)M * 3 * lora_ldt(max_rank) * 2; }
+size_t lora_scratch_bytes(int64_t M, int max_rank) {
+  return lora_few_rows(M) ? (size_t)M * max_rank * 4 : (size_t)(M + 31) / 32 * 32 * 3 * lora_ldt(max_rank) * 2;
+}
 
 hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
@@ -361,7 +394,8 @@ hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
               : g.max_rank <= 32 ? k_lora_down_tile<2>
               : g.max_rank <= 64 ? k_lora_down_tile<4>
                                  : k_lora_down_tile<8>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((g.M + kDownRows - 1) / kDownRows)), dim3(256), 0, s, g);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((g.M + kDownRows - 1) / kDownRows)),
+                     dim3(kDownWaves * 64), 0, s, g);
   return hipGetLastError();
 }
 

@@ -55,6 +55,14 @@ __device__ __forceinline__ void split3(f4v lo, f4v hi, bf8 (&p)[3]) {
   for (int i = 0; i < 3; ++i) p[i] = o[i].v;
 }
 
+// t of many rows in matrix-core operand order: of 32-row block `block`, part `part`
+// (0 to 2) and 16-rank step `step`, lane l's eight values (row l % 32, ranks 8 (l /
+// 32) ...) lie at this index, so a wave's operand is 1 KB in a row.  ldt: ranks
+// stored per row.
+__device__ __forceinline__ int64_t lora_t_index(int64_t block, int part, int step, int lane, int ldt) {
+  return (((block * 3 + part) * (ldt >> 4) + step) * 64 + lane) * 8;
+}
+
 // The first n (0 to 8) values of w, zeros behind them.
 __device__ __forceinline__ bf8 first_values(bf8 w, int n) {
   union {

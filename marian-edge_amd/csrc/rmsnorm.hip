@@ -70,15 +70,21 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
   };
 
   f4v gv[NV];
+  auto load_scale = [&]() {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if constexpr (VEC) {
-      gv[j] = *(const f4v*)(g.scale + min(4 * (j * T + t), dim - 4));
-    } else {
+    for (int j = 0; j < NV; ++j) {
+      if constexpr (VEC) {
+        gv[j] = *(const f4v*)(g.scale + min(4 * (j * T + t), dim - 4));
+      } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) gv[j][c] = g.scale[min((4 * j + c) * T + t, dim - 1)];
+        for (int c = 0; c < 4; ++c) gv[j][c] = g.scale[min((4 * j + c) * T + t, dim - 1)];
+      }
     }
-  }
+  };
+  // Few values per thread: with the row, for latency; many: once the row's
+  // squares are summed, for registers.
+  constexpr bool kEarly = NV <= 2;
+  if constexpr (kEarly) load_scale();
 
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * ROWS + (T < 256 ? wave : 0); row < g.rows;
@@ -126,6 +132,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int c = 0; c < 4; ++c) ss = __builtin_fma((double)s[j][c], (double)s[j][c], ss);
+    if constexpr (!kEarly) load_scale();
     ss = wave_sum_f64(ss);
     if constexpr (NW > 1) {
       if ((t & 63) == 0) sSum[turn][wave] = ss;
@@ -184,12 +191,11 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
   }
 }
 
-template <int T, int NV>
-hipError_t launch_rms(const RmsArgs& g, bool vec, hipStream_t s) {
+template <int T, int NV, bool VEC>
+hipError_t launch_rms(const RmsArgs& g, hipStream_t s) {
   constexpr int ROWS = T < 256 ? 256 / T : 1;
   const int64_t wgs = (g.rows + ROWS - 1) / ROWS;
-  auto kern = g.bf16 ? (vec ? k_rms_norm<T, NV, true, true> : k_rms_norm<T, NV, true, false>)
-                     : (vec ? k_rms_norm<T, NV, false, true> : k_rms_norm<T, NV, false, false>);
+  auto kern = g.bf16 ? k_rms_norm<T, NV, true, VEC> : k_rms_norm<T, NV, false, VEC>;
   hipLaunchKernelGGL(kern, dim3((unsigned)std::min<int64_t>(wgs, 1 << 20)), dim3(T < 256 ? 256 : T), 0, s, g);
   return hipGetLastError();
 }
@@ -202,13 +208,22 @@ hipError_t launch_rms_norm(const RmsArgs& g, hipStream_t s) {
   const uintptr_t in = (uintptr_t)g.x | (uintptr_t)g.r, out = (uintptr_t)g.sum | (uintptr_t)g.out | (uintptr_t)g.scale;
   const bool vec = g.dim % 4 == 0 && g.ldx % 4 == 0 && (!g.r || g.ldr % 4 == 0) && in % (g.bf16 ? 8 : 16) == 0 &&
                    out % 16 == 0 && (uintptr_t)g.q % 4 == 0;
-  if (g.dim <= 256) return launch_rms<64, 1>(g, vec, s);
-  if (g.dim <= 512) return launch_rms<64, 2>(g, vec, s);
-  if (g.dim <= 1024) return launch_rms<64, 4>(g, vec, s);
-  if (g.dim <= 2048) return launch_rms<256, 2>(g, vec, s);
-  if (g.dim <= 4096) return launch_rms<256, 4>(g, vec, s);
-  if (g.dim <= 8192) return launch_rms<1024, 2>(g, vec, s);
-  return launch_rms<1024, 4>(g, vec, s);
+  if (vec) {
+    if (g.dim <= 256) return launch_rms<64, 1, true>(g, s);
+    if (g.dim <= 512) return launch_rms<64, 2, true>(g, s);
+    if (g.dim <= 1024) return launch_rms<64, 4, true>(g, s);
+    if (g.dim <= 2048) return launch_rms<256, 2, true>(g, s);
+    if (g.dim <= 3 * 1024) return launch_rms<256, 3, true>(g, s);
+    if (g.dim <= 4096) return launch_rms<256, 4, true>(g, s);
+    if (g.dim <= 5 * 1024) return launch_rms<256, 5, true>(g, s);
+    if (g.dim <= 6 * 1024) return launch_rms<256, 6, true>(g, s);
+    if (g.dim <= 8192) return launch_rms<256, 8, true>(g, s);
+    return launch_rms<1024, 4, true>(g, s);
+  }
+  if (g.dim <= 512) return launch_rms<64, 2, false>(g, s);
+  if (g.dim <= 2048) return launch_rms<256, 2, false>(g, s);
+  if (g.dim <= 8192) return launch_rms<1024, 2, false>(g, s);
+  return launch_rms<1024, 4, false>(g, s);
 }
 
 }  // namespace mh

@@ -178,14 +178,20 @@ __device__ __forceinline__ void tile_store(const GemmArgs& g, const Epilogue& e,
 }
 
 // tile_store of fp32 outputs with the adapters' second products added: y + B_s t,
-// t (the first products) as three bf16 parts.  v_mfma_f32_32x32x16_bf16 takes rows
-// and columns l % 32 from lane l, k 8 (l / 32) .. + 8, and its results lie where the
-// int8 blocks' do.  Each distinct slot of a block's 32 rows is one product with all
-// rows' t; rows of other slots do not take it.
-template <int BM, int MB, int NB, bool RELU>
+// t (the first products) as three bf16 parts in operand order.
+// v_mfma_f32_32x32x16_bf16 takes rows and columns l % 32 from lane l, k 8 (l / 32)
+// .. + 8, and its results lie where the int8 blocks' do.  Each distinct slot of a
+// block's 32 rows is one product with all rows' t; rows of other slots do not take
+// it.  Up to RS steps of 16 ranks (STEPS: exactly) t stays in registers and a slot's
+// weights are requested while the one before it is multiplied, the first slot's
+// before the dequantization; 0: more steps, read as they are needed past the first.
+// ad: lane l's row's adapter of each block.
+template <int BM, int MB, int NB, bool RELU, int STEPS>
 __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e, const LoraArgs& l,
                                            const v16i (&acc)[MB][NB], const float* sAm, const float (&wm)[NB],
-                                           const float (&bi)[NB], bool ok, int m0, int n0, int wr, int wc) {
+                                           const float (&bi)[NB], const RowAdapter (&ad)[MB], bool ok, int m0, int n0,
+                                           int wr, int wc, bool stream) {
+  constexpr int RS = STEPS ? STEPS : 1;         // steps held
   const int lane = threadIdx.x & 63, half = lane >> 5;
 #pragma unroll
   for (int k = 0; k < NB; ++k) ok &= recip_factor(wm[k]);
@@ -196,14 +202,51 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
   const uint32_t ldb = (uint32_t)e.ldo * 4;
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
-    const int r0 = m0 + wr + 32 * i, row = min(r0 + (lane & 31), g.M - 1);
-    const RowAdapter ad = row_adapter(l, r0 + (lane & 31) < g.M ? l.slot_of_row[row] : -1, nullptr);
-    const uint16_t* t = (const uint16_t*)l.t + (int64_t)row * 3 * ldt + 8 * half;
+    const int64_t block = __builtin_amdgcn_readfirstlane((m0 + wr + 32 * i) >> 5);
+    const uint32_t with = (uint32_t)__ballot(ad[i].rank > 0);  // rows with an adapter
+    const uint16_t* tb = (const uint16_t*)l.t + lora_t_index(block, 0, 0, 0, ldt);
+    auto part = [&](int c, int step) -> bf8 {
+      return *(const bf8*)(tb + ((uint32_t)lora_t_index(0, c, step, 0, ldt) + (uint32_t)lane * 8));
+    };
+    bf8 t[RS][3];
+    if (with) {
+#pragma unroll
+      for (int s = 0; s < RS; ++s)
+#pragma unroll
+        for (int c = 0; c < 3; ++c) t[s][c] = part(c, s);
+    }
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
       const int n = n0 + wc + k * 32 + (lane & 31);
-      const uint16_t* b = l.b + (int64_t)min(n, g.N - 1) * l.max_rank;
-      float y[16];
+      const uint32_t col = (uint32_t)min(n, g.N - 1) * l.max_rank + 8 * half;
+      struct Slot {
+        int rank;
+        uint32_t rows;
+        const uint16_t* b;
+      };
+      uint32_t todo = with;
+      auto take_slot = [&]() -> Slot {
+        const int lead = __builtin_ctz(todo);
+        const int slot = __builtin_amdgcn_readlane(ad[i].slot, lead);
+        const uint32_t mine = (uint32_t)__ballot(ad[i].slot == slot && ad[i].rank > 0);
+        todo &= ~mine;
+        return {__builtin_amdgcn_readlane(ad[i].rank, lead), mine, l.b + (int64_t)slot * g.N * l.max_rank};
+      };
+      auto weights = [&](const Slot& s, int step) -> bf8 {  // a last half step past max_rank: the one before
+        const int past = 16 * step + 8 * half - (l.max_rank - 8);
+        return *(const bf8*)(s.b + (col + (uint32_t)(16 * step - max(past, 0))));
+      };
+      auto used = [&](bf8 w, int rank, int step) -> bf8 {  // zeros past the slot's rank
+        return 16 * step + 16 > rank ? first_values(w, min(max(rank - 16 * step - 8 * half, 0), 8)) : w;
+      };
+      Slot s = {0, 0, nullptr};
+      bf8 w[RS];
+      if (with) {
+        s = take_slot();
+#pragma unroll
+        for (int q = 0; q < RS; ++q) w[q] = weights(s, q);
+      }
+      v16f y;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float4 a4 = *(const float4*)(sm + i * 32 + 8 * q);
@@ -214,27 +257,47 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
           y[4 * q + c] = dequant_apply(acc[i][k][4 * q + c], inv, bi[k]);
         }
       }
-      uint32_t todo = (uint32_t)__ballot(ad.rank > 0);
-      while (todo) {
-        const int lead = __builtin_ctz(todo);
-        const int slot = __builtin_amdgcn_readlane(ad.slot, lead), rank = __builtin_amdgcn_readlane(ad.rank, lead);
-        const uint32_t mine = (uint32_t)__ballot(ad.slot == slot && ad.rank > 0);
-        todo &= ~mine;
-        const uint16_t* bs = b + (int64_t)slot * g.N * l.max_rank;
-        v16f p;
+      while (s.rows) {
+        Slot next = {0, 0, nullptr};
+        bf8 wn[RS];
+        if (todo) {
+          next = take_slot();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = 0.0f;
-        for (int k0 = 0; k0 < rank; k0 += 16) {
-          const int at = k0 + 8 * half;
-          bf8 w = *(const bf8*)(bs + min(at, l.max_rank - 8));
-          if (k0 + 16 > rank) w = first_values(w, min(max(rank - at, 0), 8));
-#pragma unroll
-          for (int c = 2; c >= 0; --c)
-            p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf8*)(t + c * ldt + k0), w, p, 0, 0, 0);
+          for (int q = 0; q < RS; ++q) wn[q] = weights(next, q);
         }
-        const uint32_t m = mine >> (4 * half);
+        const bf8 w0 = used(w[0], s.rank, 0);
+        auto steps = [&](v16f p) -> v16f {  // p + B_s t but for the largest parts' first step
 #pragma unroll
-        for (int r = 0; r < 16; ++r) y[r] += (m >> (8 * (r >> 2) + (r & 3))) & 1 ? p[r] : 0.0f;
+          for (int c = 1; c >= 0; --c) p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][c], w0, p, 0, 0, 0);
+#pragma unroll
+          for (int q = 1; q < RS; ++q) {
+            if (16 * q >= s.rank) break;
+            const bf8 wq = used(w[q], s.rank, q);
+#pragma unroll
+            for (int c = 2; c >= 0; --c) p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(t[q][c], wq, p, 0, 0, 0);
+          }
+          if constexpr (STEPS == 0) {
+            for (int q = RS; 16 * q < s.rank; ++q) {
+              const bf8 wq = used(weights(s, q), s.rank, q);
+#pragma unroll
+              for (int c = 2; c >= 0; --c) p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(part(c, q), wq, p, 0, 0, 0);
+            }
+          }
+          return p;
+        };
+        if (s.rows == 0xFFFFFFFFu) {  // the whole block
+          y = steps(__builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][2], w0, y, 0, 0, 0));
+          break;
+        }
+        const v16f none = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        const v16f p = steps(__builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][2], w0, none, 0, 0, 0));
+        const uint32_t m = s.rows >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)  // the bits of p, or zero
+          y[r] += __uint_as_float(__float_as_uint(p[r]) & (uint32_t)__builtin_amdgcn_sbfe((int)m, 8 * (r >> 2) + (r & 3), 1));
+        s = next;
+#pragma unroll
+        for (int q = 0; q < RS; ++q) w[q] = wn[q];
       }
       uint32_t off = n < g.N ? (uint32_t)(wr + 4 * half + 32 * i) * ldb + (uint32_t)n * 4 : 0x80000000u;
 #pragma unroll
@@ -243,7 +306,10 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
         for (int c = 0; c < 4; ++c) {
           float v = y[4 * q + c];
           if (RELU) v = v > 0.0f ? v : 0.0f;
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), out, off, 0, 0);
+          if (stream)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), out, off, 0, kNt);
+          else
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), out, off, 0, 0);
           off += (c == 3 ? 5u : 1u) * ldb;
         }
     }
@@ -251,7 +317,7 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
 }
 
 // lora_store with ADAPTERS, else tile_store.
-template <int BM, int BN, int WM, int WN, int PF, bool RELU, bool EXTRA, bool WIDE, bool ADAPTERS>
+template <int BM, int BN, int WM, int WN, int PF, bool RELU, bool EXTRA, bool WIDE, bool ADAPTERS, int STEPS>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epilogue& e, int tiles_n, int tiles, int stream,
                                           const LoraArgs& l) {
   constexpr int NT = WM * WN * 64;
@@ -334,14 +400,16 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epilogue& e, 
       wm[k] = g.wmult[n];
       bi[k] = g.bias[n];
     }
-    for (int c0 = 0; c0 < nslot; c0 += PF) {
-      int cl = c0 + PF;  // the chunks to request
-      if (cl == nslot) {
-        if (tile + per_xcd < hi) corner(tile + per_xcd, m1, n1);
-        point(m1, n1);
-        cl = 0;
-        if (tid < BM) sAm[tpar][tid] = am;
+    RowAdapter ad[ADAPTERS ? MB : 1];  // of this lane's row of each block
+    if constexpr (ADAPTERS) {
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const int row = m0 + wr + 32 * i + (lane & 31);
+        ad[i] = row_adapter(l, row < M ? l.slot_of_row[row] : -1, nullptr);
       }
+    }
+    // Chunks c0 .. c0 + PF - 1; LOAD: then requests PF chunks from cl.
+    auto chunks = [&](int c0, int cl, auto LOAD) {
 #pragma unroll
       for (int u = 0; u < PF; ++u) {
         const bool in_k = (c0 + u) * kTileKC + kp < K;
@@ -355,7 +423,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epilogue& e, 
           const int c = tid + i * NT, row = c >> 3;
           *(v4i*)(sB[u & 1] + row * kTileKC + (((c & 7) ^ (row & 7)) << 4)) = rb[u][i];
         }
-        gload(cl + u, ra[u], rb[u]);
+        if constexpr (LOAD()) gload(cl + u, ra[u], rb[u]);
         wg_lds_barrier();
         const int8_t* la = sA[u & 1] + (wr + (lane & 31)) * kTileKC;
         const int8_t* lb = sB[u & 1] + (wc + (lane & 31)) * kTileKC;
@@ -374,14 +442,32 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epilogue& e, 
               acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[k], acc[i][k], 0, 0, 0);
         }
       }
+    };
+    if constexpr (ADAPTERS) {
+      // One tile a workgroup: nothing is requested past it, whose registers the epilogue needs.
+      for (int c0 = 0; c0 + PF < nslot; c0 += PF) chunks(c0, c0 + PF, std::true_type());
+      if (tid < BM) sAm[tpar][tid] = am;
+      chunks(nslot - PF, 0, std::false_type());
+    } else {
+      for (int c0 = 0; c0 < nslot; c0 += PF) {
+        int cl = c0 + PF;  // the chunks to request
+        if (cl == nslot) {
+          if (tile + per_xcd < hi) corner(tile + per_xcd, m1, n1);
+          point(m1, n1);
+          cl = 0;
+          if (tid < BM) sAm[tpar][tid] = am;
+        }
+        chunks(c0, cl, std::true_type());
+      }
     }
     bool ok = true;
 #pragma unroll
     for (int i = 0; i < BM; i += 64) ok &= recip_factor(sAm[tpar][i + lane]);
     if constexpr (ADAPTERS)
-      lora_store<BM, MB, NB, RELU>(g, e, l, acc, sAm[tpar], wm, bi, ok, m0, n0, wr, wc);
+      lora_store<BM, MB, NB, RELU, STEPS>(g, e, l, acc, sAm[tpar], wm, bi, ad, ok, m0, n0, wr, wc, stream);
     else
       tile_store<BM, MB, NB, RELU, EXTRA, WIDE>(g, e, acc, sAm[tpar], wm, bi, ok, m0, n0, wr, wc, stream);
+    if constexpr (ADAPTERS) return;
     m0 = m1;
     n0 = n1;
   }
@@ -390,13 +476,13 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Epilogue& e, 
 template <int BM, int BN, int WM, int WN, int PF, bool RELU, bool EXTRA, bool WIDE>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(BM > 128 ? 2 : WM * WN / 2)))
 void k_gemm_tile(GemmArgs g, Epilogue e, int tiles_n, int tiles, int stream) {
-  gemm_tile<BM, BN, WM, WN, PF, RELU, EXTRA, WIDE, false>(g, e, tiles_n, tiles, stream, LoraArgs{});
+  gemm_tile<BM, BN, WM, WN, PF, RELU, EXTRA, WIDE, false, 0>(g, e, tiles_n, tiles, stream, LoraArgs{});
 }
 
-template <int BM, int BN, int WM, int WN, int PF, bool RELU>
-__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(BM > 128 ? 2 : WM * WN / 2)))
-void k_gemm_tile_lora(GemmArgs g, Epilogue e, int tiles_n, int tiles, LoraArgs l) {
-  gemm_tile<BM, BN, WM, WN, PF, RELU, false, false, true>(g, e, tiles_n, tiles, 0, l);
+template <int BM, int BN, int WM, int WN, int PF, bool RELU, int STEPS>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(BM > 128 ? 2 : 4)))
+void k_gemm_tile_lora(GemmArgs g, Epilogue e, int tiles_n, int tiles, int stream, LoraArgs l) {
+  gemm_tile<BM, BN, WM, WN, PF, RELU, false, false, true, STEPS>(g, e, tiles_n, tiles, stream, l);
 }
 
 // ---------------------------------------------------------------------------
@@ -614,26 +700,34 @@ hipError_t launch_gemm_tile(const GemmArgs& g, const Epilogue& e, hipStream_t s)
 }
 
 namespace {
-template <int BM, int BN, int WM, int WN, int PF>
-hipError_t launch_tile_lora(const GemmArgs& g, const LoraArgs& l, int max_wgs, hipStream_t s) {
+template <int BM, int BN, int WM, int WN>
+hipError_t launch_tile_lora(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
   const int64_t tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
   if (tiles > (int64_t)INT32_MAX / 2) return hipErrorInvalidValue;
-  const int grid = (int)std::min<int64_t>((tiles + 7) / 8 * 8, max_wgs);
   Epilogue e;
   e.out = l.out;
   e.ldo = g.N;
-  auto kern = l.relu ? k_gemm_tile_lora<BM, BN, WM, WN, PF, true> : k_gemm_tile_lora<BM, BN, WM, WN, PF, false>;
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(WM * WN * 64), 0, s, g, e, (int)tiles_n, (int)tiles, l);
+  const int steps = lora_ldt(l.max_rank) / 16;
+  auto kern = l.relu ? (steps == 1   ? k_gemm_tile_lora<BM, BN, WM, WN, 2, true, 1>
+                        : steps == 2 ? k_gemm_tile_lora<BM, BN, WM, WN, 2, true, 2>
+                                     : k_gemm_tile_lora<BM, BN, WM, WN, 2, true, 0>)
+                     : (steps == 1   ? k_gemm_tile_lora<BM, BN, WM, WN, 2, false, 1>
+                        : steps == 2 ? k_gemm_tile_lora<BM, BN, WM, WN, 2, false, 2>
+                                     : k_gemm_tile_lora<BM, BN, WM, WN, 2, false, 0>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(WM * WN * 64), 0, s, g, e, (int)tiles_n,
+                     (int)tiles, (int)tile_streams(g, e), l);
   return hipGetLastError();
 }
 }  // namespace
 
+// Tiles of 64x64 while they leave a chip's worth of 128x128 ones unfilled, as in
+// launch_gemm_tile; the largest do not pay here (the epilogue's registers leave
+// them one workgroup a CU).
 hipError_t launch_gemm_tile_lora(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
   if (g.K <= 0 || g.K % 64 || g.N <= 0 || g.N > kLoraMaxN || g.lda % 16) return hipErrorInvalidValue;
   if (g.M <= 0) return hipSuccess;
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
-  if (tiles(128, 128) >= 224) return launch_tile_lora<128, 128, 2, 4, 2>(g, l, 1 << 30, s);
-  return launch_tile_lora<64, 64, 2, 2, 2>(g, l, 1024, s);
+  return tiles(128, 128) >= 224 ? launch_tile_lora<128, 128, 2, 4>(g, l, s) : launch_tile_lora<64, 64, 2, 2>(g, l, s);
 }
 
 static int64_t f32_tiles(const GemmArgs& g, int bn) {
