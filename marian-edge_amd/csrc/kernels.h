@@ -152,6 +152,10 @@ constexpr int lora_ldt(int max_rank) { return (max_rank + 15) / 16 * 16; }
 // Whether M rows count as few: each row its own adapter (below), else tiles of
 // rows that mostly share one.
 bool lora_few_rows(int64_t M);
+// Whether a call is one launch (launch_lora_one: no scratch, no codes needed; base.A
+// null: from fp32 rows).
+bool lora_one_launch(int64_t M, int64_t K, int max_rank);
+hipError_t launch_lora_one(const GemmArgs& base, const LoraArgs& g, hipStream_t s);
 size_t lora_scratch_bytes(int64_t M, int max_rank);
 hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s);
 hipError_t launch_lora_linear(const GemmArgs& base, const LoraArgs& g, hipStream_t s);

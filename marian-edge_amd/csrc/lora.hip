@@ -26,14 +26,16 @@ namespace mh {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Few rows, first product: one workgroup of four waves per row.  Each wave holds
-// the row (lane l: values 8l + 512 j ...) and takes every fourth r.  KJ: row
-// pieces in registers (K up to 512 KJ); 0: read again for each r.
+// Few rows, first product: one workgroup of NW waves per row.  Each wave holds
+// the row (lane l: values 8l + 512 j ...) and takes four ranks at a time; NW is
+// as many waves as ranks / 4 keep busy, so that a row's weights are requested at
+// once (200 rows, K 1536, rank 64: 9.6 us with 4 waves).  KJ: row pieces in
+// registers (K up to 512 KJ); 0: read again for each batch.
 // ---------------------------------------------------------------------------
-constexpr int kDownBatch = 4;  // r's whose weights are in flight together
+constexpr int kDownBatch = 4;  // ranks whose weights are in flight together
 
-template <int KJ>
-__global__ __launch_bounds__(256) void k_lora_down_rows(LoraArgs g) {
+template <int KJ, int NW>
+__global__ __launch_bounds__(NW * 64) void k_lora_down_rows(LoraArgs g) {
   touch_kernargs<sizeof(LoraArgs)>();
   const int64_t m = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -108,9 +110,9 @@ __global__ __launch_bounds__(256) void k_lora_down_rows(LoraArgs g) {
     }
   }
 
-  for (int r = a.rank + tid; r < g.max_rank; r += 256) t[r] = 0.0f;
+  for (int r = a.rank + tid; r < g.max_rank; r += NW * 64) t[r] = 0.0f;
   const uint16_t* wa = g.a + (int64_t)a.slot * g.max_rank * K;
-  for (int r0 = wave; r0 < a.rank; r0 += 4 * kDownBatch) {
+  for (int r0 = wave; r0 < a.rank; r0 += NW * kDownBatch) {
     float s[kDownBatch];
 #pragma unroll
     for (int b = 0; b < kDownBatch; ++b) s[b] = 0.0f;
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(256) void k_lora_down_rows(LoraArgs g) {
       const int k = min(512 * j + 8 * lane, K - 8);
       uint4 w[kDownBatch];
 #pragma unroll
-      for (int b = 0; b < kDownBatch; ++b) w[b] = *(const uint4*)(wa + (int64_t)min(r0 + 4 * b, a.rank - 1) * K + k);
+      for (int b = 0; b < kDownBatch; ++b) w[b] = *(const uint4*)(wa + (int64_t)min(r0 + NW * b, a.rank - 1) * K + k);
 #pragma unroll
       for (int b = 0; b < kDownBatch; ++b) {
         const uint32_t d[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
@@ -142,27 +144,30 @@ __global__ __launch_bounds__(256) void k_lora_down_rows(LoraArgs g) {
 #pragma unroll
     for (int b = 0; b < kDownBatch; ++b) {
       const float sum = tree_combine_wave(s[b]);
-      if (lane == 0 && r0 + 4 * b < a.rank) t[r0 + 4 * b] = sum * gain;
+      if (lane == 0 && r0 + NW * b < a.rank) t[r0 + NW * b] = sum * gain;
     }
   }
 }
 
 // ---------------------------------------------------------------------------
 // Few rows, the layer: 16 rows and 16 CT columns per workgroup, its NW waves
-// split K (wave w: k-steps w, w + NW, ...), their exact i32 partials meet in LDS,
-// and each thread finishes whole outputs: dequantization, then the row's t
-// against its slot's 16-byte pieces of B, the first 16 ranks requested before the
-// products start.
+// split K (wave w: k-steps w, w + NW, ...) and their exact i32 partials meet in
+// LDS.  The rows' second products go PL neighbouring lanes to an output, 8 ranks
+// (16 bytes of B) each, so that a wave reads B's rows whole; they are requested
+// before the products start, and their sums meet the dequantized outputs in LDS.
 // ---------------------------------------------------------------------------
 constexpr int kUpRows = 16;
 
-template <int NW, int CT, int KSW>
+template <int NW, int CT, int KSW, int PL>
 __global__ __launch_bounds__(NW * 64) void k_lora_rows(GemmArgs g, LoraArgs l) {
   touch_kernargs<sizeof(GemmArgs) + sizeof(LoraArgs)>();
   constexpr int NT = NW * 64, COLS = 16 * CT, LDC = COLS + 1;
   constexpr int PER = kUpRows * COLS / NT;  // outputs per thread
+  constexpr int ITEMS = PER * PL;           // pieces of 8 ranks per thread
   static_assert(PER >= 1 && PER * NT == kUpRows * COLS, "whole outputs");
   __shared__ int32_t sP[NW][kUpRows * LDC];
+  __shared__ float sD[kUpRows * LDC];
+  __shared__ __attribute__((aligned(16))) float sT[kUpRows * (kLoraMaxRank + 4)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = blockIdx.x * COLS, m0 = blockIdx.y * kUpRows;
   const int ksteps = g.K >> 6, kq = (lane >> 4) * 16;
@@ -183,36 +188,30 @@ __global__ __launch_bounds__(NW * 64) void k_lora_rows(GemmArgs g, LoraArgs l) {
   };
   load(0);
 
+  // Piece i: of output tid / PL + i NT / PL, row-major; ranks from 8 (tid % PL).
+  const int R = l.max_rank, r8 = 8 * (tid % PL), ldt = R + 4;
+  RowAdapter ad[ITEMS];
+  uint4 w[ITEMS];
+  const uint16_t* b[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int o = tid / PL + i * (NT / PL), row = min(m0 + o / COLS, g.M - 1), n = min(n0 + o % COLS, g.N - 1);
+    ad[i] = row_adapter(l, l.slot_of_row[row], nullptr);
+    b[i] = l.b + ((int64_t)ad[i].slot * g.N + n) * R;
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) w[i] = *(const uint4*)(b[i] + min(r8, R - 8));
+  // t's rows into LDS, 4 floats between them.
+  for (int i = tid; i < kUpRows * R / 4; i += NT) {
+    const int row = i / (R / 4), r = i % (R / 4) * 4;
+    *(f4v*)(sT + row * ldt + r) = *(const f4v*)((const float*)l.t + (int64_t)min(m0 + row, g.M - 1) * R + r);
+  }
   // This thread's outputs: column n, rows tid / COLS + k (NT / COLS).
   const int n = min(n0 + tid % COLS, g.N - 1);
   const float wm = g.wmult[n], bias = g.bias[n];
   float am[PER];
-  RowAdapter ad[PER];
-  int64_t row[PER];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    row[k] = min(m0 + tid / COLS + k * (NT / COLS), g.M - 1);
-    am[k] = g.a[row[k]];
-    ad[k] = row_adapter(l, l.slot_of_row[row[k]], nullptr);
-  }
-  // Pieces of 8 ranks: B's 16 bytes and t's 32, rank8 below max_rank.
-  struct Piece {
-    uint4 w;
-    f4v t0, t1;
-  };
-  auto piece = [&](int k, int r8) {
-    Piece p;
-    p.w = *(const uint4*)(l.b + ((int64_t)ad[k].slot * g.N + n) * l.max_rank + r8);
-    const f4v* t = (const f4v*)((const float*)l.t + row[k] * l.max_rank + r8);
-    p.t0 = t[0];
-    p.t1 = t[1];
-    return p;
-  };
-  Piece first[PER][2];
-#pragma unroll
-  for (int k = 0; k < PER; ++k)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) first[k][h] = piece(k, min(8 * h, l.max_rank - 8));
+  for (int k = 0; k < PER; ++k) am[k] = g.a[min(m0 + tid / COLS + k * (NT / COLS), g.M - 1)];
 
   v4i acc[CT];
 #pragma unroll
@@ -234,28 +233,183 @@ __global__ __launch_bounds__(NW * 64) void k_lora_rows(GemmArgs g, LoraArgs l) {
   wg_lds_barrier();
 
 #pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int o = tid / PL + i * (NT / PL), row = o / COLS;
+    float d = 0.0f;
+    auto add = [&](uint4 v, int r) {  // ranks past the slot's: weights of any value, not used
+      const f4v t0 = *(const f4v*)(sT + row * ldt + r), t1 = *(const f4v*)(sT + row * ldt + r + 4);
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float wv = __uint_as_float(c & 1 ? u[c >> 1] & 0xFFFF0000u : u[c >> 1] << 16);
+        const float e = __builtin_fmaf(c < 4 ? t0[c & 3] : t1[c & 3], wv, d);
+        d = r + c < ad[i].rank ? e : d;
+      }
+    };
+    add(w[i], min(r8, R - 8));
+    if (r8 >= R) d = 0.0f;  // fewer pieces than lanes
+    if (PL == 8 && r8 + 64 < R) add(*(const uint4*)(b[i] + r8 + 64), r8 + 64);
+    d += __int_as_float(dpp_mov<0xB1>(__float_as_int(d)));                      // over the output's lanes
+    if constexpr (PL >= 4) d += __int_as_float(dpp_mov<0x4E>(__float_as_int(d)));
+    if constexpr (PL >= 8) d += __int_as_float(dpp_mov<0x141>(__float_as_int(d)));  // row_half_mirror
+    if (tid % PL == 0) sD[row * LDC + o % COLS] = d;
+  }
+  wg_lds_barrier();
+
+#pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int at = (tid / COLS + k * (NT / COLS)) * LDC + tid % COLS;
+    const int row = tid / COLS + k * (NT / COLS), at = row * LDC + tid % COLS;
+    int32_t iv = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) iv += sP[i][at];
+    float y = dequant(iv, am[k], wm, bias) + sD[at];
+    if (l.relu) y = y > 0.0f ? y : 0.0f;
+    if (m0 + row < g.M && n0 + tid % COLS < g.N) l.out[(int64_t)(m0 + row) * g.N + n] = y;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The fewest rows: both products, and the quantization when the caller has no
+// codes, in one launch of 16 CT columns a workgroup.  Each workgroup repeats its
+// rows' first products, which costs less than a second launch and the gap before
+// it while they are few (lora_one_launch).  The waves share (row, four ranks)
+// items of the first product.
+// ---------------------------------------------------------------------------
+constexpr int kOneRows = 16;
+constexpr int kOneMaxK = 2048;
+
+template <int NW, int CT, int KSW>
+__global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
+  touch_kernargs<sizeof(GemmArgs) + sizeof(LoraArgs)>();
+  constexpr int NT = NW * 64, COLS = 16 * CT, LDC = COLS + 1, PER = kOneRows * COLS / NT;
+  __shared__ int32_t sP[NW][kOneRows * LDC];
+  __shared__ __attribute__((aligned(16))) float sT[kOneRows][kLoraMaxRank];
+  __shared__ __attribute__((aligned(16))) int8_t sX[kOneRows * (kOneMaxK + 16)];  // codes made here
+  __shared__ float sM[kOneRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int M = g.M, K = g.K, n0 = blockIdx.x * COLS, ksteps = K >> 6, kq = (lane >> 4) * 16;
+  const int8_t* br[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) br[c] = g.W + (int64_t)min(n0 + 16 * c + (lane & 15), g.N - 1) * K + kq;
+  v4i bf[KSW][CT];
+#pragma unroll
+  for (int i = 0; i < KSW; ++i)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) bf[i][c] = *(const v4i*)(br[c] + min(wave + NW * i, ksteps - 1) * 64);
+  const int n = min(n0 + tid % COLS, g.N - 1);
+  const float wm = g.wmult[n], bias = g.bias[n];
+
+  // ---- the rows' codes ----
+  const int ldx = K + 16;  // of sX: consecutive rows start in other banks
+  if (!g.A) {
+    for (int m = wave; m < M; m += NW) {
+      const float* x = l.x + (int64_t)m * K;
+      f4v v[kOneMaxK / 256];
+      float mx = 0.0f;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < kOneMaxK / 256; ++j)
+        if (256 * j < K) v[j] = *(const f4v*)(x + min(256 * j + 4 * lane, K - 4));
+#pragma unroll
+      for (int j = 0; j < kOneMaxK / 256; ++j)
+        if (256 * j < K)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            mx = fmaxf(mx, fabsf(v[j][c]));
+            bad |= !(fabsf(v[j][c]) < INFINITY);
+          }
+      const float a = row_multiplier(wave_max(mx));
+      if (lane == 0) sM[m] = a;
+      if (__any(bad) && lane == 0 && l.err) *l.err = 1;
+#pragma unroll
+      for (int j = 0; j < kOneMaxK / 256; ++j)
+        if (256 * j + 4 * lane < K)
+          *(uint32_t*)(sX + m * ldx + 256 * j + 4 * lane) = quantize_pack4(v[j][0], v[j][1], v[j][2], v[j][3], a);
+    }
+  }
+
+  // ---- the first product: items of a row and four ranks ----
+  const int quads = (l.max_rank + 3) >> 2;
+  for (int i = wave; i < M * quads; i += NW) {
+    const int m = i / quads, r0 = i % quads * 4;
+    const RowAdapter a = row_adapter(l, l.slot_of_row[m], l.err);
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (r0 < a.rank) {
+      const float* x = l.x + (int64_t)m * K;
+      const uint16_t* w = l.a + (int64_t)a.slot * l.max_rank * K;
+#pragma unroll 2
+      for (int k0 = 0; k0 < K; k0 += 512) {
+        const int k = min(k0 + 8 * lane, K - 8);
+        const bool in = k0 + 8 * lane < K;
+        const f4v x0 = *(const f4v*)(x + k), x1 = *(const f4v*)(x + k + 4);
+        uint4 wr[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) wr[b] = *(const uint4*)(w + (int64_t)min(r0 + b, a.rank - 1) * K + k);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const uint32_t d[4] = {wr[b].x, wr[b].y, wr[b].z, wr[b].w};
+          float e = s[b];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const f4v& xv = c < 2 ? x0 : x1;
+            e = __builtin_fmaf(xv[2 * (c & 1)], __uint_as_float(d[c] << 16), e);
+            e = __builtin_fmaf(xv[2 * (c & 1) + 1], __uint_as_float(d[c] & 0xFFFF0000u), e);
+          }
+          s[b] = in ? e : s[b];
+        }
+      }
+    }
+    const float gain = l.scale[a.slot];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float sum = tree_combine_wave(s[b]);
+      if (lane == 0 && r0 + b < l.max_rank) sT[m][r0 + b] = r0 + b < a.rank ? sum * gain : 0.0f;
+    }
+  }
+  wg_lds_barrier();
+
+  // ---- the layer ----
+  v4i acc[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) acc[c] = v4i{0, 0, 0, 0};
+  const int m = min(lane & 15, M - 1);
+#pragma unroll
+  for (int i = 0; i < KSW; ++i) {
+    const int s = min(wave + NW * i, ksteps - 1);
+    const v4i v = g.A ? *(const v4i*)(g.A + (int64_t)m * g.lda + kq + s * 64) : *(const v4i*)(sX + m * ldx + kq + s * 64);
+    const v4i a = keep_or_zero(v, wave + NW * i < ksteps);
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, bf[i][c], acc[c], 0, 0, 0);
+  }
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sP[wave][((lane >> 4) * 4 + r) * LDC + 16 * c + (lane & 15)] = acc[c][r];
+  wg_lds_barrier();
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int row = tid / COLS + k * (NT / COLS), at = row * LDC + tid % COLS;
+    if (row >= M || n0 + tid % COLS >= g.N) continue;
     int32_t iv = 0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) iv += sP[w][at];
-    float y = dequant(iv, am[k], wm, bias);
+    float y = dequant(iv, g.A ? g.a[row] : sM[row], wm, bias);
+    const RowAdapter a = row_adapter(l, l.slot_of_row[row], nullptr);
+    const uint16_t* b = l.b + ((int64_t)a.slot * g.N + n) * l.max_rank;
     float d = 0.0f;
-    auto add = [&](const Piece& p, int r8) {  // ranks past the slot's: weights of any value, not used
-      const uint32_t w[4] = {p.w.x, p.w.y, p.w.z, p.w.w};
+    for (int r8 = 0; r8 < a.rank; r8 += 8) {
+      const uint4 w = *(const uint4*)(b + r8);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const float b = __uint_as_float(c & 1 ? w[c >> 1] & 0xFFFF0000u : w[c >> 1] << 16);
-        const float e = __builtin_fmaf(c < 4 ? p.t0[c & 3] : p.t1[c & 3], b, d);
-        d = r8 + c < ad[k].rank ? e : d;
+        const float e = __builtin_fmaf(
+            sT[row][r8 + c], __uint_as_float(c & 1 ? u[c >> 1] & 0xFFFF0000u : u[c >> 1] << 16), d);
+        d = r8 + c < a.rank ? e : d;
       }
-    };
-    add(first[k][0], 0);
-    add(first[k][1], 8);
-    for (int r8 = 16; r8 < l.max_rank && __any(r8 < ad[k].rank); r8 += 8) add(piece(k, r8), r8);
+    }
     y += d;
     if (l.relu) y = y > 0.0f ? y : 0.0f;
-    if (m0 + tid / COLS + k * (NT / COLS) < g.M && n0 + tid % COLS < g.N) l.out[row[k] * g.N + n] = y;
+    l.out[(int64_t)row * g.N + n] = y;
   }
 }
 
@@ -377,15 +531,25 @@ size_t lora_scratch_bytes(int64_t M, int max_rank) {
   return lora_few_rows(M) ? (size_t)M * max_rank * 4 : (size_t)(M + 31) / 32 * 32 * 3 * lora_ldt(max_rank) * 2;
 }
 
+template <int NW>
+static hipError_t launch_down_rows_k(const LoraArgs& g, hipStream_t s) {
+  auto kern = g.K <= 512    ? k_lora_down_rows<1, NW>
+              : g.K <= 1024 ? k_lora_down_rows<2, NW>
+              : g.K <= 1536 ? k_lora_down_rows<3, NW>
+              : g.K <= 2048 ? k_lora_down_rows<4, NW>
+                            : k_lora_down_rows<0, NW>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)g.M), dim3(NW * 64), 0, s, g);
+  return hipGetLastError();
+}
+static hipError_t launch_down_rows(const LoraArgs& g, hipStream_t s) {
+  return g.max_rank <= 16   ? launch_down_rows_k<4>(g, s)
+         : g.max_rank <= 32 ? launch_down_rows_k<8>(g, s)
+                            : launch_down_rows_k<16>(g, s);
+}
+
 hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
-  if (lora_few_rows(g.M)) {
-    auto kern = g.K <= 512 ? k_lora_down_rows<1> : g.K <= 1024 ? k_lora_down_rows<2>
-                : g.K <= 2048                    ? k_lora_down_rows<4>
-                                                 : k_lora_down_rows<0>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)g.M), dim3(256), 0, s, g);
-    return hipGetLastError();
-  }
+  if (lora_few_rows(g.M)) return launch_down_rows(g, s);
   if (g.xq) {
     const hipError_t rc = launch_quantize_rows(g.x, g.K, (int)g.M, nullptr, g.K, g.xq, g.K, g.xa, g.err, s);
     if (rc != hipSuccess) return rc;
@@ -399,20 +563,46 @@ hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int NW, int KSW>
+// Every workgroup repeats the M rank first products, four at a time on four or
+// eight waves.  us a call, one launch | two (K 512, N 2048): 1 row of rank 8 8.0 |
+// 11.1, 4 of 16 8.5 | 11.4, 2 of 64 14.3 | 11.7, 8 of 16 13.8 | 11.2; K 2048, N 512: 2
+// rows of 16 8.1 | 11.3, 4 of 16 11.9 | 11.2, 1 of 64 12.3 | 11.9.
+bool lora_one_launch(int64_t M, int64_t K, int max_rank) {
+  return M <= kOneRows && K <= kOneMaxK && M * max_rank <= 64 && M * max_rank * K <= 65536;
+}
+
+hipError_t launch_lora_one(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
+  if (g.M <= 0) return hipSuccess;
+  if (g.M > kOneRows || g.K > kOneMaxK) return hipErrorInvalidValue;
+  const dim3 wide((g.N + 31) / 32), narrow((g.N + 15) / 16);
+  if (g.K <= 512)
+    hipLaunchKernelGGL(g.N >= 1024 ? (k_lora_one<4, 2, 2>) : (k_lora_one<4, 1, 2>), g.N >= 1024 ? wide : narrow, dim3(256), 0, s, g, l);
+  else
+    hipLaunchKernelGGL(g.N >= 1024 ? (k_lora_one<8, 2, 4>) : (k_lora_one<4, 1, 8>), g.N >= 1024 ? wide : narrow,
+                       dim3(g.N >= 1024 ? 512 : 256), 0, s, g, l);
+  return hipGetLastError();
+}
+
+template <int NW, int KSW, int PL>
 static hipError_t launch_rows(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
   const int rows = (g.M + kUpRows - 1) / kUpRows;
   if (g.N >= 1024)
-    hipLaunchKernelGGL((k_lora_rows<NW, 2, KSW>), dim3((g.N + 31) / 32, rows), dim3(NW * 64), 0, s, g, l);
+    hipLaunchKernelGGL((k_lora_rows<NW, 2, KSW, PL>), dim3((g.N + 31) / 32, rows), dim3(NW * 64), 0, s, g, l);
   else
-    hipLaunchKernelGGL((k_lora_rows<4, 1, KSW * NW / 4>), dim3((g.N + 15) / 16, rows), dim3(256), 0, s, g, l);
+    hipLaunchKernelGGL((k_lora_rows<4, 1, KSW * NW / 4, PL>), dim3((g.N + 15) / 16, rows), dim3(256), 0, s, g, l);
   return hipGetLastError();
+}
+template <int PL>
+static hipError_t launch_rows_k(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
+  return g.K <= 512 ? launch_rows<4, 2, PL>(g, l, s) : launch_rows<8, 4, PL>(g, l, s);
 }
 
 hipError_t launch_lora_linear(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
   if (!lora_few_rows(g.M)) return launch_gemm_tile_lora(g, l, s);
-  return g.K <= 512 ? launch_rows<4, 2>(g, l, s) : launch_rows<8, 4>(g, l, s);
+  return l.max_rank <= 16   ? launch_rows_k<2>(g, l, s)
+         : l.max_rank <= 32 ? launch_rows_k<4>(g, l, s)
+                            : launch_rows_k<8>(g, l, s);
 }
 
 }  // namespace mh

@@ -327,15 +327,6 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
     return refuse("q8_linear_lora: x, xq, w, lora_a, lora_b and workspace must be 16-byte aligned");
   if (M == 0) return MARIAN_HIP_OK;
   hipStream_t s = (hipStream_t)stream;
-  const LoraWorkspace ws = lora_workspace(M, K, max_rank, xq != nullptr);
-  if (workspace) {
-    if (workspace_bytes < ws.bytes) return refuse("q8_linear_lora: the workspace is too small");
-  } else {
-    // A graph would go on using scratch that a later call may replace.
-    if (capturing(s)) return refuse("q8_linear_lora: a call that is captured into a graph needs a workspace");
-    workspace = op_scratch(3, ws.bytes, s);
-    if (!workspace) return op_status(hipErrorOutOfMemory, "q8_linear_lora scratch");
-  }
   LoraArgs l;
   l.x = x;
   l.M = M;
@@ -348,18 +339,9 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
   l.slots = (int)slots;
   l.max_rank = (int)max_rank;
   l.slot_of_row = slot_of_row;
-  l.t = workspace;
   l.relu = relu;
   l.out = out_f32;
   l.err = err;
-  if (!xq) {
-    l.xq = (int8_t*)workspace + ws.codes;
-    l.xa = (float*)((char*)workspace + ws.mults);
-    xq = l.xq;
-    xa = l.xa;
-  }
-  const int rc = op_status(launch_lora_down(l, s), "q8_linear_lora down");
-  if (rc) return rc;
   GemmArgs g;
   g.A = xq;
   g.a = xa;
@@ -370,6 +352,29 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
   g.wmult = w_mult;
   g.bias = bias;
   g.N = (int)N;
+  const LoraWorkspace ws = lora_workspace(M, K, max_rank, xq != nullptr);
+  if (workspace) {
+    if (workspace_bytes < ws.bytes) return refuse("q8_linear_lora: the workspace is too small");
+  } else if (capturing(s)) {
+    // A graph would go on using scratch that a later call may replace.
+    return refuse("q8_linear_lora: a call that is captured into a graph needs a workspace");
+  }
+  // In place a workgroup would store its columns over rows that others still read.
+  if (lora_one_launch(M, K, (int)max_rank) && !overlap(x, (size_t)M * K * 4, out_f32, (size_t)M * N * 4))
+    return op_status(launch_lora_one(g, l, s), "q8_linear_lora");
+  if (!workspace) {
+    workspace = op_scratch(3, ws.bytes, s);
+    if (!workspace) return op_status(hipErrorOutOfMemory, "q8_linear_lora scratch");
+  }
+  l.t = workspace;
+  if (!xq) {
+    l.xq = (int8_t*)workspace + ws.codes;
+    l.xa = (float*)((char*)workspace + ws.mults);
+    g.A = l.xq;
+    g.a = l.xa;
+  }
+  const int rc = op_status(launch_lora_down(l, s), "q8_linear_lora down");
+  if (rc) return rc;
   return op_status(launch_lora_linear(g, l, s), "q8_linear_lora");
 }
 
