@@ -479,7 +479,8 @@ int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int6
  * A row with a negative slot has no adapter.  lora_a [slots, max_rank, K] and
  * lora_b [slots, N, max_rank] hold bfloat16 values; slot s uses its first
  * lora_rank[s] (0 to max_rank) rows of A and columns of B, the rest is not used.
- * max_rank is a multiple of 8 up to 128, K a multiple of 64, N below 2^20.  A slot at or past
+ * max_rank is a multiple of 8 up to 128, K a multiple of 64, N below 2^20,
+ * M up to 2^26, slots up to 2^20.  A slot at or past
  * `slots`, or a rank out of range, sets *err (device int, may be NULL) to 1 and
  * counts as no adapter; a row's result does not depend on other rows' adapters.
  * x (fp32 [M, K]) is always given, it is what the adapters read; xq / xa are its

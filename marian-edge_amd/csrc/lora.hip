@@ -414,42 +414,42 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows, first product: 16 rows per workgroup, its eight waves split K in
+// Many rows, first product: 16 rows per workgroup, its NW waves split K in
 // chunks of 32, RT tiles of 16 ranks.  v_mfma_f32_16x16x32_bf16: lane l holds k
 // 8 (l / 16) .. + 8 of x's row l % 16 and of A's row l % 16, and of the result
 // column (rank) l % 16, rows 4 (l / 16) + r.  A wave reads and splits its x once, 512
-// columns of the row at a time, and multiplies it with each slot of the tile.
+// columns of the row at a time, and multiplies it with each slot of the tile; its two
+// chunks are neighbours, whole cache lines of A.  blockIdx.y: RT tiles of ranks each.
 // ---------------------------------------------------------------------------
 constexpr int kDownRows = 16;
-constexpr int kDownWaves = 8;
 constexpr int kDownChunks = 2;  // chunks of a wave held at once
 
-template <int RT>
-__global__ __launch_bounds__(kDownWaves * 64) void k_lora_down_tile(LoraArgs g) {
+template <int RT, int NW>
+__global__ __launch_bounds__(NW * 64) void k_lora_down_tile(LoraArgs g) {
   touch_kernargs<sizeof(LoraArgs)>();
   constexpr int LDS_LD = 16 * RT + 1;
-  __shared__ float sT[kDownWaves][kDownRows * LDS_LD];
+  __shared__ float sT[NW][kDownRows * LDS_LD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t m0 = (int64_t)blockIdx.x * kDownRows;
-  const int K = g.K, kq = 8 * (lane >> 4), chunks = K >> 5;
+  const int K = g.K, kq = 8 * (lane >> 4), chunks = K >> 5, r0 = blockIdx.y * (16 * RT);
   const int64_t row = m0 + (lane & 15) < g.M ? m0 + (lane & 15) : g.M - 1;
   const float* x = g.x + row * K + kq;
   f4v x0[kDownChunks], x1[kDownChunks];
   auto load_x = [&](int c0) {  // past K: the last chunk again
 #pragma unroll
     for (int u = 0; u < kDownChunks; ++u) {
-      const int c = min(c0 + kDownWaves * u, chunks - 1);
+      const int c = min(c0 + u, chunks - 1);
       x0[u] = *(const f4v*)(x + 32 * c);
       x1[u] = *(const f4v*)(x + 32 * c + 4);
     }
   };
-  load_x(wave);
+  load_x(kDownChunks * wave);
   const RowAdapter ad = row_adapter(g, m0 + (lane & 15) < g.M ? g.slot_of_row[row] : -1, g.err);
   const uint32_t with = (uint32_t)__ballot(ad.rank > 0) & 0xFFFFu;  // rows with an adapter
   f4v sum[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) sum[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c0 = wave; with && c0 < chunks; c0 += kDownWaves * kDownChunks) {
+  for (int c0 = kDownChunks * wave; with && c0 < chunks; c0 += NW * kDownChunks) {
     bf8 p[kDownChunks][3];
     for (uint32_t todo = with; todo;) {  // the tile's slots, one after another
       const int lead = __builtin_ctz(todo);
@@ -468,16 +468,16 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down_tile(LoraArgs g) 
         for (int u = 0; u < kDownChunks; ++u)
 #pragma unroll
           for (int t = 0; t < AT; ++t)
-            w[u][t] = *(const bf8*)(a + (int64_t)min(16 * (t0 + t) + (lane & 15), rank - 1) * K +
-                                    32 * min(c0 + kDownWaves * u, chunks - 1));
+            w[u][t] = *(const bf8*)(a + (int64_t)min(r0 + 16 * (t0 + t) + (lane & 15), rank - 1) * K +
+                                    32 * min(c0 + u, chunks - 1));
         if (t0 == 0 && todo == with) {
 #pragma unroll
           for (int u = 0; u < kDownChunks; ++u) split3(x0[u], x1[u], p[u]);
-          if (c0 + kDownWaves * kDownChunks < chunks) load_x(c0 + kDownWaves * kDownChunks);
+          if (c0 + NW * kDownChunks < chunks) load_x(c0 + NW * kDownChunks);
         }
 #pragma unroll
         for (int u = 0; u < kDownChunks; ++u)
-          if (c0 + kDownWaves * u < chunks)  // uniform
+          if (c0 + u < chunks)  // uniform
 #pragma unroll
             for (int t = 0; t < AT; ++t)
 #pragma unroll
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down_tile(LoraArgs g) 
       for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (((mine >> (4 * (lane >> 4) + r)) & 1) && 16 * t + (lane & 15) < rank)
+          if (((mine >> (4 * (lane >> 4) + r)) & 1) && r0 + 16 * t + (lane & 15) < rank)
             sum[t][r] += acc[t][r] * gain;
       todo &= ~mine;
     }
@@ -501,9 +501,9 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down_tile(LoraArgs g) 
   wg_lds_barrier();
   // Eight ranks of a row per thread: the waves' sums, split, one 16-byte store a part.
   const int ldt = lora_ldt(g.max_rank);
-  for (int i = tid; i < kDownRows * 2 * RT; i += kDownWaves * 64) {
+  for (int i = tid; i < kDownRows * 2 * RT; i += NW * 64) {
     const int r = i % kDownRows, c = i / kDownRows * 8;
-    if (c >= ldt) break;
+    if (r0 + c >= ldt) break;
     f4v v[2];
 #pragma unroll
     for (int h = 0; h < 8; ++h) {
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down_tile(LoraArgs g) 
       constexpr int W = kDownRows * LDS_LD;
       float d = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kDownWaves; ++w) d += s[w * W];
+      for (int w = 0; w < NW; ++w) d += s[w * W];
       v[h >> 2][h & 3] = d;
     }
     bf8 p[3];
@@ -519,12 +519,16 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down_tile(LoraArgs g) 
     const int64_t m = m0 + r;
 #pragma unroll
     for (int k = 0; k < 3; ++k)
-      *(bf8*)((uint16_t*)g.t + lora_t_index(m >> 5, k, c >> 4, (int)(m & 31) + 32 * ((c >> 3) & 1), ldt)) = p[k];
+      *(bf8*)((uint16_t*)g.t + lora_t_index(m >> 5, k, (r0 + c) >> 4, (int)(m & 31) + 32 * ((c >> 3) & 1), ldt)) = p[k];
   }
 }
 
 }  // namespace
 
+// us a call, each row its own adapter (above) | tiles; K 2048, N 512, rank 64: 320
+// rows of one request after another 25 | 33, of requests in turn 26 | 111; 1000 rows
+// 51 | 34 and 55 | 118; K 512, N 2048, rank 64, 320 rows: 26 | 17 and 26 | 51.  Which it is
+// the host cannot see; decode batches are in turn and small, prompts neither.
 bool lora_few_rows(int64_t M) { return M <= 320; }
 
 size_t lora_scratch_bytes(int64_t M, int max_rank) {
@@ -547,6 +551,23 @@ static hipError_t launch_down_rows(const LoraArgs& g, hipStream_t s) {
                             : launch_down_rows_k<16>(g, s);
 }
 
+// While 16-row tiles do not fill the chip, a workgroup per 16 ranks too, and as many
+// waves as a long row has work for: each (512 or 1024 columns, slot) is a round trip
+// to memory (500 rows, K 2048, rank 64, us: 26.5 with eight waves and all ranks, 15.6
+// with a workgroup per 16 ranks).
+static hipError_t launch_down_tile(const LoraArgs& g, hipStream_t s) {
+  const int64_t tiles = (g.M + kDownRows - 1) / kDownRows;
+  const int steps = lora_ldt(g.max_rank) / 16;
+  const int rt = steps == 1 || tiles < 256 ? 1 : steps == 2 || tiles < 512 ? 2 : 4;
+  const bool wide = rt == 1 && g.K > 1024;
+  auto kern = wide      ? k_lora_down_tile<1, 16>
+              : rt == 1 ? k_lora_down_tile<1, 8>
+              : rt == 2 ? k_lora_down_tile<2, 8>
+                        : k_lora_down_tile<4, 8>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (steps + rt - 1) / rt), dim3(wide ? 1024 : 512), 0, s, g);
+  return hipGetLastError();
+}
+
 hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
   if (lora_few_rows(g.M)) return launch_down_rows(g, s);
@@ -554,13 +575,7 @@ hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
     const hipError_t rc = launch_quantize_rows(g.x, g.K, (int)g.M, nullptr, g.K, g.xq, g.K, g.xa, g.err, s);
     if (rc != hipSuccess) return rc;
   }
-  auto kern = g.max_rank <= 16   ? k_lora_down_tile<1>
-              : g.max_rank <= 32 ? k_lora_down_tile<2>
-              : g.max_rank <= 64 ? k_lora_down_tile<4>
-                                 : k_lora_down_tile<8>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((g.M + kDownRows - 1) / kDownRows)),
-                     dim3(kDownWaves * 64), 0, s, g);
-  return hipGetLastError();
+  return launch_down_tile(g, s);
 }
 
 // Every workgroup repeats the M rank first products, four at a time on four or

@@ -192,7 +192,7 @@ LoraWorkspace lora_workspace(int64_t M, int64_t K, int64_t max_rank, bool has_xq
   return w;
 }
 bool lora_sizes_ok(int64_t M, int64_t K, int64_t max_rank) {
-  return M >= 0 && M <= INT32_MAX && K > 0 && K <= INT32_MAX && K % 64 == 0 && max_rank > 0 &&
+  return M >= 0 && M <= kLoraMaxRows && K > 0 && K <= INT32_MAX && K % 64 == 0 && max_rank > 0 &&
          max_rank <= kLoraMaxRank && max_rank % 8 == 0;
 }
 
@@ -318,7 +318,7 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
                               const int32_t* lora_rank, int64_t slots, int64_t max_rank,
                               const int32_t* slot_of_row, float* out_f32, void* workspace,
                               size_t workspace_bytes, int* err, void* stream) {
-  if (!lora_sizes_ok(M, K, max_rank) || N <= 0 || N > kLoraMaxN || slots <= 0 || slots > INT32_MAX)
+  if (!lora_sizes_ok(M, K, max_rank) || N <= 0 || N > kLoraMaxN || slots <= 0 || slots > kLoraMaxSlots)
     return refuse("q8_linear_lora: sizes out of range");
   if (!x || !w || !w_mult || !bias || !lora_a || !lora_b || !lora_scale || !lora_rank || !slot_of_row || !out_f32 ||
       !xq != !xa)
@@ -326,6 +326,15 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
   if (((uintptr_t)x | (uintptr_t)xq | (uintptr_t)w | (uintptr_t)lora_a | (uintptr_t)lora_b | (uintptr_t)workspace) % 16)
     return refuse("q8_linear_lora: x, xq, w, lora_a, lora_b and workspace must be 16-byte aligned");
   if (M == 0) return MARIAN_HIP_OK;
+  const size_t out_bytes = (size_t)M * N * 4, table = (size_t)slots * max_rank * 2;
+  const struct { const void* p; size_t bytes; } others[] = {
+      {xq, (size_t)M * K}, {xa, (size_t)M * 4}, {w, (size_t)N * K}, {w_mult, (size_t)N * 4}, {bias, (size_t)N * 4},
+      {lora_a, table * K}, {lora_b, table * N}, {lora_scale, (size_t)slots * 4}, {lora_rank, (size_t)slots * 4},
+      {slot_of_row, (size_t)M * 4}, {workspace, workspace_bytes}};
+  for (const auto& o : others)
+    if (overlap(out_f32, out_bytes, o.p, o.bytes)) return refuse("q8_linear_lora: out overlaps an input that is not x");
+  if (overlap(workspace, workspace_bytes, x, (size_t)M * K * 4))
+    return refuse("q8_linear_lora: the workspace overlaps x");
   hipStream_t s = (hipStream_t)stream;
   LoraArgs l;
   l.x = x;

@@ -65,7 +65,9 @@ def lora_args(**change):
     (dict(ls=None), "missing"), (dict(lr=None), "missing"), (dict(slot=None), "missing"), (dict(out=None), "missing"),
     (dict(x=at(0) + 4), "aligned"), (dict(la=at(6) + 2), "aligned"), (dict(lb=at(7) + 8), "aligned"),
     (dict(w=at(3) + 1), "aligned"), (dict(xq=at(1) + 8), "aligned"), (dict(ws=at(12) + 4), "aligned"),
-    (dict(ws_bytes=16), "too small"),
+    (dict(ws_bytes=16), "too small"), (dict(M=(1 << 26) + 1), "out of range"), (dict(N=1 << 20), "out of range"),
+    (dict(out=at(1) + 16), "overlaps"), (dict(out=at(3)), "overlaps"), (dict(out=at(7) + 32), "overlaps"),
+    (dict(out=at(10)), "overlaps"), (dict(out=at(12) + 64), "overlaps"), (dict(ws=at(0) + 256), "overlaps"),
 ])
 def test_lora_refuses(pkg, lib, change, why):
     assert lib.marian_hip_q8_linear_lora(*lora_args(**change)) == pkg._lib.ERR_INVALID_INPUT
