@@ -9,11 +9,13 @@
 // which lie next to rounding borders, come out the same for every launch
 // shape, and a and q are what marian_hip_quantize_rows makes of the stored y.
 // 64-bit products run at the rate of 32-bit ones here and the kernel waits for
-// memory, so they cost nothing.
+// memory, so they cost nothing: 65536 rows of 512, bf16 in, sum, out and q stored,
+// 67 us, 5.5 TB/s (a copy of that size: 5.1); one row of 512: 2.0 us, the launch.
 #include "device_common.h"
 #include "kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mh {
 namespace {
@@ -39,13 +41,19 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// T threads hold a row: VEC: float4 number j of thread t at columns 4(jT + t);
-// otherwise (a width, stride or address that is no multiple of four values)
-// value i of thread t at column iT + t.  Loads past the row are clamped to its
-// last values and zeroed, so that all of a row's loads are in flight at once.
-// One wave per row up to 1024 columns (four rows a workgroup, no barrier), a
-// workgroup of 256 or 1024 threads above.
-template <int T, int NV, bool BF16, bool VEC>
+// Four values at any address of theirs.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32u __attribute__((aligned(1)));
+
+// T threads hold a row, four neighbouring values at a time: quad number j of
+// thread t begins at column 4(jT + t).  A quad that ends past the row (TAIL: a width
+// that is no multiple of four) holds its last four values instead, of which the sum
+// takes those that the quad before does not have; both compute and store the same
+// values for the others.  Quads past the row load the last four too, so that all of a
+// row's loads are in flight at once.  T = 64: a wave per row, four rows a workgroup and
+// no barrier.
+template <int T, int NV, bool BF16, bool TAIL>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
   touch_kernargs<sizeof(RmsArgs)>();
   constexpr int ROWS = T < 256 ? 256 / T : 1, NW = T / 64;
@@ -54,32 +62,38 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
   const int t = threadIdx.x % T, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int dim = g.dim;
 
-  auto load = [&](const void* p, int64_t at) -> f4v {  // four values from element `at`
+  const bool tiny = TAIL && T == 64 && NV == 1 && dim < 4;  // less than a quad, in thread 0
+  auto quad = [&](int j) { return 4 * (j * T + t); };
+  auto load_f32 = [&](const float* p, int j) -> f4v {
+    if (tiny) return f4v{p[0], p[min(1, dim - 1)], p[dim - 1], 0.0f};
+    return *(const f4u*)(p + min(quad(j), dim - 4));
+  };
+  using Quad = std::conditional_t<BF16, h4u, f4v>;
+  auto load = [&](const void* row, int64_t first, int j) -> Quad {
     if constexpr (BF16) {
-      const ushort4 h = *(const ushort4*)((const uint16_t*)p + at);
-      return f4v{bf16_to_f32(h.x), bf16_to_f32(h.y), bf16_to_f32(h.z), bf16_to_f32(h.w)};
+      const uint16_t* p = (const uint16_t*)row + first;
+      if (tiny) return h4u{p[0], p[min(1, dim - 1)], p[dim - 1], 0};
+      return *(const h4u*)(p + min(quad(j), dim - 4));
     } else {
-      return *(const f4v*)((const float*)p + at);
+      return load_f32((const float*)row + first, j);
     }
   };
-  auto load1 = [&](const void* p, int64_t at) -> float {
+  auto f32 = [](Quad v, int c) -> float {
     if constexpr (BF16)
-      return bf16_to_f32(((const uint16_t*)p)[at]);
+      return bf16_to_f32(v[c]);
     else
-      return ((const float*)p)[at];
+      return v[c];
+  };
+  // Whether value c of quad j is one of the row's and no other quad's.
+  auto counts = [&](int j, int c) {
+    if constexpr (TAIL) return tiny ? t == 0 && c < dim : quad(j) < dim && min(quad(j), dim - 4) + c >= quad(j);
+    return quad(j) < dim;
   };
 
   f4v gv[NV];
   auto load_scale = [&]() {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if constexpr (VEC) {
-        gv[j] = *(const f4v*)(g.scale + min(4 * (j * T + t), dim - 4));
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) gv[j][c] = g.scale[min((4 * j + c) * T + t, dim - 1)];
-      }
-    }
+    for (int j = 0; j < NV; ++j) gv[j] = load_f32(g.scale, j);
   };
   // Few values per thread: with the row, for latency; many: once the row's
   // squares are summed, for registers.
@@ -89,49 +103,34 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * ROWS + (T < 256 ? wave : 0); row < g.rows;
        row += (int64_t)gridDim.x * ROWS, turn ^= 1) {
-    f4v s[NV], rv[NV];
-    const int64_t x0 = row * g.ldx, r0 = row * g.ldr, o0 = row * dim;
-    if constexpr (VEC) {
+    f4v s[NV];
+    Quad xv[NV], rv[NV];
+    const int64_t o0 = row * dim;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) s[j] = load(g.x, x0 + min(4 * (j * T + t), dim - 4));
-      if (g.r) {
+    for (int j = 0; j < NV; ++j) xv[j] = load(g.x, row * g.ldx, j);
+    if (g.r) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) rv[j] = load(g.r, r0 + min(4 * (j * T + t), dim - 4));
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[j][c] = s[j][c] + rv[j][c];
-      }
+      for (int j = 0; j < NV; ++j) rv[j] = load(g.r, row * g.ldr, j);
+      __builtin_amdgcn_sched_barrier(0);  // all loads first
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[j][c] = 4 * (j * T + t) < dim ? s[j][c] : 0.0f;
+        for (int c = 0; c < 4; ++c) s[j][c] = f32(xv[j], c) + f32(rv[j], c);
     } else {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[j][c] = load1(g.x, x0 + min((4 * j + c) * T + t, dim - 1));
-      if (g.r) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) rv[j][c] = load1(g.r, r0 + min((4 * j + c) * T + t, dim - 1));
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[j][c] = s[j][c] + rv[j][c];
-      }
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[j][c] = (4 * j + c) * T + t < dim ? s[j][c] : 0.0f;
+        for (int c = 0; c < 4; ++c) s[j][c] = f32(xv[j], c);
     }
-
     double ss = 0.0;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) ss = __builtin_fma((double)s[j][c], (double)s[j][c], ss);
+      for (int c = 0; c < 4; ++c) {
+        const double v = counts(j, c) ? s[j][c] : 0.0f;
+        ss = __builtin_fma(v, v, ss);
+      }
     if constexpr (!kEarly) load_scale();
     ss = wave_sum_f64(ss);
     if constexpr (NW > 1) {
@@ -150,8 +149,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         y[j][c] = (float)((double)s[j][c] * inv * (double)gv[j][c]);
-        const bool in = VEC ? 4 * (j * T + t) < dim : (4 * j + c) * T + t < dim;
-        mx = max(mx, in ? __float_as_uint(y[j][c]) & 0x7fffffffu : 0u);
+        mx = max(mx, !tiny || c < dim ? __float_as_uint(y[j][c]) & 0x7fffffffu : 0u);
       }
     if (g.q || g.err) {
       mx = row16_max(mx);
@@ -169,61 +167,55 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rms_norm(RmsArgs g) {
     if (g.a && t == 0) g.a[row] = a;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if constexpr (VEC) {
-        const int c = 4 * (j * T + t);
-        if (c < dim) {
-          if (g.sum) *(f4v*)(g.sum + o0 + c) = s[j];
-          if (g.out) *(f4v*)(g.out + o0 + c) = y[j];
-          if (g.q) *(uint32_t*)(g.q + o0 + c) = quantize_pack4(y[j][0], y[j][1], y[j][2], y[j][3], a);
+      if (quad(j) >= dim) continue;
+      const uint32_t q = quantize_pack4(y[j][0], y[j][1], y[j][2], y[j][3], a);
+      if (tiny) {
+        for (int i = 0; i < dim; ++i) {
+          if (g.sum) g.sum[o0 + i] = i == 0 ? s[j][0] : i == 1 ? s[j][1] : s[j][2];
+          if (g.out) g.out[o0 + i] = i == 0 ? y[j][0] : i == 1 ? y[j][1] : y[j][2];
+          if (g.q) g.q[o0 + i] = (int8_t)(q >> 8 * i);
         }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int col = (4 * j + c) * T + t;
-          if (col < dim) {
-            if (g.sum) g.sum[o0 + col] = s[j][c];
-            if (g.out) g.out[o0 + col] = y[j][c];
-            if (g.q) g.q[o0 + col] = (int8_t)quantize_one(y[j][c], a);
-          }
-        }
+        continue;
       }
+      const int64_t at = o0 + min(quad(j), dim - 4);
+      if (g.sum) *(f4u*)(g.sum + at) = s[j];
+      if (g.out) *(f4u*)(g.out + at) = y[j];
+      if (g.q) *(u32u*)(g.q + at) = q;
     }
   }
 }
 
-template <int T, int NV, bool VEC>
+template <int T, int NV>
 hipError_t launch_rms(const RmsArgs& g, hipStream_t s) {
   constexpr int ROWS = T < 256 ? 256 / T : 1;
   const int64_t wgs = (g.rows + ROWS - 1) / ROWS;
-  auto kern = g.bf16 ? k_rms_norm<T, NV, true, VEC> : k_rms_norm<T, NV, false, VEC>;
+  auto kern = g.dim % 4 ? (g.bf16 ? k_rms_norm<T, NV, true, true> : k_rms_norm<T, NV, false, true>)
+                        : (g.bf16 ? k_rms_norm<T, NV, true, false> : k_rms_norm<T, NV, false, false>);
   hipLaunchKernelGGL(kern, dim3((unsigned)std::min<int64_t>(wgs, 1 << 20)), dim3(T < 256 ? 256 : T), 0, s, g);
   return hipGetLastError();
 }
 
 }  // namespace
 
+// The fewest threads that hold the row in registers: more threads wait for each
+// other, and quads past the row cost what others do.  us for 2^25 bf16 | fp32 values
+// (sum, out, q stored): 512 columns, one wave 67 | 76, 256 threads 124 | 107; 1001: one
+// wave 69 | 88, 256 threads 99 | 88; 2047: 256 threads, 2 quads 84 | 81, 512 threads 94 | 87;
+// 5000: 256 threads, 6 quads 74 | 81, 8 quads 74 | 80, 512 threads, 4 quads 86 | 83; 8192:
+// 256 threads 69 | 81, 512 threads 75 | 82; 12001: 512 threads, 6 quads 85 | 86, 8 quads
+// 89 | 89; 16384: 512 threads 76 | 86, 1024 threads 76 | 86.
 hipError_t launch_rms_norm(const RmsArgs& g, hipStream_t s) {
   if (!g.x || !g.scale || g.dim <= 0 || g.dim > kRmsMaxDim || g.rows < 0) return hipErrorInvalidValue;
   if (g.rows == 0) return hipSuccess;
-  const uintptr_t in = (uintptr_t)g.x | (uintptr_t)g.r, out = (uintptr_t)g.sum | (uintptr_t)g.out | (uintptr_t)g.scale;
-  const bool vec = g.dim % 4 == 0 && g.ldx % 4 == 0 && (!g.r || g.ldr % 4 == 0) && in % (g.bf16 ? 8 : 16) == 0 &&
-                   out % 16 == 0 && (uintptr_t)g.q % 4 == 0;
-  if (vec) {
-    if (g.dim <= 256) return launch_rms<64, 1, true>(g, s);
-    if (g.dim <= 512) return launch_rms<64, 2, true>(g, s);
-    if (g.dim <= 1024) return launch_rms<64, 4, true>(g, s);
-    if (g.dim <= 2048) return launch_rms<256, 2, true>(g, s);
-    if (g.dim <= 3 * 1024) return launch_rms<256, 3, true>(g, s);
-    if (g.dim <= 4096) return launch_rms<256, 4, true>(g, s);
-    if (g.dim <= 5 * 1024) return launch_rms<256, 5, true>(g, s);
-    if (g.dim <= 6 * 1024) return launch_rms<256, 6, true>(g, s);
-    if (g.dim <= 8192) return launch_rms<256, 8, true>(g, s);
-    return launch_rms<1024, 4, true>(g, s);
-  }
-  if (g.dim <= 512) return launch_rms<64, 2, false>(g, s);
-  if (g.dim <= 2048) return launch_rms<256, 2, false>(g, s);
-  if (g.dim <= 8192) return launch_rms<1024, 2, false>(g, s);
-  return launch_rms<1024, 4, false>(g, s);
+  if (g.dim <= 256) return launch_rms<64, 1>(g, s);
+  if (g.dim <= 512) return launch_rms<64, 2>(g, s);
+  if (g.dim <= 1024) return launch_rms<64, 4>(g, s);
+  if (g.dim <= 2048) return launch_rms<256, 2>(g, s);
+  if (g.dim <= 4096) return launch_rms<256, 4>(g, s);
+  if (g.dim <= 6144) return launch_rms<256, 6>(g, s);
+  if (g.dim <= 8192) return launch_rms<256, 8>(g, s);
+  if (g.dim <= 12288) return launch_rms<512, 6>(g, s);
+  return launch_rms<512, 8>(g, s);
 }
 
 }  // namespace mh

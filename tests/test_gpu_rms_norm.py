@@ -44,8 +44,8 @@ def case(rng, rows, dim, ldx, ldr, residual, bf16):
     return x, r, scale, x, r
 
 
-DIMS = [1, 2, 3, 4, 5, 63, 64, 65, 255, 256, 257, 384, 512, 513, 1000, 1024, 1025, 2048, 2049, 4096, 4100, 5000, 8192,
-        8195, 16383, 16384]
+DIMS = [1, 2, 3, 4, 5, 63, 64, 65, 255, 256, 257, 384, 512, 513, 1000, 1024, 1025, 2048, 2049, 4096, 4100, 5000, 6001,
+        6144, 8192, 8195, 12287, 12289, 16383, 16384]
 
 
 @pytest.mark.parametrize("residual", [True, False])
@@ -88,7 +88,7 @@ def test_row_counts(dev, rows):
 
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("dim, ldx, ldr, off", [(512, 1536, 520, 0), (512, 515, 513, 1), (100, 101, 100, 3),
-                                                (1500, 1504, 2000, 1), (6000, 6004, 6001, 2)])
+                                                (1500, 1504, 2000, 1), (6000, 6004, 6001, 2), (3, 5, 4, 1), (4099, 4101, 4103, 3)])
 def test_strides_and_addresses(dev, dim, ldx, ldr, off, bf16):
     rows, size = 9, 2 if bf16 else 4
     rng = np.random.default_rng(dim + off)
@@ -104,7 +104,7 @@ def test_strides_and_addresses(dev, dim, ldx, ldr, off, bf16):
     check(s.host(), out.host(), q.host(), a.host(), *dso.rms_norm(view(x, ldx), view(r, ldr), scale, 1e-6))
 
 
-@pytest.mark.parametrize("dim", [384, 2000, 10000])
+@pytest.mark.parametrize("dim", [1, 3, 7, 384, 1001, 2000, 5003, 7997, 10000, 10001])
 def test_optional_outputs_and_in_place(dev, dim):
     rows = 33
     rng = np.random.default_rng(dim)
