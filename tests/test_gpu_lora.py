@@ -69,6 +69,16 @@ SHAPES = [  # M, K, N, R, slots, run length
     (127, 704, 1000, 56, 6, 20), (129, 512, 2300, 16, 8, 1), (200, 1536, 384, 64, 24, 1), (256, 512, 2048, 128, 40, 1),
     (257, 384, 1536, 8, 300, 1), (700, 512, 512, 16, 5, 33), (1459, 512, 2048, 16, 32, 25), (2100, 384, 1152, 48, 9, 1),
     (3000, 64, 70, 8, 20, 100),
+    # one launch from codes and from rows, on both column widths and row lengths
+    (1, 2048, 512, 16, 3, 1), (2, 1536, 2300, 16, 2, 1), (1, 1088, 1025, 32, 2, 1), (4, 640, 1030, 16, 4, 1),
+    (8, 512, 1000, 8, 5, 1), (16, 256, 1027, 8, 9, 1),
+    # few rows past the registers' row pieces, every group of ranks
+    (9, 2560, 300, 128, 4, 1), (40, 2112, 1100, 16, 6, 1), (320, 4096, 96, 24, 30, 1), (18, 960, 2050, 72, 4, 1),
+    # many rows: one, two and four tiles of ranks a workgroup, long rows, ranks over several workgroups
+    (321, 2048, 520, 64, 4, 40), (340, 1088, 200, 128, 3, 50), (4100, 512, 64, 32, 7, 60), (4099, 64, 128, 64, 3, 1),
+    (8200, 192, 96, 64, 6, 100), (8195, 128, 65, 128, 4, 300), (4097, 1152, 70, 128, 5, 90),
+    # tiles of 128 columns
+    (4100, 128, 1000, 16, 6, 70), (4101, 192, 900, 24, 8, 1), (4102, 128, 897, 48, 5, 33),
 ]
 
 
