@@ -463,7 +463,8 @@ int marian_hip_residual_layer_norm(const float* x, const float* r, const float* 
  * 127).  The mean and y are computed in 64 bits and rounded once, so results do
  * not depend on the launch; a and q are what marian_hip_quantize_rows makes of y.
  * x and r (r may be NULL: s = x) are fp32 rows, or bfloat16 with in_bf16 != 0, ldx
- * and ldr values apart, at any value-aligned address.  dim 1 to 16384, eps > 0.
+ * and ldr values apart (at most 2^29), at any value-aligned address.  dim 1 to 16384,
+ * eps > 0.
  * sum (s, the residual stream), out (y) and q with a are contiguous rows, each
  * optional, but one of out and q must be given.  fp32 outputs may be x or r
  * themselves when those are fp32 rows dim apart; other overlaps are refused.
@@ -482,7 +483,8 @@ int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int6
  * max_rank is a multiple of 8 up to 128, K a multiple of 64, N below 2^20,
  * M up to 2^26, slots up to 2^20.  A slot at or past
  * `slots`, or a rank out of range, sets *err (device int, may be NULL) to 1 and
- * counts as no adapter; a row's result does not depend on other rows' adapters.
+ * counts as no adapter; a row's result does not depend on other rows' adapters
+ * (the order of its fp32 sums depends on M: a call picks its kernels by the sizes).
  * x (fp32 [M, K]) is always given, it is what the adapters read; xq / xa are its
  * codes and multipliers (both or neither: then the call quantizes x, and a
  * non-finite x sets *err).  The adapters' products are sums of fp32 with exact bf16
@@ -552,13 +554,14 @@ int marian_hip_candidate_argmax(const int8_t* xq, const float* xa, int64_t M, in
  * p ~ exp(logit / temperature): top_k keeps the first k, top_p of those the
  * shortest prefix (at least one id) with top_p of their mass, min_p of those the
  * ids with p >= min_p * max(p).  token[m] is the first kept id in ascending order
- * whose running kept mass exceeds u of the kept mass; logprob[m] (optional) the
- * logarithm of its share of the kept mass.  Masses are multiples of 2^-44 of the
+ * whose running kept mass exceeds u of the kept mass (u rounded down to a multiple
+ * of 2^-32); logprob[m] (optional) the logarithm of its share of the kept mass.
+ * token and logprob may share no memory with each other or an input.  Masses are multiples of 2^-44 of the
  * maximum's, and their sums exact: ids below 2^-45 of it are never drawn, and a
  * row's result does not depend on the launch or on other rows.  A row of only
  * -inf and NaN gets id 0 and logprob -inf.  A setting or u out of range sets *err
  * (device int, may be NULL) to 1, and the row's maximum is taken.
- * V up to 524288, rows up to 1048576.  Nothing is allocated. */
+ * V up to 524288, rows up to 1048576, ld up to 2^29.  Nothing is allocated. */
 int marian_hip_sample_logits(const void* logits, int64_t ld, int64_t rows, int64_t V, int in_bf16,
                              const float* temperature, const int32_t* top_k, const float* top_p,
                              const float* min_p, const float* u, int32_t* token, float* logprob,

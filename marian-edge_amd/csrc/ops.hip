@@ -166,6 +166,8 @@ int linear_op(const float* x, float act, const int8_t* xq, const float* xa, int6
   return op_status(launch_gemm_store(g, e, s), what);
 }
 
+constexpr int64_t kMaxStride = 1 << 29;  // of a caller's rows, in values: 2^31 rows stay within 64-bit offsets
+
 // Records why a call is refused.
 int refuse(const char* what) {
   g_op_error = what;
@@ -268,7 +270,7 @@ int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int6
                                  int in_bf16, float* sum, float* out, int8_t* q, float* a, int* err,
                                  void* stream) {
   if (!x || !scale || rows < 0 || rows > INT32_MAX || dim <= 0 || dim > kRmsMaxDim || ldx < dim ||
-      (r && ldr < dim) || !(eps > 0.0f) || !std::isfinite(eps))
+      ldx > kMaxStride || (r && (ldr < dim || ldr > kMaxStride)) || !(eps > 0.0f) || !std::isfinite(eps))
     return refuse("residual_rms_norm: sizes, strides or eps out of range, or x or scale missing");
   if (!out && !q) return refuse("residual_rms_norm: neither out nor q is given");
   if (!q != !a) return refuse("residual_rms_norm: q and a go together");
@@ -387,12 +389,25 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
   return op_status(launch_lora_linear(g, l, s), "q8_linear_lora");
 }
 
+namespace {
+// Outputs of a sampling call share no memory with each other or with the inputs
+// (rows are drawn in any order).  logits_bytes: as far as the host knows them.
+bool sample_overlap(const SampleArgs& g, size_t logits_bytes) {
+  const size_t w = (size_t)g.rows * 4;
+  const struct { const void* p; size_t bytes; } ins[] = {{g.logits, logits_bytes}, {g.off, w + 4}, {g.temperature, w},
+                                                         {g.top_k, w}, {g.top_p, w}, {g.min_p, w}, {g.u, w}};
+  for (const auto& i : ins)
+    if (overlap(g.token, w, i.p, i.bytes) || overlap(g.logprob, w, i.p, i.bytes)) return true;
+  return overlap(g.token, w, g.logprob, w);
+}
+}  // namespace
+
 int marian_hip_sample_logits(const void* logits, int64_t ld, int64_t rows, int64_t V, int in_bf16,
                              const float* temperature, const int32_t* top_k, const float* top_p,
                              const float* min_p, const float* u, int32_t* token, float* logprob,
                              int* err, void* stream) {
   if (!logits || !u || !token) return refuse("sample_logits: logits, u or token is missing");
-  if (rows < 0 || rows > kSampleMaxRows || V <= 0 || V > kSampleMaxIds || ld < V)
+  if (rows < 0 || rows > kSampleMaxRows || V <= 0 || V > kSampleMaxIds || ld < V || ld > kMaxStride)
     return refuse("sample_logits: sizes out of range");
   SampleArgs g;
   g.logits = logits;
@@ -408,6 +423,8 @@ int marian_hip_sample_logits(const void* logits, int64_t ld, int64_t rows, int64
   g.token = token;
   g.logprob = logprob;
   g.err = err;
+  if (sample_overlap(g, rows ? ((size_t)(rows - 1) * ld + V) * (in_bf16 ? 2 : 4) : 0))
+    return refuse("sample_logits: an output overlaps an input or the other output");
   return op_status(launch_sample(g, (hipStream_t)stream), "sample_logits");
 }
 
@@ -433,6 +450,7 @@ int marian_hip_sample_candidates(const float* logits, const uint32_t* cand, cons
   g.token = token;
   g.logprob = logprob;
   g.err = err;
+  if (sample_overlap(g, 0)) return refuse("sample_candidates: an output overlaps an input or the other output");
   return op_status(launch_sample(g, (hipStream_t)stream), "sample_candidates");
 }
 

@@ -28,7 +28,8 @@ def norm_args(**change):
     (dict(x=None), "missing"), (dict(scale=None), "missing"),
     (dict(rows=-1), "out of range"), (dict(rows=1 << 31), "out of range"),
     (dict(dim=0), "out of range"), (dict(dim=16385, ldx=1 << 15, ldr=1 << 15), "out of range"),
-    (dict(ldx=95), "out of range"), (dict(ldr=95), "out of range"),
+    (dict(ldx=95), "out of range"), (dict(ldr=95), "out of range"), (dict(ldx=1 << 30), "out of range"),
+    (dict(ldr=1 << 61), "out of range"),
     (dict(eps=0.0), "out of range"), (dict(eps=-1e-6), "out of range"), (dict(eps=float("nan")), "out of range"),
     (dict(eps=float("inf")), "out of range"),
     (dict(out=None, q=None, a=None), "neither"),
@@ -59,7 +60,7 @@ def lora_args(**change):
     (dict(M=-1), "out of range"), (dict(M=1 << 31), "out of range"), (dict(K=0), "out of range"),
     (dict(K=100), "out of range"), (dict(N=0), "out of range"), (dict(N=1 << 31), "out of range"),
     (dict(max_rank=0), "out of range"), (dict(max_rank=12), "out of range"), (dict(max_rank=136), "out of range"),
-    (dict(slots=0), "out of range"), (dict(slots=1 << 31), "out of range"),
+    (dict(slots=0), "out of range"), (dict(slots=(1 << 20) + 1), "out of range"), (dict(slots=1 << 31), "out of range"),
     (dict(x=None), "missing"), (dict(xq=None), "missing"), (dict(xa=None), "missing"), (dict(w=None), "missing"),
     (dict(mult=None), "missing"), (dict(bias=None), "missing"), (dict(la=None), "missing"), (dict(lb=None), "missing"),
     (dict(ls=None), "missing"), (dict(lr=None), "missing"), (dict(slot=None), "missing"), (dict(out=None), "missing"),
@@ -103,7 +104,10 @@ def sample_args(**change):
 @pytest.mark.parametrize("change, why", [
     (dict(logits=None), "missing"), (dict(u=None), "missing"), (dict(token=None), "missing"),
     (dict(rows=-1), "out of range"), (dict(rows=(1 << 20) + 1), "out of range"), (dict(V=0), "out of range"),
-    (dict(V=(1 << 19) + 1, ld=1 << 20), "out of range"), (dict(ld=95), "out of range"),
+    (dict(V=(1 << 19) + 1, ld=1 << 20), "out of range"), (dict(ld=95), "out of range"), (dict(ld=1 << 62), "out of range"),
+    (dict(token=at(0) + 64), "overlaps"), (dict(token=at(0) + 4 * 395), "overlaps"), (dict(token=at(1)), "overlaps"),
+    (dict(lp=at(2) + 12), "overlaps"), (dict(lp=at(3), t=at(3)), "overlaps"), (dict(k=at(2)), "overlaps"),
+    (dict(p=at(2) + 4), "overlaps"), (dict(mp=at(2) - 4), "overlaps"),
 ])
 def test_sample_logits_refuses(pkg, lib, change, why):
     assert lib.marian_hip_sample_logits(*sample_args(**change)) == pkg._lib.ERR_INVALID_INPUT
@@ -121,6 +125,8 @@ def candidate_args(**change):
     (dict(logits=None), "missing"), (dict(cand=None), "missing"), (dict(off=None), "missing"), (dict(u=None), "missing"),
     (dict(token=None), "missing"), (dict(rows=-1), "out of range"), (dict(rows=(1 << 20) + 1), "out of range"),
     (dict(most=0), "out of range"), (dict(most=(1 << 19) + 1), "out of range"),
+    (dict(token=at(2) + 16), "overlaps"), (dict(token=at(3) + 8), "overlaps"), (dict(lp=at(4)), "overlaps"),
+    (dict(k=at(4) + 4), "overlaps"),
 ])
 def test_sample_candidates_refuses(pkg, lib, change, why):
     assert lib.marian_hip_sample_candidates(*candidate_args(**change)) == pkg._lib.ERR_INVALID_INPUT
