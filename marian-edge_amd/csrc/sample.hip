@@ -28,7 +28,7 @@ constexpr int kBins = 2048;
 constexpr int kBinsPerOctave = 32;             // of p, in the histograms over log2 p
 constexpr int kLastBin = 46 * kBinsPerOctave;  // ids past it have no mass
 constexpr int kMassBits = 44;                  // mass of the row's maximum
-constexpr int kList = 256;                     // ids compared pairwise
+constexpr int kList = 256;                     // ids put in order at once
 
 // 2^(j/32)
 __device__ const double kExp2[32] = {
@@ -119,8 +119,10 @@ struct SampleLds {
   uint64_t hist[kBins];      // masses or counts
   double exp2[32];
   uint64_t seg[SEGS];  // kept mass of every 256 consecutive ids
-  ulonglong2 entry[kList];  // the list: pair, weight
-  uint64_t before[kList];
+  __attribute__((aligned(16))) uint64_t entry[kList];   // the list's pairs
+  __attribute__((aligned(16))) uint64_t sorted[kList];  // in order
+  uint32_t ahead[kList];                                // of an entry: how many come before it; zero between uses
+  uint32_t kept[kList / 64];
   uint64_t wsum[NW];
   float wmax[NW];
   int found, best;
@@ -187,15 +189,17 @@ __device__ __forceinline__ Found locate(Lds& L, Need&& need_of) {
 // and masses in registers, they took half as long again).
 //
 // Few ids to draw from (at most kList ids in the row, or a top-k of which at most
-// kList ids can be part): all of them in a list, compared pairwise.  The k-th
-// largest of the threads' maxima is a lower bound of the k-th largest id, so a
-// histogram of T values finds the ids that the list needs.
+// kList ids can be part): all of them in a list, put in order by counting the entries
+// ahead of each; every setting is then a prefix sum over the threads (a pass of
+// comparisons per setting took four times as long: 453 lists of up to 215 ids,
+// mixed settings, 44 us then and 12 now).  The k-th largest of the threads'
+// maxima is a lower bound of the k-th largest id, so a histogram of T values finds
+// the ids that the list needs.
 //
 // Otherwise the border of top-k, then of top-p among what is left: a histogram over
 // log2 p (of counts, or of masses), the bin where the count or mass is reached, then
-// every id of that bin against every other.  A bin of more than kList ids (many
-// equal logits) is cut again by (logit, id) pairs, kBins ways a time, until few
-// are left.
+// that bin's ids in order.  A bin of more than kList ids (many equal logits) is cut
+// again by (logit, id) pairs, kBins ways a time, until few are left.
 enum Stage { LIST_ALL, LIST_TOP, BORDER_K, BORDER_P, DRAW, DRAWN };
 
 template <int T, int IDS, bool BF16>
@@ -322,6 +326,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     L.listed = 0;
   }
   if (t < 32) L.exp2[t] = kExp2[t];
+  if (t < kList) L.ahead[t] = 0;
   for (int b = t; b < kBins; b += T) L.hist[b] = 0;
   for (int s = t; s < SampleLds<T, IDS>::SEGS; s += T) L.seg[s] = 0;
   wg_lds_barrier();
@@ -430,18 +435,69 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     });
   };
 
+  // How many of list's first `count` entries come before entry t (larger & mask), for
+  // t < count: 64, 128 or 256 threads take one entry each, and as many groups of
+  // them as there are share the comparisons.
+  auto count_ahead = [&](const uint64_t* list, uint32_t count, uint64_t mask) -> uint32_t {
+    const int lg = count <= 64 ? 6 : count <= 128 ? 7 : 8;
+    static_assert(kList == 256, "groups of up to 256 threads");
+    const uint32_t at = t & ((1 << lg) - 1), group = wave >> (lg - 6), groups = T >> lg;
+    if (at < count) {
+      const uint64_t mine = list[at] & mask;
+      uint32_t ahead = 0;
+#pragma unroll 4
+      for (uint32_t i = 2 * group; i + 1 < count; i += 2 * groups) {
+        const ulonglong2 e = *(const ulonglong2*)(list + i);
+        ahead += (e.x & mask) > mine ? 1u : 0u;
+        ahead += (e.y & mask) > mine ? 1u : 0u;
+      }
+      if ((count & 1) && group == 0) ahead += (list[count - 1] & mask) > mine ? 1u : 0u;
+      if (ahead) lds_add(&L.ahead[at], ahead);
+    }
+    wg_lds_barrier();
+    const uint32_t all = L.ahead[t & (kList - 1)];
+    wg_lds_barrier();
+    if (t < kList) L.ahead[t] = 0;
+    return all;
+  };
+  // The sum of w over the threads before this one, of the first kList.
+  auto scan_threads = [&](uint64_t w, uint64_t& total) -> uint64_t {
+    uint64_t s = wave_scan_mass(w);
+    if (lane == 63) L.wsum[wave] = s;
+    wg_lds_barrier();
+    s -= w;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kList / 64; ++i) {
+      const uint64_t v = L.wsum[i];
+      total += v;
+      s += i < wave ? v : 0ull;
+    }
+    return s;
+  };
+
   int drawn = -1;  // in the thread that holds it: the id, its logit, the kept mass
   float drawn_v = 0.0f;
   uint64_t drawn_of = 0;
   int stage = n <= kList ? LIST_ALL : !by_k ? (by_p ? BORDER_P : DRAW) : top_k <= kList * 3 / 4 ? LIST_TOP : BORDER_K;
 #pragma unroll 1
   while (stage < DRAW) {
-    // ---- the list: of the stage's bins, of a part of one when it is crowded ----
-    int first = 0, last = kLastBin, shift = -1;  // shift: of a part's number
-    uint64_t need = 0, lo = 0, hi = ~0ull;       // pairs looked at
+    // ---- the list: all ids at their own places, or those of the stage's bins (of a
+    // part of one when it is crowded) ----
+    uint32_t listed = n;
+    uint64_t need = 0;
+    if (stage == LIST_ALL) {
+      each([&](int, int i, f4v v) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (i + c < n) L.entry[i + c] = pair_of(v[c], (uint32_t)(i + c));
+      });
+      wg_lds_barrier();
+    } else {
+      int first = 0, last = 0, shift = -1;  // shift: of a part's number
+      uint64_t lo = 0, hi = ~0ull;          // pairs looked at
 #pragma unroll 1
-    for (;;) {
-      if (stage != LIST_ALL) {
+      for (;;) {
         if (shift >= 0) {
           each([&](int, int i, f4v v) {
 #pragma unroll
@@ -480,99 +536,92 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
           first = stage == LIST_TOP ? 0 : f.bin;
         }
         need -= f.before;
-      }
-      if (last >= 0) {
-        const float least = least_of(last), most = first ? most_of(first) : INFINITY;
-        each([&](int, int i, f4v v) {
-          bool in[4];
+        if (last >= 0) {
+          const float least = least_of(last), most = first ? most_of(first) : INFINITY;
+          each([&](int, int i, f4v v) {
+            bool in[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) in[c] = (v[c] >= least) & (v[c] <= most);
-          if (!__any((in[0] | in[1]) | (in[2] | in[3]))) return;
+            for (int c = 0; c < 4; ++c) in[c] = (v[c] >= least) & (v[c] <= most);
+            if (!__any((in[0] | in[1]) | (in[2] | in[3]))) return;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (!in[c]) continue;
-            const int b = bin_of(v[c]);
-            const uint64_t p = pair_of(v[c], (uint32_t)(i + c));
-            if (b < first || b > last || p < lo || p > hi || p < pair_of(border_v, (uint32_t)border_id)) continue;
-            const uint32_t at = lds_add(&L.listed, 1u);
-            if (at < (uint32_t)kList) L.entry[at].x = p;
-            if (shift < 0 && stage >= BORDER_K) {  // the range of all, should they be too many
-              __hip_atomic_fetch_min(&L.lo, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-              __hip_atomic_fetch_max(&L.hi, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int c = 0; c < 4; ++c) {
+              if (!in[c]) continue;
+              const int b = bin_of(v[c]);
+              const uint64_t p = pair_of(v[c], (uint32_t)(i + c));
+              if (b < first || b > last || p < lo || p > hi || p < pair_of(border_v, (uint32_t)border_id)) continue;
+              const uint32_t at = lds_add(&L.listed, 1u);
+              if (at < (uint32_t)kList) L.entry[at] = p;
+              if (shift < 0 && stage >= BORDER_K) {  // the range of all, should they be too many
+                __hip_atomic_fetch_min(&L.lo, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                __hip_atomic_fetch_max(&L.hi, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+              }
             }
-          }
-        });
+          });
+        }
+        wg_lds_barrier();
+        if (last < 0 || L.listed <= (uint32_t)kList || stage == LIST_TOP) break;
+        if (shift < 0) {
+          lo = L.lo;
+          hi = L.hi;
+        }
+        shift = max(0, 64 - 11 - __builtin_clzll((hi - lo) | 1));  // kBins parts of [lo, hi]
       }
-      wg_lds_barrier();
-      if (last < 0 || L.listed <= (uint32_t)kList || stage == LIST_TOP) break;
-      if (shift < 0) {
-        lo = L.lo;
-        hi = L.hi;
+      listed = L.listed;
+      if (last < 0 || listed > (uint32_t)kList) {  // too few ids with mass for top_k, too many for the list
+        stage = stage == LIST_TOP ? BORDER_K : by_p ? BORDER_P : DRAW;
+        continue;
       }
-      shift = max(0, 64 - 11 - __builtin_clzll((hi - lo) | 1));  // kBins parts of [lo, hi]
-    }
-    const uint32_t listed = L.listed;
-    if (last < 0 || listed > (uint32_t)kList) {  // too few ids with mass for top_k, too many for the list
-      stage = stage == LIST_TOP ? BORDER_K : by_p ? BORDER_P : DRAW;
-      continue;
     }
 
-    // ---- its entries against each other: 64, 128 or 256 threads take one entry each, and
-    // as many groups of them as there are share the comparisons ----
-    const int lg = listed <= 64 ? 6 : listed <= 128 ? 7 : 8;
-    static_assert(kList == 256, "groups of up to 256 threads");
-    const uint32_t at = t & ((1 << lg) - 1), groups = T >> lg;
-    const uint64_t mine = L.entry[min(at, listed - 1)].x;
-    const float v = pair_logit(mine);
-    const uint64_t m = mass_of(v);
-    const bool own = t < (int)listed;  // one thread per entry
-    bool keep = own, hit = false;
-    int pass = stage == BORDER_P || (stage == LIST_ALL && !by_k) ? 1 : 0;  // 0: count, 1: mass, 2: draw
-    const int end = stage >= BORDER_K ? pass : 2;
-#pragma unroll 1
-    for (; pass <= end; ++pass) {
-      if (pass == 1 && !by_p) continue;
-      if (pass == 2) keep = keep && v >= least_v;
-      const uint64_t w = !keep ? 0ull : pass ? m : 1ull;
-      const uint64_t ws = wave_scan_mass(w);
-      if (lane == 63) L.wsum[wave] = ws;
-      if (own) L.entry[t].y = w;
-      if (t < kList) L.before[t] = 0;
-      wg_lds_barrier();
-      uint64_t sum = 0;
-#pragma unroll
-      for (int i = 0; i < kList / 64; ++i) sum += L.wsum[i];
-      if (stage < BORDER_K) need = pass == 0 ? (uint64_t)top_k : pass == 1 ? need_p(sum) : need_u(sum);
-      const uint64_t mask = pass == 2 ? 0xFFFFFFFFull : ~0ull;  // the draw goes by id alone
-      if (at < listed) {
-        uint64_t s = 0;
-#pragma unroll 4
-        for (uint32_t i = t >> lg; i < listed; i += groups) {
-          const ulonglong2 e = L.entry[i];
-          s += (e.x & mask) > (mine & mask) ? e.y : 0ull;
-        }
-        if (s) lds_add(&L.before[at], s);
-      }
-      wg_lds_barrier();
-      const uint64_t before = L.before[at];
-      hit = keep && before < need && need <= before + w;  // the sum reaches need here
-      keep = keep && before < need;
-      drawn_of = sum;
-      wg_lds_barrier();
+    // ---- in order: thread t's entry goes where as many come before it ----
+    const uint32_t own_rank = count_ahead(L.entry, listed, ~0ull);
+    if (t < (int)listed) L.sorted[own_rank] = L.entry[t];
+    wg_lds_barrier();
+    if (stage == BORDER_K) {
+      border_v = pair_logit(L.sorted[need - 1]);
+      border_id = pair_id(L.sorted[need - 1]);
+      stage = by_p ? BORDER_P : DRAW;
+      wg_lds_barrier();  // before the next list
+      continue;
     }
-    if (stage < BORDER_K) {
-      if (hit) {
-        drawn = pair_id(mine);
-        drawn_v = v;
-      }
-      stage = DRAWN;
-    } else {
-      if (hit) L.border = mine;
+    const uint32_t upto = stage == LIST_ALL || stage == LIST_TOP ? (by_k ? min(listed, (uint32_t)top_k) : listed) : listed;
+    uint64_t pair = L.sorted[min((uint32_t)t, listed - 1)], total;
+    uint64_t m = (uint32_t)t < upto ? mass_of(pair_logit(pair)) : 0ull;
+    uint64_t before = scan_threads(m, total);
+    if (stage == BORDER_P) {
+      if (before < need && need <= before + m) L.border = pair;
       wg_lds_barrier();
       border_v = pair_logit(L.border);
       border_id = pair_id(L.border);
-      stage = stage == BORDER_K && by_p ? BORDER_P : DRAW;
+      stage = DRAW;
+      continue;
     }
+    const bool keep = (uint32_t)t < upto && (!by_p || before < need_p(total)) && pair_logit(pair) >= least_v;
+    const uint32_t mine = (uint32_t)__builtin_popcountll(__ballot(keep));
+    if (lane == 0 && wave < kList / 64) L.kept[wave] = mine;
+    wg_lds_barrier();
+    uint32_t kept = 0;  // the first so many
+#pragma unroll
+    for (int i = 0; i < kList / 64; ++i) kept += L.kept[i];
+    // The draw, in ascending ids: the places of a list of all, else sorted once more.
+    if (stage == LIST_ALL) {
+      pair = L.entry[min((uint32_t)t, listed - 1)];
+      m = (uint32_t)t < listed && own_rank < kept ? mass_of(pair_logit(pair)) : 0ull;
+    } else {
+      const uint32_t id_rank = count_ahead(L.sorted, kept, 0xFFFFFFFFull);
+      if ((uint32_t)t < kept) L.entry[id_rank] = pair;
+      wg_lds_barrier();
+      pair = L.entry[min((uint32_t)t, kept - 1)];
+      m = (uint32_t)t < kept ? mass_of(pair_logit(pair)) : 0ull;
+    }
+    before = scan_threads(m, total);
+    const uint64_t number = need_u(total);
+    if (before < number && number <= before + m) {
+      drawn = pair_id(pair);
+      drawn_v = pair_logit(pair);
+      drawn_of = total;
+    }
+    stage = DRAWN;
   }
 
   // ---- the draw: kept mass of every 256 consecutive ids, then one id ----
