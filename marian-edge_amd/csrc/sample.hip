@@ -30,59 +30,65 @@ constexpr int kLastBin = 46 * kBinsPerOctave;  // ids past it have no mass
 constexpr int kMassBits = 44;                  // mass of the row's maximum
 constexpr int kList = 256;                     // ids put in order at once
 
-// 2^(j/32)
-__device__ const double kExp2[32] = {
-    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
-    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
-    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
-    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
-    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
-    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
+// The bits of 2^(44 + j/32) less j * 2^47: with n * 2^47 added (n % 32 = j) those of
+// 2^(44 + n/32).
+__device__ const uint64_t kExp2[32] = {
+    0x42b0000000000000ull, 0x42afd9b0d3158574ull, 0x42afb5586cf9890full, 0x42af9301d0125b51ull,
+    0x42af72b83c7d517bull, 0x42af54873168b9aaull, 0x42af387a6e756238ull, 0x42af1e9df51fdee1ull,
+    0x42af06fe0a31b715ull, 0x42aef1a7373aa9cbull, 0x42aedea64c123422ull, 0x42aece086061892dull,
+    0x42aebfdad5362a27ull, 0x42aeb42b569d4f82ull, 0x42aeab07dd485429ull, 0x42aea47eb03a5585ull,
+    0x42aea09e667f3bcdull, 0x42ae9f75e8ec5f74ull, 0x42aea11473eb0187ull, 0x42aea589994cce13ull,
+    0x42aeace5422aa0dbull, 0x42aeb737b0cdc5e5ull, 0x42aec49182a3f090ull, 0x42aed503b23e255dull,
+    0x42aee89f995ad3adull, 0x42aeff76f2fb5e47ull, 0x42af199bdd85529cull, 0x42af3720dcef9069ull,
+    0x42af5818dcfba487ull, 0x42af7c97337b9b5full, 0x42afa4afa2a490daull, 0x42afd0765b6e4540ull,
 };
 
-// log2 of p over the maximum's (at least -60; NaN counts as that) in steps of
-// 1/32, and what is left, |rest| <= 1/64.  Adding 1.5 * 2^47 rounds to a step and
-// leaves their number in the low word: conversion and rounding instructions take
-// four times an addition's time.  steps is monotone in the logit, so -steps is the
-// histogram's bin.
+// Of a logit d below the maximum (a double, exact): log2 of p over the maximum's, at
+// least -60, in steps of 1/32, and what is left, |rest| <= 1/64.  Adding 1.5 * 2^47
+// rounds to a step and leaves their number in the low word: conversion and rounding
+// instructions take four times an addition's time.  steps is monotone in the logit, so
+// -steps is the histogram's bin.
+struct Octaves {
+  double per_logit, least;  // steps' scale (not 0, so that -inf stays below the rest); the d of -60
+};
 struct Octave {
   int steps;
   double rest;
 };
-__device__ __forceinline__ Octave octave_steps(double y) {
-  y = fmax(y, -60.0);
-  const double t = y + 0x1.8p47;
-  return {(int)(uint32_t)__double_as_longlong(t), y - (t - 0x1.8p47)};
+__device__ __forceinline__ Octave octave_steps(double d, const Octaves& o) {
+  d = fmax(d, o.least);
+  const double t = __builtin_fma(d, o.per_logit, 0x1.8p47);
+  return {(int)(uint32_t)__double_as_longlong(t), __builtin_fma(d, o.per_logit, -(t - 0x1.8p47))};
 }
-// round(2^44 2^y): a table of 2^(j/32), a polynomial of degree 4 (interpolated at
-// Chebyshev nodes, relative error 8e-14), the power of two added to the exponent,
-// and an addition of 2^52, which leaves the integer in the low 52 bits.  The
-// table's entries fill every LDS bank once: no lane waits for another.
-__device__ __forceinline__ uint64_t mass_of_steps(Octave o, const double* exp2) {
-  double p = 0x1.3b2b1bee88b09p-7;
-  p = __builtin_fma(p, o.rest, 0x1.c6b167e571135p-5);
+// round(2^44 2^y) + kMassBias: a table of 2^(j/32) to whose exponent the whole octaves
+// are added, a polynomial of degree 4 (interpolated at Chebyshev nodes, relative error
+// 8e-14), and 2^52 added to their product, which leaves the integer in the low 52
+// bits.  The table's entries fill every LDS bank once: no lane waits for another.
+constexpr uint64_t kMassBias = 0x4330000000000000ull;  // of 2^52
+__device__ __forceinline__ uint64_t biased_mass(Octave o, const uint64_t* exp2) {
+  const uint64_t e = exp2[o.steps & 31];
+  double p = __builtin_fma(0x1.3b2b1bee88b09p-7, o.rest, 0x1.c6b167e571135p-5);
   p = __builtin_fma(p, o.rest, 0x1.ebfbdff8131c3p-3);
   p = __builtin_fma(p, o.rest, 0x1.62e42fef6d01ap-1);
-  p = __builtin_fma(p, o.rest, 0x1.0000000000000p+0) * exp2[o.steps & 31];
-  const int e = (o.steps >> 5) + kMassBits;  // -16 to 44
-  p = __hiloint2double(__double2hiint(p) + e * (1 << 20), __double2loint(p));
-  return (uint64_t)__double_as_longlong(p + 0x1p52) & 0x000FFFFFFFFFFFFFull;
+  p = __builtin_fma(p, o.rest, 0x1.0000000000000p+0);
+  const double scale = __hiloint2double((int)((uint32_t)(e >> 32) + ((uint32_t)o.steps << 15)), (int)(uint32_t)e);
+  return (uint64_t)__double_as_longlong(__builtin_fma(p, scale, 0x1p52));
+}
+__device__ __forceinline__ uint64_t mass_of_steps(Octave o, const uint64_t* exp2) {
+  return biased_mass(o, exp2) & 0x000FFFFFFFFFFFFFull;
 }
 
 // Inclusive prefix sums over the wave, in 12 additions that move the lanes
-// themselves (the compiler moves them first: 36 instructions).  A lane's result is read by the
-// next step two instructions later, as the hardware asks.
+// themselves (the compiler moves them first: 36 instructions).  The hardware asks for
+// two instructions between a lane's result and the next step's read of it.
 __device__ __forceinline__ uint64_t wave_scan_mass(uint64_t v) {
   uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
-#define STEP(CTRL)                                                                     \
-  "s_nop 1\n\tv_add_co_u32_dpp %0, vcc, %0, %0 " CTRL                                  \
-  " bank_mask:0xf bound_ctrl:0\n\ts_nop 1\n\tv_addc_co_u32_dpp %1, vcc, %1, %1, vcc " \
-  CTRL " bank_mask:0xf bound_ctrl:0\n\t"
-  asm(STEP("row_shr:1 row_mask:0xf") STEP("row_shr:2 row_mask:0xf") STEP("row_shr:4 row_mask:0xf")
+#define STEP(CTRL)                                                                           \
+  "v_add_co_u32_dpp %0, vcc, %0, %0 " CTRL " bank_mask:0xf bound_ctrl:0\n\t"                 \
+  "v_addc_co_u32_dpp %1, vcc, %1, %1, vcc " CTRL " bank_mask:0xf bound_ctrl:0\n\ts_nop 0\n\t"
+  asm("s_nop 1\n\t" STEP("row_shr:1 row_mask:0xf") STEP("row_shr:2 row_mask:0xf") STEP("row_shr:4 row_mask:0xf")
           STEP("row_shr:8 row_mask:0xf") STEP("row_bcast:15 row_mask:0xa") STEP("row_bcast:31 row_mask:0xc")
-              "s_nop 1"
+              "s_nop 0"
       : "+v"(lo), "+v"(hi)
       :
       : "vcc");
@@ -117,7 +123,7 @@ struct SampleLds {
   static constexpr int NW = T / 64, SEGS = (IDS ? IDS : kSampleMaxIds) / 256;
   float val[IDS ? IDS : 4];  // the row, each value written and read by one thread
   uint64_t hist[kBins];      // masses or counts
-  double exp2[32];
+  uint64_t exp2[32];
   uint64_t seg[SEGS];  // kept mass of every 256 consecutive ids
   __attribute__((aligned(16))) uint64_t entry[kList];   // the list's pairs
   __attribute__((aligned(16))) uint64_t sorted[kList];  // in order
@@ -127,7 +133,8 @@ struct SampleLds {
   float wmax[NW];
   int found, best;
   uint32_t listed;
-  uint64_t lo, hi, found_before, border;
+  uint64_t lo, hi, found_before;
+  uint32_t border;
 };
 
 // The first of the kBins of L.hist at which the running sum reaches need(sum of
@@ -186,7 +193,9 @@ __device__ __forceinline__ Found locate(Lds& L, Need&& need_of) {
 // row, so instructions per id and pass are what bounds it, and, as every
 // instruction is fetched once per row, the size of the code: the passes are rolled
 // loops and the stages below share one piece of code (unrolled, with values
-// and masses in registers, they took half as long again).
+// and masses in registers, they took half as long again).  32000 fp32 ids, one row, a
+// nucleus: 20 us, of which the maximum 2, the histogram of masses 7, the bin's ids 3, the
+// draw's masses 6.5; the row itself would be read in 0.03 us by the whole chip.
 //
 // Few ids to draw from (at most kList ids in the row, or a top-k of which at most
 // kList ids can be part): all of them in a list, put in order by counting the entries
@@ -359,8 +368,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   }
   const double per_logit = 1.4426950408889634 / (double)temp;  // octaves of p
   auto octave = [&](float v) -> double { return ((double)v - (double)lmax) * per_logit; };
-  auto mass_of = [&](float v) -> uint64_t { return mass_of_steps(octave_steps(octave(v)), L.exp2); };
-  auto bin_of = [&](float v) -> int { return -octave_steps(octave(v)).steps; };
+  const Octaves scale = {fmax(per_logit, 0x1p-900), -60.0 / fmax(per_logit, 0x1p-900)};
+  auto steps_of = [&](float v) -> Octave { return octave_steps((double)v - (double)lmax, scale); };
+  auto mass_of = [&](float v) -> uint64_t { return mass_of_steps(steps_of(v), L.exp2); };
+  auto bin_of = [&](float v) -> int { return -steps_of(v).steps; };
   // Values of bins [first, last] lie within [least_of(last), most_of(first)]: a
   // cheap test before the exact one (a tenth of a bin and rounding errors to spare).
   const float logits_per_bin = 1.0f / (float)(per_logit * kBinsPerOctave), slack = fabsf(lmax) * 0x1p-21f;
@@ -405,7 +416,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   // Ids kept are those at or before (border_v, border_id).
   float border_v = -INFINITY;
   int border_id = 0x7FFFFFFF;
-  // f(j, octaves and masses of the kept ids), for every slot; slots without any are left out
+  // f(j, octaves and masses with kMassBias of the kept ids), for every slot; slots without any are left out
   auto each_mass = [&](auto&& f) {
     const bool all = border_v == -INFINITY;
     each([&](int j, int i, f4v v) {
@@ -428,8 +439,8 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
       uint64_t m[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        o[c] = octave_steps(octave(v[c]));
-        m[c] = mass_of_steps(o[c], L.exp2);
+        o[c] = steps_of(v[c]);
+        m[c] = biased_mass(o[c], L.exp2);
       }
       f(j, o, m);
     });
@@ -521,7 +532,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
           each_mass([&](int, const Octave (&o)[4], const uint64_t (&m)[4]) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              if (m[c]) lds_add(&L.hist[-o[c].steps], m[c]);
+              if (m[c] != kMassBias) lds_add(&L.hist[-o[c].steps], m[c] & ~kMassBias);
           });
         }
         const Found f = locate<T>(L, [&](uint64_t total) {
@@ -589,10 +600,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     uint64_t m = (uint32_t)t < upto ? mass_of(pair_logit(pair)) : 0ull;
     uint64_t before = scan_threads(m, total);
     if (stage == BORDER_P) {
-      if (before < need && need <= before + m) L.border = pair;
+      if (before < need && need <= before + m) L.border = t;
       wg_lds_barrier();
-      border_v = pair_logit(L.border);
-      border_id = pair_id(L.border);
+      border_v = pair_logit(L.sorted[L.border]);
+      border_id = pair_id(L.sorted[L.border]);
       stage = DRAW;
       continue;
     }
@@ -632,7 +643,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     }
     each_mass([&](int j, const Octave (&)[4], const uint64_t (&m)[4]) {
       const uint64_t s = wave_scan_mass((m[0] + m[1]) + (m[2] + m[3]));
-      if (lane == 63) L.seg[j * NW + wave] = s;
+      if (lane == 63) L.seg[j * NW + wave] = s - 256 * kMassBias;
     });
     wg_lds_barrier();
     // Each wave finds the group by itself, 64 PER sums at a time.
