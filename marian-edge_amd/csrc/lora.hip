@@ -5,8 +5,9 @@
 // A_s is [rank_s, K], B_s [N, rank_s] (bf16, stored max_rank apart), x fp32.
 // Two launches: t = c_s A_s x_m (and the rows' quantization when the caller has
 // none), then the int8 product with B_s t added in its epilogue.  Fusing both
-// would repeat A_s x_m in every column workgroup; a third launch for the addition
-// would read and write the output once more.
+// repeats A_s x_m in every column workgroup, which pays for the fewest rows only
+// (one launch, k_lora_one); a third launch for the addition would read and write the
+// output once more.
 //
 // Few rows (a decode step): neighbouring rows belong to different requests, so
 // each row multiplies with its own A_s and B_s on the vector units and reads them
@@ -419,10 +420,52 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
 // 8 (l / 16) .. + 8 of x's row l % 16 and of A's row l % 16, and of the result
 // column (rank) l % 16, rows 4 (l / 16) + r.  A wave reads and splits its x once, 512
 // columns of the row at a time, and multiplies it with each slot of the tile; its two
-// chunks are neighbours, whole cache lines of A.  blockIdx.y: RT tiles of ranks each.
+// chunks are neighbours, whole cache lines of A.  blockIdx.y: RT tiles of ranks each;
+// the first of them quantizes the rows when the caller has no codes, a row per wave,
+// whose second read of x is the cache's (a call of 1459 rows, K 384, N 384, rank 40,
+// 15.8 us, 17.7 with a launch of its own for the codes).
+//
+// A workgroup is a chain of round trips (slot, rank, weights, the waves' sums) that two
+// workgroups a CU hide in part: 16384 x 512, rank 32: 17 us, 2.2 TB/s; a call of 4200
+// rows, K 2048, N 512, rank 24: 37.6 us, 41.1 with four waves a workgroup.
 // ---------------------------------------------------------------------------
 constexpr int kDownRows = 16;
 constexpr int kDownChunks = 2;  // chunks of a wave held at once
+
+// One wave: row m's codes and multiplier, as the row quantization makes them.
+__device__ __forceinline__ void quantize_row(const LoraArgs& g, int64_t m, int lane) {
+  constexpr int COLS = 1024;  // at a time; a longer row is read again for its codes
+  const int K = g.K;
+  const float* x = g.x + m * K;
+  f4v v[COLS / 256];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < COLS / 256; ++j) v[j] = *(const f4v*)(x + min(k0 + 256 * j + 4 * lane, K - 4));
+  };
+  float mx = 0.0f;
+  bool bad = false;
+  for (int k0 = 0; k0 < K; k0 += COLS) {
+    load(k0);
+#pragma unroll
+    for (int j = 0; j < COLS / 256; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx = fmaxf(mx, fabsf(v[j][c]));
+        bad |= !(fabsf(v[j][c]) < INFINITY);
+      }
+  }
+  const float a = row_multiplier(wave_max(mx));
+  if (lane == 0) g.xa[m] = a;
+  if (__any(bad) && lane == 0 && g.err) *g.err = 1;
+  for (int k0 = 0; k0 < K; k0 += COLS) {
+    if (K > COLS) load(k0);
+#pragma unroll
+    for (int j = 0; j < COLS / 256; ++j) {
+      const int k = k0 + 256 * j + 4 * lane;
+      if (k < K) *(uint32_t*)(g.xq + m * K + k) = quantize_pack4(v[j][0], v[j][1], v[j][2], v[j][3], a);
+    }
+  }
+}
 
 template <int RT, int NW>
 __global__ __launch_bounds__(NW * 64) void k_lora_down_tile(LoraArgs g) {
@@ -446,6 +489,8 @@ __global__ __launch_bounds__(NW * 64) void k_lora_down_tile(LoraArgs g) {
   load_x(kDownChunks * wave);
   const RowAdapter ad = row_adapter(g, m0 + (lane & 15) < g.M ? g.slot_of_row[row] : -1, g.err);
   const uint32_t with = (uint32_t)__ballot(ad.rank > 0) & 0xFFFFu;  // rows with an adapter
+  if (g.xq && blockIdx.y == 0)
+    for (int r = wave; r < kDownRows && m0 + r < g.M; r += NW) quantize_row(g, m0 + r, lane);
   f4v sum[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) sum[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -570,12 +615,7 @@ static hipError_t launch_down_tile(const LoraArgs& g, hipStream_t s) {
 
 hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
-  if (lora_few_rows(g.M)) return launch_down_rows(g, s);
-  if (g.xq) {
-    const hipError_t rc = launch_quantize_rows(g.x, g.K, (int)g.M, nullptr, g.K, g.xq, g.K, g.xa, g.err, s);
-    if (rc != hipSuccess) return rc;
-  }
-  return launch_down_tile(g, s);
+  return lora_few_rows(g.M) ? launch_down_rows(g, s) : launch_down_tile(g, s);
 }
 
 // Every workgroup repeats the M rank first products, four at a time on four or
