@@ -480,18 +480,18 @@ int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int6
  * A row with a negative slot has no adapter.  lora_a [slots, max_rank, K] and
  * lora_b [slots, N, max_rank] hold bfloat16 values; slot s uses its first
  * lora_rank[s] (0 to max_rank) rows of A and columns of B, the rest is not used.
- * max_rank is a multiple of 8 up to 128, K a multiple of 64, N below 2^20,
- * M up to 2^26, slots up to 2^20.  A slot at or past
- * `slots`, or a rank out of range, sets *err (device int, may be NULL) to 1 and
- * counts as no adapter; a row's result does not depend on other rows' adapters
- * (the order of its fp32 sums depends on M: a call picks its kernels by the sizes).
+ * max_rank is a multiple of 8 up to 128, K a multiple of 64 up to 2^17, N below
+ * 2^20, M up to 2^26, slots up to 2^20.  A slot at or past `slots`, or a rank out
+ * of range, sets *err (device int, may be NULL) to 1 and counts as no adapter; a
+ * row's result does not depend on other rows' adapters (the order of its fp32 sums
+ * depends on M: a call picks its kernels by the sizes).
  * x (fp32 [M, K]) is always given, it is what the adapters read; xq / xa are its
  * codes and multipliers (both or neither: then the call quantizes x, and a
  * non-finite x sets *err).  The adapters' products are sums of fp32 with exact bf16
  * weights.  out may share memory with x (not with xq, nor with the
  * weights).  x, xq, w, lora_a, lora_b and workspace must be 16-byte aligned.
- * workspace: device memory of marian_hip_q8_linear_lora_workspace bytes that no
- * other call uses meanwhile, or NULL for library scratch.  A call captured into
+ * workspace: device memory of marian_hip_q8_linear_lora_workspace bytes, apart from
+ * every other argument's, that no other call uses meanwhile, or NULL for library scratch.  A call captured into
  * a graph must bring one (the graph owns it for its life). */
 int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa, int64_t M, int64_t K,
                               const int8_t* w, const float* w_mult, const float* bias, int64_t N, int relu,

@@ -194,7 +194,7 @@ LoraWorkspace lora_workspace(int64_t M, int64_t K, int64_t max_rank, bool has_xq
   return w;
 }
 bool lora_sizes_ok(int64_t M, int64_t K, int64_t max_rank) {
-  return M >= 0 && M <= kLoraMaxRows && K > 0 && K <= INT32_MAX && K % 64 == 0 && max_rank > 0 &&
+  return M >= 0 && M <= kLoraMaxRows && K > 0 && K <= kLoraMaxK && K % 64 == 0 && max_rank > 0 &&
          max_rank <= kLoraMaxRank && max_rank % 8 == 0;
 }
 
@@ -332,11 +332,13 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
   const struct { const void* p; size_t bytes; } others[] = {
       {xq, (size_t)M * K}, {xa, (size_t)M * 4}, {w, (size_t)N * K}, {w_mult, (size_t)N * 4}, {bias, (size_t)N * 4},
       {lora_a, table * K}, {lora_b, table * N}, {lora_scale, (size_t)slots * 4}, {lora_rank, (size_t)slots * 4},
-      {slot_of_row, (size_t)M * 4}, {workspace, workspace_bytes}};
-  for (const auto& o : others)
+      {slot_of_row, (size_t)M * 4}};
+  for (const auto& o : others) {
     if (overlap(out_f32, out_bytes, o.p, o.bytes)) return refuse("q8_linear_lora: out overlaps an input that is not x");
-  if (overlap(workspace, workspace_bytes, x, (size_t)M * K * 4))
-    return refuse("q8_linear_lora: the workspace overlaps x");
+    if (overlap(workspace, workspace_bytes, o.p, o.bytes)) return refuse("q8_linear_lora: the workspace overlaps an input");
+  }
+  if (overlap(workspace, workspace_bytes, x, (size_t)M * K * 4) || overlap(workspace, workspace_bytes, out_f32, out_bytes))
+    return refuse("q8_linear_lora: the workspace overlaps x or out");
   hipStream_t s = (hipStream_t)stream;
   LoraArgs l;
   l.x = x;

@@ -58,7 +58,7 @@ def lora_args(**change):
 
 @pytest.mark.parametrize("change, why", [
     (dict(M=-1), "out of range"), (dict(M=1 << 31), "out of range"), (dict(K=0), "out of range"),
-    (dict(K=100), "out of range"), (dict(N=0), "out of range"), (dict(N=1 << 31), "out of range"),
+    (dict(K=100), "out of range"), (dict(K=(1 << 17) + 64), "out of range"), (dict(K=1 << 40), "out of range"), (dict(N=0), "out of range"), (dict(N=1 << 31), "out of range"),
     (dict(max_rank=0), "out of range"), (dict(max_rank=12), "out of range"), (dict(max_rank=136), "out of range"),
     (dict(slots=0), "out of range"), (dict(slots=(1 << 20) + 1), "out of range"), (dict(slots=1 << 31), "out of range"),
     (dict(x=None), "missing"), (dict(xq=None), "missing"), (dict(xa=None), "missing"), (dict(w=None), "missing"),
@@ -69,6 +69,7 @@ def lora_args(**change):
     (dict(ws_bytes=16), "too small"), (dict(M=(1 << 26) + 1), "out of range"), (dict(N=1 << 20), "out of range"),
     (dict(out=at(1) + 16), "overlaps"), (dict(out=at(3)), "overlaps"), (dict(out=at(7) + 32), "overlaps"),
     (dict(out=at(10)), "overlaps"), (dict(out=at(12) + 64), "overlaps"), (dict(ws=at(0) + 256), "overlaps"),
+    (dict(ws=at(1)), "overlaps"), (dict(ws=at(6) - 1024), "overlaps"), (dict(ws=at(10)), "overlaps"), (dict(ws=at(11)), "overlaps"),
 ])
 def test_lora_refuses(pkg, lib, change, why):
     assert lib.marian_hip_q8_linear_lora(*lora_args(**change)) == pkg._lib.ERR_INVALID_INPUT
