@@ -283,9 +283,10 @@ template <int NW, int CT, int KSW>
 __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
   touch_kernargs<sizeof(GemmArgs) + sizeof(LoraArgs)>();
   constexpr int NT = NW * 64, COLS = 16 * CT, LDC = COLS + 1, PER = kOneRows * COLS / NT;
+  constexpr int MAXK = NW * KSW * 64;
   __shared__ int32_t sP[NW][kOneRows * LDC];
   __shared__ __attribute__((aligned(16))) float sT[kOneRows][kLoraMaxRank];
-  __shared__ __attribute__((aligned(16))) int8_t sX[kOneRows * (kOneMaxK + 16)];  // codes made here
+  __shared__ __attribute__((aligned(16))) int8_t sX[kOneRows * (MAXK + 16)];  // codes made here
   __shared__ float sM[kOneRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int M = g.M, K = g.K, n0 = blockIdx.x * COLS, ksteps = K >> 6, kq = (lane >> 4) * 16;
@@ -305,14 +306,14 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
   if (!g.A) {
     for (int m = wave; m < M; m += NW) {
       const float* x = l.x + (int64_t)m * K;
-      f4v v[kOneMaxK / 256];
+      f4v v[MAXK / 256];
       float mx = 0.0f;
       bool bad = false;
 #pragma unroll
-      for (int j = 0; j < kOneMaxK / 256; ++j)
+      for (int j = 0; j < MAXK / 256; ++j)
         if (256 * j < K) v[j] = *(const f4v*)(x + min(256 * j + 4 * lane, K - 4));
 #pragma unroll
-      for (int j = 0; j < kOneMaxK / 256; ++j)
+      for (int j = 0; j < MAXK / 256; ++j)
         if (256 * j < K)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
       if (lane == 0) sM[m] = a;
       if (__any(bad) && lane == 0 && l.err) *l.err = 1;
 #pragma unroll
-      for (int j = 0; j < kOneMaxK / 256; ++j)
+      for (int j = 0; j < MAXK / 256; ++j)
         if (256 * j + 4 * lane < K)
           *(uint32_t*)(sX + m * ldx + 256 * j + 4 * lane) = quantize_pack4(v[j][0], v[j][1], v[j][2], v[j][3], a);
     }

@@ -288,9 +288,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     return v;
   };
   // f(j, first id, four values) for this thread's slots, from memory, the next
-  // BATCH slots requested before BATCH are worked on.
+  // BATCH slots requested before BATCH are worked on (from memory: 256 rows of 100003
+  // bf16 ids 113 us with one, 110 with two, 112 with four, which are more code).
   auto each_read = [&](auto&& f) {
-    constexpr int BATCH = IDS ? NJ : 4;
+    constexpr int BATCH = IDS ? NJ : 2;
     if (full > 0) {
       f4v v[BATCH], next[BATCH];
 #pragma unroll
