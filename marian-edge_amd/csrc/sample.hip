@@ -120,6 +120,8 @@ typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
 
 template <int T, int IDS>
 struct SampleLds {
+  // Ids of a top-k that a list is too short for: one per thread where a thread holds many.
+  static constexpr int PART = T == 1024 ? T : 0;
   static constexpr int NW = T / 64, SEGS = (IDS ? IDS : kSampleMaxIds) / 256;
   float val[IDS ? IDS : 4];  // the row, each value written and read by one thread
   uint64_t hist[kBins];      // masses or counts
@@ -128,6 +130,7 @@ struct SampleLds {
   __attribute__((aligned(16))) uint64_t entry[kList];   // the list's pairs
   __attribute__((aligned(16))) uint64_t sorted[kList];  // in order
   uint32_t ahead[kList];                                // of an entry: how many come before it; zero between uses
+  uint64_t part[PART ? PART : 1];  // pairs
   uint32_t kept[kList / 64];
   uint64_t wsum[NW];
   float wmax[NW];
@@ -208,7 +211,10 @@ __device__ __forceinline__ Found locate(Lds& L, Need&& need_of) {
 // Otherwise the border of top-k, then of top-p among what is left: a histogram over
 // log2 p (of counts, or of masses), the bin where the count or mass is reached, then
 // that bin's ids in order.  A bin of more than kList ids (many equal logits) is cut
-// again by (logit, id) pairs, kBins ways a time, until few are left.
+// again by (logit, id) pairs, kBins ways a time, until few are left.  The ids of a top-k
+// of up to PART go on by themselves, one a thread, in what follows (us: 64 rows of 32000
+// ids, mixed settings, 32.6 without and 27.8 so, 7 of 108601 69 and 50; a nucleus' ids,
+// whose number is not known before, cost more to gather than that saves: 24.0 and 27.8).
 enum Stage { LIST_ALL, LIST_TOP, BORDER_K, BORDER_P, DRAW, DRAWN };
 
 template <int T, int IDS, bool BF16>
@@ -287,12 +293,17 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     }
     return v;
   };
+  constexpr int PART = SampleLds<T, IDS>::PART;
+  bool parted = false;  // the kept ids are the top_k of L.part alone
+  auto part4 = [&]() -> f4v {  // this thread's id there, by itself in a slot
+    return f4v{t < top_k ? pair_logit(L.part[t]) : -INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  };
   // f(j, first id, four values) for this thread's slots, from memory, the next
   // BATCH slots requested before BATCH are worked on (from memory: 256 rows of 100003
   // bf16 ids 113 us with one, 110 with two, 112 with four, which are more code).
   auto each_read = [&](auto&& f) {
     constexpr int BATCH = IDS ? NJ : 2;
-    if (full > 0) {
+    if (full > 0 && !parted) {
       f4v v[BATCH], next[BATCH];
 #pragma unroll
       for (int b = 0; b < BATCH; ++b) v[b] = load4(min(b, full - 1));
@@ -310,12 +321,31 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
         }
       }
     }
-    if (slots > full) f(full, 4 * (full * T + t), clean(last4(full)));
+    if (parted || slots > full) {  // one copy of f
+      int i = 4 * (full * T + t);
+      f4v v;
+      if (parted) {
+        i = pair_id(L.part[min(t, top_k - 1)]);
+        v = part4();
+      } else {
+        v = clean(last4(full));
+      }
+      f(full, i, v);
+    }
   };
   auto each = [&](auto&& f) {
     if constexpr (IDS > 0) {
+      const int last = parted ? 1 : slots;
 #pragma unroll 1
-      for (int j = 0; j < slots; ++j) f(j, 4 * (j * T + t), *(const f4v*)(L.val + 4 * (j * T + t)));
+      for (int j = 0; j < last; ++j) {
+        int i = 4 * (j * T + t);
+        f4v v = *(const f4v*)(L.val + i);
+        if (PART > 0 && parted) {
+          i = pair_id(L.part[min(t, top_k - 1)]);
+          v = part4();
+        }
+        f(j, i, v);
+      }
     } else {
       each_read(f);
     }
@@ -417,7 +447,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   // Ids kept are those at or before (border_v, border_id).
   float border_v = -INFINITY;
   int border_id = 0x7FFFFFFF;
-  // f(j, octaves and masses with kMassBias of the kept ids), for every slot; slots without any are left out
+  // f(j, first id, octaves and masses with kMassBias of the kept ids), for every slot; slots without any are left out
   auto each_mass = [&](auto&& f) {
     const bool all = border_v == -INFINITY;
     each([&](int j, int i, f4v v) {
@@ -443,7 +473,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
         o[c] = steps_of(v[c]);
         m[c] = biased_mass(o[c], L.exp2);
       }
-      f(j, o, m);
+      f(j, i, o, m);
     });
   };
 
@@ -530,7 +560,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
             }
           });
         } else {
-          each_mass([&](int, const Octave (&o)[4], const uint64_t (&m)[4]) {
+          each_mass([&](int, int, const Octave (&o)[4], const uint64_t (&m)[4]) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               if (m[c] != kMassBias) lds_add(&L.hist[-o[c].steps], m[c] & ~kMassBias);
@@ -593,7 +623,21 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
       border_v = pair_logit(L.sorted[need - 1]);
       border_id = pair_id(L.sorted[need - 1]);
       stage = by_p ? BORDER_P : DRAW;
+      if (t == 0) L.listed = 0;
       wg_lds_barrier();  // before the next list
+      if (PART > 0 && top_k <= PART) {
+        each([&](int, int i, f4v v) {
+          if (!__any((v[0] >= border_v) | (v[1] >= border_v) | (v[2] >= border_v) | (v[3] >= border_v))) return;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (v[c] > border_v || (v[c] == border_v && i + c <= border_id)) {  // top_k of them
+              const uint32_t at = lds_add(&L.listed, 1u);
+              if (at < (uint32_t)PART) L.part[at] = pair_of(v[c], (uint32_t)(i + c));
+            }
+        });
+        wg_lds_barrier();
+        parted = true;
+      }
       continue;
     }
     const uint32_t upto = stage == LIST_ALL || stage == LIST_TOP ? (by_k ? min(listed, (uint32_t)top_k) : listed) : listed;
@@ -642,7 +686,11 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
       border_v = least_v;
       border_id = 0x7FFFFFFF;
     }
-    each_mass([&](int j, const Octave (&)[4], const uint64_t (&m)[4]) {
+    each_mass([&](int j, int i, const Octave (&)[4], const uint64_t (&m)[4]) {
+      if (parted) {
+        if (m[0] != kMassBias) lds_add(&L.seg[i >> 8], m[0] - kMassBias);
+        return;
+      }
       const uint64_t s = wave_scan_mass((m[0] + m[1]) + (m[2] + m[3]));
       if (lane == 63) L.seg[j * NW + wave] = s - 256 * kMassBias;
     });

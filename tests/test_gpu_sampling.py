@@ -272,3 +272,20 @@ def test_captured_graph(pkg, dev):
         agree(token.host(), lp.host(), l, u, top_p=p)
     graph.close()
     stream.close()
+
+
+@pytest.mark.parametrize("n", [4097, 32000, 40000])
+def test_top_k_around_the_threads_of_a_row(dev, n):
+    """A top-k too long for the list: on its own up to 1024 ids, with top-p and min-p, ties at the border."""
+    print(f"sample top-k n={n}", flush=True)
+    rng = np.random.default_rng(n)
+    ks = [193, 255, 256, 257, 600, 1000, 1023, 1024, 1025, 2000, n - 1, n]
+    for kind in ("normal", "bf16", "two", "flat", "masked"):
+        rows = 3 * len(ks)
+        l = values_of(kind, rng, rows, n)
+        u = rng.random(rows).astype(np.float32)
+        f = dict(temperature=np.full(rows, 1.1, np.float32), top_k=np.repeat(ks, 3).astype(np.int32),
+                 top_p=np.tile([1, 0.9, 0.6], len(ks)).astype(np.float32), min_p=np.tile([0, 0, 0.02], len(ks)).astype(np.float32))
+        token, lp, err = draw(dev, l, u, **f)
+        assert err == 0
+        agree(token, lp, l, u, **f)
