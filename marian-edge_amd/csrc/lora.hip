@@ -30,7 +30,7 @@ namespace {
 // Few rows, first product: one workgroup of NW waves per row.  Each wave holds
 // the row (lane l: values 8l + 512 j ...) and takes four ranks at a time; NW is
 // as many waves as ranks / 4 keep busy, so that a row's weights are requested at
-// once (200 rows, K 1536, rank 64: 9.6 us with 4 waves).  KJ: row pieces in
+// once (200 rows, K 1536, rank 64: 9.6 us with 4 waves, 6.4 with 16).  KJ: row pieces in
 // registers (K up to 512 KJ); 0: read again for each batch.
 // ---------------------------------------------------------------------------
 constexpr int kDownBatch = 4;  // ranks whose weights are in flight together
@@ -151,17 +151,22 @@ __global__ __launch_bounds__(NW * 64) void k_lora_down_rows(LoraArgs g) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows, the layer: 16 rows and 16 CT columns per workgroup, its NW waves
-// split K (wave w: k-steps w, w + NW, ...) and their exact i32 partials meet in
-// LDS.  The rows' second products go PL neighbouring lanes to an output, 8 ranks
-// (16 bytes of B) each, so that a wave reads B's rows whole; they are requested
-// before the products start, and their sums meet the dequantized outputs in LDS.
+// Few rows, the layer: 16 rows and 16 CT columns per workgroup, its four waves
+// split K (wave w: k-steps w, w + 4, ..., two held at a time) and their exact i32
+// partials meet in LDS.  The rows' second products go two neighbouring lanes to an
+// output, 8 ranks (16 bytes of B) each a time; the first ones are requested before the
+// layer's products start, and the sums meet the dequantized outputs in LDS.  Each
+// row reads its own B, from the L2: 300 rows, N 2048, rank 64, 79 MB, bound it (us a
+// call, K 512: 19.0; four lanes an output 19.5, eight, with whole rows of B a wave
+// but 64 registers of it a thread, 25.2; rank 16: 11.4, 14.0, 23.4).  Few rows or
+// ranks: the two launches.
 // ---------------------------------------------------------------------------
 constexpr int kUpRows = 16;
 
-template <int NW, int CT, int KSW, int PL>
-__global__ __launch_bounds__(NW * 64) void k_lora_rows(GemmArgs g, LoraArgs l) {
+template <int CT>
+__global__ __launch_bounds__(256) void k_lora_rows(GemmArgs g, LoraArgs l) {
   touch_kernargs<sizeof(GemmArgs) + sizeof(LoraArgs)>();
+  constexpr int NW = 4, KSW = 2, PL = 2;  // waves, k-steps held, lanes per output
   constexpr int NT = NW * 64, COLS = 16 * CT, LDC = COLS + 1;
   constexpr int PER = kUpRows * COLS / NT;  // outputs per thread
   constexpr int ITEMS = PER * PL;           // pieces of 8 ranks per thread
@@ -248,11 +253,9 @@ __global__ __launch_bounds__(NW * 64) void k_lora_rows(GemmArgs g, LoraArgs l) {
       }
     };
     add(w[i], min(r8, R - 8));
-    if (r8 >= R) d = 0.0f;  // fewer pieces than lanes
-    if (PL == 8 && r8 + 64 < R) add(*(const uint4*)(b[i] + r8 + 64), r8 + 64);
-    d += __int_as_float(dpp_mov<0xB1>(__float_as_int(d)));                      // over the output's lanes
-    if constexpr (PL >= 4) d += __int_as_float(dpp_mov<0x4E>(__float_as_int(d)));
-    if constexpr (PL >= 8) d += __int_as_float(dpp_mov<0x141>(__float_as_int(d)));  // row_half_mirror
+    if (r8 >= R) d = 0.0f;  // R 8: one piece
+    for (int r = r8 + 8 * PL; r < R; r += 8 * PL) add(*(const uint4*)(b[i] + r), r);
+    d += __int_as_float(dpp_mov<0xB1>(__float_as_int(d)));  // the output's other lane
     if (tid % PL == 0) sD[row * LDC + o % COLS] = d;
   }
   wg_lds_barrier();
@@ -271,7 +274,8 @@ __global__ __launch_bounds__(NW * 64) void k_lora_rows(GemmArgs g, LoraArgs l) {
 
 // ---------------------------------------------------------------------------
 // The fewest rows: both products, and the quantization when the caller has no
-// codes, in one launch of 16 CT columns a workgroup.  Each workgroup repeats its
+// codes, in one launch of 16 CT columns a workgroup (one row, K 512, N 2048, rank 8:
+// 5.2 us, a chain of round trips: x, slot, rank, A, B).  Each workgroup repeats its
 // rows' first products, which costs less than a second launch and the gap before
 // it while they are few (lora_one_launch).  The waves share (row, four ranks)
 // items of the first product.
@@ -600,7 +604,10 @@ static hipError_t launch_down_rows(const LoraArgs& g, hipStream_t s) {
 // While 16-row tiles do not fill the chip, a workgroup per 16 ranks too, and as many
 // waves as a long row has work for: each (512 or 1024 columns, slot) is a round trip
 // to memory (500 rows, K 2048, rank 64, us: 26.5 with eight waves and all ranks, 15.6
-// with a workgroup per 16 ranks).
+// with a workgroup per 16 ranks; 1459 rows, rank 16, eight waves | 16: K 512 11.5 | 12.7,
+// K 2048 25.9 | 21.8).  More tiles: two or four steps of 16 ranks a workgroup, which read
+// x fewer times (K 512, rank 64, one | two | four: 1459 rows 15.6 | 16.0 | 18.4, 5000 27.1 |
+// 24.2 | 23.9, 9000 42.7 | 38.2 | 35.0).
 static hipError_t launch_down_tile(const LoraArgs& g, hipStream_t s) {
   const int64_t tiles = (g.M + kDownRows - 1) / kDownRows;
   const int steps = lora_ldt(g.max_rank) / 16;
@@ -639,26 +646,17 @@ hipError_t launch_lora_one(const GemmArgs& g, const LoraArgs& l, hipStream_t s) 
   return hipGetLastError();
 }
 
-template <int NW, int KSW, int PL>
-static hipError_t launch_rows(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
-  const int rows = (g.M + kUpRows - 1) / kUpRows;
-  if (g.N >= 1024)
-    hipLaunchKernelGGL((k_lora_rows<NW, 2, KSW, PL>), dim3((g.N + 31) / 32, rows), dim3(NW * 64), 0, s, g, l);
-  else
-    hipLaunchKernelGGL((k_lora_rows<4, 1, KSW * NW / 4, PL>), dim3((g.N + 15) / 16, rows), dim3(256), 0, s, g, l);
-  return hipGetLastError();
-}
-template <int PL>
-static hipError_t launch_rows_k(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
-  return g.K <= 512 ? launch_rows<4, 2, PL>(g, l, s) : launch_rows<8, 4, PL>(g, l, s);
-}
-
+// 32 columns a workgroup, 16 where they are few (us a call, 300 rows, rank 16, 16 | 32
+// columns: K 512, N 384 10.5 | 10.6; K 2048, N 2048 25.0 | 20.8).
 hipError_t launch_lora_linear(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
   if (!lora_few_rows(g.M)) return launch_gemm_tile_lora(g, l, s);
-  return l.max_rank <= 16   ? launch_rows_k<2>(g, l, s)
-         : l.max_rank <= 32 ? launch_rows_k<4>(g, l, s)
-                            : launch_rows_k<8>(g, l, s);
+  const int rows = (g.M + kUpRows - 1) / kUpRows;
+  if (g.N >= 1024)
+    hipLaunchKernelGGL(k_lora_rows<2>, dim3((g.N + 31) / 32, rows), dim3(256), 0, s, g, l);
+  else
+    hipLaunchKernelGGL(k_lora_rows<1>, dim3((g.N + 15) / 16, rows), dim3(256), 0, s, g, l);
+  return hipGetLastError();
 }
 
 }  // namespace mh
