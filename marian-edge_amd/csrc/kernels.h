@@ -152,9 +152,6 @@ struct LoraArgs {
   int* err = nullptr;    // set to 1 on a slot or rank out of range (the row then has no adapter)
 };
 constexpr int lora_ldt(int max_rank) { return (max_rank + 15) / 16 * 16; }
-// Whether M rows count as few: each row its own adapter (below), else tiles of
-// rows that mostly share one.
-bool lora_few_rows(int64_t M);
 // Whether a call is one launch (launch_lora_one: no scratch, no codes needed; base.A
 // null: from fp32 rows).
 bool lora_one_launch(int64_t M, int64_t K, int max_rank);

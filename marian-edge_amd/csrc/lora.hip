@@ -575,15 +575,18 @@ __global__ __launch_bounds__(NW * 64) void k_lora_down_tile(LoraArgs g) {
 
 }  // namespace
 
-// us a call, each row its own adapter (above) | tiles; K 2048, N 512, rank 64: 320
-// rows of one request after another 25 | 33, of requests in turn 26 | 111; 1000 rows
-// 51 | 34 and 55 | 118; K 512, N 2048, rank 64, 320 rows: 26 | 17 and 26 | 51.  Which it is
-// the host cannot see; decode batches are in turn and small, prompts neither.
-bool lora_few_rows(int64_t M) { return M <= 320; }
-
-size_t lora_scratch_bytes(int64_t M, int max_rank) {
-  return lora_few_rows(M) ? (size_t)M * max_rank * 4 : (size_t)(M + 31) / 32 * 32 * 3 * lora_ldt(max_rank) * 2;
+// A row's own A and B cost M rank (K + N) values from the L2; tiles cost a chain per
+// distinct slot of their rows.  us a call, rows | tiles, of rows in runs and of rows in
+// turn: K 2048, N 512, rank 64: 160 rows 15 | 21 and 16 | 61, 320 24 | 22 and 26 | 59, 1000
+// 49 | 25 and 53 | 61; K 512, N 2048, rank 16: 320 12 | 11 and 12 | 21, 500 14 | 11 and 14 | 23,
+// 1000 22 | 12 and 22 | 24; K 512, N 512, rank 16: 1000 11 | 11 and 11 | 22.  Which they are
+// the host cannot see: rows while the worse side of either choice is about alike.
+static bool lora_few_rows(const LoraArgs& g) {
+  return g.M <= 320 || (g.M <= 1024 && g.M * g.max_rank * (g.K + g.N) <= 1 << 25);
 }
+
+// t of few rows (4 bytes a value) takes less.
+size_t lora_scratch_bytes(int64_t M, int max_rank) { return (size_t)(M + 31) / 32 * 32 * 3 * lora_ldt(max_rank) * 2; }
 
 template <int NW>
 static hipError_t launch_down_rows_k(const LoraArgs& g, hipStream_t s) {
@@ -623,7 +626,7 @@ static hipError_t launch_down_tile(const LoraArgs& g, hipStream_t s) {
 
 hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
-  return lora_few_rows(g.M) ? launch_down_rows(g, s) : launch_down_tile(g, s);
+  return lora_few_rows(g) ? launch_down_rows(g, s) : launch_down_tile(g, s);
 }
 
 // Every workgroup repeats the M rank first products, four at a time on four or
@@ -650,7 +653,7 @@ hipError_t launch_lora_one(const GemmArgs& g, const LoraArgs& l, hipStream_t s) 
 // columns: K 512, N 384 10.5 | 10.6; K 2048, N 2048 25.0 | 20.8).
 hipError_t launch_lora_linear(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
-  if (!lora_few_rows(g.M)) return launch_gemm_tile_lora(g, l, s);
+  if (!lora_few_rows(l)) return launch_gemm_tile_lora(g, l, s);
   const int rows = (g.M + kUpRows - 1) / kUpRows;
   if (g.N >= 1024)
     hipLaunchKernelGGL(k_lora_rows<2>, dim3((g.N + 31) / 32, rows), dim3(256), 0, s, g, l);

@@ -77,6 +77,9 @@ SHAPES = [  # M, K, N, R, slots, run length
     # many rows: one, two and four tiles of ranks a workgroup, long rows, ranks over several workgroups
     (321, 2048, 520, 64, 4, 40), (340, 1088, 200, 128, 3, 50), (4100, 512, 64, 32, 7, 60), (4099, 64, 128, 64, 3, 1),
     (8200, 192, 96, 64, 6, 100), (8195, 128, 65, 128, 4, 300), (4097, 1152, 70, 128, 5, 90),
+    # rows by themselves up to 1024, tiles before and after
+    (321, 512, 512, 16, 9, 1), (1024, 512, 512, 16, 20, 1), (1025, 512, 512, 16, 20, 3), (1024, 64, 2300, 8, 7, 2),
+    (818, 2048, 512, 16, 5, 4), (1000, 2048, 512, 16, 5, 4),
     # tiles of 128 columns
     (4100, 128, 1000, 16, 6, 70), (4101, 192, 900, 24, 8, 1), (4102, 128, 897, 48, 5, 33),
 ]
