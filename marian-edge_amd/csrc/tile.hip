@@ -287,12 +287,14 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
           }
           return p;
         };
-        if (s.rows == 0xFFFFFFFFu) {  // the whole block
-          y = steps(__builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][2], w0, y, 0, 0, 0));
-          break;
-        }
+        // Summed from zero and then added, for whole blocks too: a row's order of sums is the
+        // same whatever adapters the rows beside it use.
         const v16f none = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         const v16f p = steps(__builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][2], w0, none, 0, 0, 0));
+        if (s.rows == 0xFFFFFFFFu) {
+          y += p;
+          break;
+        }
         const uint32_t m = s.rows >> (4 * half);
 #pragma unroll
         for (int r = 0; r < 16; ++r)  // the bits of p, or zero
