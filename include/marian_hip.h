@@ -477,7 +477,7 @@ int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int6
 /* marian_hip_q8_linear with each row's own low-rank adapter (no counterpart in
  * the reference), s = slot_of_row[m]:
  *   out[m] = (relu of) acc * (1/(xa[m] w_mult)) + bias + lora_scale[s] * B_s (A_s x[m])
- * A row with a negative slot has no adapter.  lora_a [slots, max_rank, K] and
+ * A row with a negative slot has no adapter.  relu keeps a NaN.  lora_a [slots, max_rank, K] and
  * lora_b [slots, N, max_rank] hold bfloat16 values; slot s uses its first
  * lora_rank[s] (0 to max_rank) rows of A and columns of B, the rest is not used.
  * max_rank is a multiple of 8 up to 128, K a multiple of 64 up to 2^17, N below

@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256) void k_lora_rows(GemmArgs g, LoraArgs l) {
 #pragma unroll
     for (int i = 0; i < NW; ++i) iv += sP[i][at];
     float y = dequant(iv, am[k], wm, bias) + sD[at];
-    if (l.relu) y = y > 0.0f ? y : 0.0f;
+    if (l.relu) y = lora_relu(y);
     if (m0 + row < g.M && n0 + tid % COLS < g.N) l.out[(int64_t)(m0 + row) * g.N + n] = y;
   }
 }
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
       }
     }
     y += d;
-    if (l.relu) y = y > 0.0f ? y : 0.0f;
+    if (l.relu) y = lora_relu(y);
     l.out[(int64_t)row * g.N + n] = y;
   }
 }

@@ -21,6 +21,9 @@ __device__ __forceinline__ RowAdapter row_adapter(const LoraArgs& g, int slot, i
   return {s, ok ? r : 0};
 }
 
+// Keeps a NaN, so that a broken adapter does not come out as clean zeros.
+__device__ __forceinline__ float lora_relu(float y) { return y <= 0.0f ? 0.0f : y; }
+
 // A value's three bf16 parts, by truncation: the top 8 bits of the value, of what
 // is left, and of what is left then.  Both differences are exact and the last
 // part holds all that remains, so their sum is the value (down to 2^-126; an

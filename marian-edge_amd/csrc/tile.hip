@@ -309,7 +309,7 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float v = y[4 * q + c];
-          if (RELU) v = v > 0.0f ? v : 0.0f;
+          if (RELU) v = lora_relu(v);
           if (stream)
             __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), out, off, 0, kNt);
           else
