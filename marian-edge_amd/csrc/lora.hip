@@ -125,11 +125,13 @@ __global__ __launch_bounds__(NW * 64) void k_lora_down_rows(LoraArgs g) {
 #pragma unroll
       for (int b = 0; b < kDownBatch; ++b) {
         const uint32_t d[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+        float e = s[b];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s[b] = __builtin_fmaf(p[c >> 1][2 * (c & 1)], __uint_as_float(d[c] << 16), s[b]);
-          s[b] = __builtin_fmaf(p[c >> 1][2 * (c & 1) + 1], __uint_as_float(d[c] & 0xFFFF0000u), s[b]);
+          e = __builtin_fmaf(p[c >> 1][2 * (c & 1)], __uint_as_float(d[c] << 16), e);
+          e = __builtin_fmaf(p[c >> 1][2 * (c & 1) + 1], __uint_as_float(d[c] & 0xFFFF0000u), e);
         }
+        s[b] = 512 * j + 8 * lane < K ? e : s[b];  // past K: weights of another column
       }
     };
     if constexpr (KJ > 0) {

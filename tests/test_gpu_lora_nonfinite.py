@@ -42,7 +42,7 @@ def agree(got, c, x, relu):
     with np.errstate(invalid="ignore"):
         want, bound = dso.lora(x, q, a, c["w"], c["mult"], c["bias"], c["la"], c["lb"], c["scale"], c["rank"], c["slot"],
                                relu)
-    sound = np.isfinite(bound)
+    sound = np.isfinite(bound)  # the rest: not finite, or an infinity that relu took to zero
     assert np.isfinite(want[sound]).all() and (np.abs(got - want)[sound] <= bound[sound]).all()
     assert not sound.all() and np.array_equal(got[~sound], want[~sound], equal_nan=True)
 
@@ -55,6 +55,26 @@ def test_nan_in_an_adapter(dev, M, K, N, R, relu):
     put(c, "la", (3, R - 2, K - 3), np.nan)  # A: in the last eight columns
     put(c, "la", (1, R - 1, 5), np.nan)
     put(c, "lb", (2, 3, 0), np.nan)  # B: one output
+    got, err = run(dev, c, relu)
+    assert err == 0
+    agree(got, c, c["x"], relu)
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+@pytest.mark.parametrize("M, K, N, R", [s for s in SHAPES if s[0] <= 40])
+def test_infinity_in_an_adapter(dev, M, K, N, R, value, relu):
+    print(f"lora infinity M={M} K={K} N={N} R={R} {value} relu={relu}", flush=True)
+    c = broken(M, K, N, R)
+    put(c, "la", (3, R - 2, K - 3), value)
+    put(c, "la", (1, R - 1, 5), value)
+    got, err = run(dev, c, relu)
+    assert err == 0
+    agree(got, c, c["x"], relu)
+    c = broken(M, K, N, R)
+    put(c, "lb", (1, N - 1, 0), value)
+    put(c, "lb", (2, 3, 0), value)
+    put(c, "lb", (3, N // 2, R - 2), value)
     got, err = run(dev, c, relu)
     assert err == 0
     agree(got, c, c["x"], relu)
