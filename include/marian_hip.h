@@ -488,7 +488,8 @@ int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int6
  * x (fp32 [M, K]) is always given, it is what the adapters read; xq / xa are its
  * codes and multipliers (both or neither: then the call quantizes x, and a
  * non-finite x sets *err).  The adapters' products are sums of fp32 with exact bf16
- * weights.  out may share memory with x (not with xq, nor with the
+ * weights; an infinity or NaN in a row or its adapter gives what the formula gives,
+ * in that row alone.  out may share memory with x (not with xq, nor with the
  * weights).  x, xq, w, lora_a, lora_b and workspace must be 16-byte aligned.
  * workspace: device memory of marian_hip_q8_linear_lora_workspace bytes, apart from
  * every other argument's, that no other call uses meanwhile, or NULL for library scratch.  A call captured into

@@ -290,15 +290,33 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
         // Summed from zero and then added, for whole blocks too: a row's order of sums is the
         // same whatever adapters the rows beside it use.
         const v16f none = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        const v16f p = steps(__builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][2], w0, none, 0, 0, 0));
-        if (s.rows == 0xFFFFFFFFu) {
-          y += p;
-          break;
-        }
+        v16f p = steps(__builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][2], w0, none, 0, 0, 0));
         const uint32_t m = s.rows >> (4 * half);
+        if (s.rows != 0xFFFFFFFFu) {  // the bits of p, or zero
 #pragma unroll
-        for (int r = 0; r < 16; ++r)  // the bits of p, or zero
-          y[r] += __uint_as_float(__float_as_uint(p[r]) & (uint32_t)__builtin_amdgcn_sbfe((int)m, 8 * (r >> 2) + (r & 3), 1));
+          for (int r = 0; r < 16; ++r)
+            p[r] = __uint_as_float(__float_as_uint(p[r]) & (uint32_t)__builtin_amdgcn_sbfe((int)m, 8 * (r >> 2) + (r & 3), 1));
+        }
+        float all = p[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) all += p[r];
+        if (__any(!(fabsf(all) < INFINITY))) {  // an infinite weight times a zero part of t made NaN: from t itself
+#pragma unroll 1
+          for (int r = 0; r < 16; ++r) {
+            const int row = 8 * (r >> 2) + (r & 3);
+            if (!((m >> row) & 1) || fabsf(p[r]) < INFINITY) continue;
+            float d = 0.0f;
+            for (int q = 0; q < s.rank; ++q) {
+              const int at = (int)lora_t_index(0, 0, q >> 4, row + 4 * half + 32 * ((q >> 3) & 1), ldt) + (q & 7);
+              const int parts = (int)lora_t_index(0, 1, 0, 0, ldt);
+              const float tv = (bf16_to_f32(tb[at]) + bf16_to_f32(tb[at + parts])) + bf16_to_f32(tb[at + 2 * parts]);
+              d = __builtin_fmaf(tv, bf16_to_f32(s.b[col - 8 * half + q]), d);
+            }
+            p[r] = d;
+          }
+        }
+        y += p;
+        if (s.rows == 0xFFFFFFFFu) break;
         s = next;
 #pragma unroll
         for (int q = 0; q < RS; ++q) w[q] = wn[q];

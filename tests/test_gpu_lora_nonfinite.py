@@ -1,5 +1,5 @@
-"""marian_hip_q8_linear_lora with values that are not finite in a row's own adapter: what the definition gives, in that
-adapter's rows alone."""
+"""marian_hip_q8_linear_lora with values that are not finite in a row's own adapter, or in the row: what the definition
+gives, in those rows alone."""
 
 import numpy as np
 import pytest
@@ -43,7 +43,7 @@ def agree(got, c, x, relu):
         want, bound = dso.lora(x, q, a, c["w"], c["mult"], c["bias"], c["la"], c["lb"], c["scale"], c["rank"], c["slot"],
                                relu)
     sound = np.isfinite(bound)  # the rest: not finite, or an infinity that relu took to zero
-    assert np.isfinite(want[sound]).all() and (np.abs(got - want)[sound] <= bound[sound]).all()
+    assert np.isfinite(want[sound]).all() and (np.abs(got[sound] - want[sound]) <= bound[sound]).all()
     assert not sound.all() and np.array_equal(got[~sound], want[~sound], equal_nan=True)
 
 
@@ -62,7 +62,7 @@ def test_nan_in_an_adapter(dev, M, K, N, R, relu):
 
 @pytest.mark.parametrize("relu", [False, True])
 @pytest.mark.parametrize("value", [np.inf, -np.inf])
-@pytest.mark.parametrize("M, K, N, R", [s for s in SHAPES if s[0] <= 40])
+@pytest.mark.parametrize("M, K, N, R", SHAPES)
 def test_infinity_in_an_adapter(dev, M, K, N, R, value, relu):
     print(f"lora infinity M={M} K={K} N={N} R={R} {value} relu={relu}", flush=True)
     c = broken(M, K, N, R)
@@ -78,3 +78,22 @@ def test_infinity_in_an_adapter(dev, M, K, N, R, value, relu):
     got, err = run(dev, c, relu)
     assert err == 0
     agree(got, c, c["x"], relu)
+
+
+@pytest.mark.parametrize("M, K, N, R", SHAPES)
+def test_a_broken_row(dev, M, K, N, R):
+    """A row that is not finite, its codes given: its own adapter's product takes it up, no other row does."""
+    print(f"lora non-finite rows M={M} K={K} N={N} R={R}", flush=True)
+    D = dev.DeviceArray
+    c = broken(M, K, N, R)
+    x = c["x"].copy()
+    x[0, 7], x[1, 7] = np.inf, -np.inf
+    if M > 2:
+        x[2, 9] = np.nan
+    q, a = dso.quantize_rows(c["x"])
+    out = D.zeros((M, N), np.float32)
+    f = {k: D.from_host(c[k]) for k in ("w", "mult", "bias", "la_bits", "lb_bits", "scale", "rank", "slot")}
+    dev.q8_linear_lora(D.from_host(x), f["w"], f["mult"], f["bias"], f["la_bits"], f["lb_bits"], f["scale"], f["rank"],
+                       f["slot"], out, xq=D.from_host(q), xa=D.from_host(a))
+    dev.synchronize()
+    agree(out.host(), c, x, False)
