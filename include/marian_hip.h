@@ -573,7 +573,9 @@ int marian_hip_sample_logits(const void* logits, int64_t ld, int64_t rows, int64
  * the ids at the same places of cand (ascending), and token[m] is one of those.
  * max_cands (up to 524288) bounds every list's length: a longer list sets *err and
  * only its first max_cands are looked at.  An empty list gives token -1 and
- * logprob -inf; decreasing offsets set *err and count as an empty list. */
+ * logprob -inf; decreasing offsets set *err and count as an empty list.  The call
+ * knows where logits and cand begin, not how long they are: it refuses outputs over
+ * their first values only. */
 int marian_hip_sample_candidates(const float* logits, const uint32_t* cand, const uint32_t* cand_offsets,
                                  int64_t rows, int64_t max_cands, const float* temperature,
                                  const int32_t* top_k, const float* top_p, const float* min_p,

@@ -393,11 +393,13 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
 
 namespace {
 // Outputs of a sampling call share no memory with each other or with the inputs
-// (rows are drawn in any order).  logits_bytes: as far as the host knows them.
+// (rows are drawn in any order).  logits_bytes: as far as the host knows them; of lists
+// it knows the first value and the first id.
 bool sample_overlap(const SampleArgs& g, size_t logits_bytes) {
   const size_t w = (size_t)g.rows * 4;
-  const struct { const void* p; size_t bytes; } ins[] = {{g.logits, logits_bytes}, {g.off, w + 4}, {g.temperature, w},
-                                                         {g.top_k, w}, {g.top_p, w}, {g.min_p, w}, {g.u, w}};
+  const struct { const void* p; size_t bytes; } ins[] = {{g.logits, logits_bytes}, {g.cand, 4}, {g.off, w + 4},
+                                                         {g.temperature, w}, {g.top_k, w}, {g.top_p, w}, {g.min_p, w},
+                                                         {g.u, w}};
   for (const auto& i : ins)
     if (overlap(g.token, w, i.p, i.bytes) || overlap(g.logprob, w, i.p, i.bytes)) return true;
   return overlap(g.token, w, g.logprob, w);
@@ -452,7 +454,7 @@ int marian_hip_sample_candidates(const float* logits, const uint32_t* cand, cons
   g.token = token;
   g.logprob = logprob;
   g.err = err;
-  if (sample_overlap(g, 0)) return refuse("sample_candidates: an output overlaps an input or the other output");
+  if (sample_overlap(g, 4)) return refuse("sample_candidates: an output overlaps an input or the other output");
   return op_status(launch_sample(g, (hipStream_t)stream), "sample_candidates");
 }
 
