@@ -404,8 +404,9 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   auto mass_of = [&](float v) -> uint64_t { return mass_of_steps(steps_of(v), L.exp2); };
   auto bin_of = [&](float v) -> int { return -steps_of(v).steps; };
   // Values of bins [first, last] lie within [least_of(last), most_of(first)]: a
-  // cheap test before the exact one (a tenth of a bin and rounding errors to spare).
-  const float logits_per_bin = 1.0f / (float)(per_logit * kBinsPerOctave), slack = fabsf(lmax) * 0x1p-21f;
+  // cheap test before the exact one (a tenth of a bin, rounding errors and, for bins less
+  // than 2^-126 wide, all of them to spare).
+  const float logits_per_bin = 1.0f / (float)(per_logit * kBinsPerOctave), slack = fabsf(lmax) * 0x1p-21f + 0x1p-114f;
   auto least_of = [&](int b) -> float { return lmax - ((float)b + 0.6f) * logits_per_bin - slack; };
   auto most_of = [&](int b) -> float { return lmax - ((float)b - 0.6f) * logits_per_bin + slack; };
   // The least mass that is at least top_p of the whole: exact, top_p as a multiple of 2^-64.
