@@ -285,16 +285,18 @@ __global__ __launch_bounds__(256) void k_lora_rows(GemmArgs g, LoraArgs l) {
 // it while they are few (lora_one_launch).  The waves share (row, four ranks)
 // items of the first product.
 // ---------------------------------------------------------------------------
-constexpr int kOneRows = 16;
+constexpr int kOneRows = 8;    // of the matrix cores' 16
+constexpr int kOneRanks = 64;  // rows times max_rank
 constexpr int kOneMaxK = 2048;
 
 template <int NW, int CT, int KSW>
 __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
   touch_kernargs<sizeof(GemmArgs) + sizeof(LoraArgs)>();
-  constexpr int NT = NW * 64, COLS = 16 * CT, LDC = COLS + 1, PER = kOneRows * COLS / NT;
+  constexpr int NT = NW * 64, COLS = 16 * CT, LDC = COLS + 1;
   constexpr int MAXK = NW * KSW * 64;
+  static_assert(kOneRows * COLS <= NT, "an output per thread at most");
   __shared__ int32_t sP[NW][kOneRows * LDC];
-  __shared__ __attribute__((aligned(16))) float sT[kOneRows][kLoraMaxRank];
+  __shared__ __attribute__((aligned(16))) float sT[kOneRanks];  // row m's from m max_rank
   __shared__ __attribute__((aligned(16))) int8_t sX[kOneRows * (MAXK + 16)];  // codes made here
   __shared__ float sM[kOneRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -374,7 +376,7 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const float sum = tree_combine_wave(s[b]);
-      if (lane == 0 && r0 + b < l.max_rank) sT[m][r0 + b] = r0 + b < a.rank ? sum * gain : 0.0f;
+      if (lane == 0 && r0 + b < l.max_rank) sT[m * l.max_rank + r0 + b] = r0 + b < a.rank ? sum * gain : 0.0f;
     }
   }
   wg_lds_barrier();
@@ -392,36 +394,35 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, bf[i][c], acc[c], 0, 0, 0);
   }
+  if (lane < 16 * kOneRows / 4) {  // 16 lanes hold four rows
 #pragma unroll
-  for (int c = 0; c < CT; ++c)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sP[wave][((lane >> 4) * 4 + r) * LDC + 16 * c + (lane & 15)] = acc[c][r];
-  wg_lds_barrier();
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int row = tid / COLS + k * (NT / COLS), at = row * LDC + tid % COLS;
-    if (row >= M || n0 + tid % COLS >= g.N) continue;
-    int32_t iv = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) iv += sP[w][at];
-    float y = dequant(iv, g.A ? g.a[row] : sM[row], wm, bias);
-    const RowAdapter a = row_adapter(l, l.slot_of_row[row], nullptr);
-    const uint16_t* b = l.b + ((int64_t)a.slot * g.N + n) * l.max_rank;
-    float d = 0.0f;
-    for (int r8 = 0; r8 < a.rank; r8 += 8) {
-      const uint4 w = *(const uint4*)(b + r8);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const float e = __builtin_fmaf(
-            sT[row][r8 + c], __uint_as_float(c & 1 ? u[c >> 1] & 0xFFFF0000u : u[c >> 1] << 16), d);
-        d = r8 + c < a.rank ? e : d;
-      }
-    }
-    y += d;
-    if (l.relu) y = lora_relu(y);
-    l.out[(int64_t)row * g.N + n] = y;
+      for (int r = 0; r < 4; ++r) sP[wave][((lane >> 4) * 4 + r) * LDC + 16 * c + (lane & 15)] = acc[c][r];
   }
+  wg_lds_barrier();
+  const int row = tid / COLS, at = row * LDC + tid % COLS;
+  if (row >= M || n0 + tid % COLS >= g.N) return;
+  int32_t iv = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) iv += sP[w][at];
+  float y = dequant(iv, g.A ? g.a[row] : sM[row], wm, bias);
+  const RowAdapter a = row_adapter(l, l.slot_of_row[row], nullptr);
+  const uint16_t* b = l.b + ((int64_t)a.slot * g.N + n) * l.max_rank;
+  const float* t = sT + row * l.max_rank;
+  float d = 0.0f;
+  for (int r8 = 0; r8 < a.rank; r8 += 8) {
+    const uint4 w = *(const uint4*)(b + r8);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float e = __builtin_fmaf(t[r8 + c], __uint_as_float(c & 1 ? u[c >> 1] & 0xFFFF0000u : u[c >> 1] << 16), d);
+      d = r8 + c < a.rank ? e : d;
+    }
+  }
+  y += d;
+  if (l.relu) y = lora_relu(y);
+  l.out[(int64_t)row * g.N + n] = y;
 }
 
 // ---------------------------------------------------------------------------
@@ -665,12 +666,13 @@ hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
 // 11.1, 4 of 16 8.5 | 11.4, 2 of 64 14.3 | 11.7, 8 of 16 13.8 | 11.2; K 2048, N 512: 2
 // rows of 16 8.1 | 11.3, 4 of 16 11.9 | 11.2, 1 of 64 12.3 | 11.9.
 bool lora_one_launch(int64_t M, int64_t K, int max_rank) {
-  return M <= kOneRows && K <= kOneMaxK && M * max_rank <= 64 && M * max_rank * K <= 65536;
+  static_assert(kOneRows == kOneRanks / 8, "max_rank is 8 at least");
+  return M * max_rank <= kOneRanks && K <= kOneMaxK && M * max_rank * K <= 65536;
 }
 
 hipError_t launch_lora_one(const GemmArgs& g, const LoraArgs& l, hipStream_t s) {
   if (g.M <= 0) return hipSuccess;
-  if (g.M > kOneRows || g.K > kOneMaxK) return hipErrorInvalidValue;
+  if (!lora_one_launch(g.M, g.K, l.max_rank)) return hipErrorInvalidValue;
   const dim3 wide((g.N + 31) / 32), narrow((g.N + 15) / 16);
   if (g.K <= 512)
     hipLaunchKernelGGL(g.N >= 1024 ? (k_lora_one<4, 2, 2>) : (k_lora_one<4, 1, 2>), g.N >= 1024 ? wide : narrow, dim3(256), 0, s, g, l);
