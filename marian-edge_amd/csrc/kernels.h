@@ -131,7 +131,7 @@ hipError_t launch_gemm_store(const GemmArgs& g, const Epilogue& e, hipStream_t s
 constexpr int kLoraMaxRank = 128;  // and a multiple of 8
 constexpr int kLoraMaxK = 1 << 17;  // 127 * 127 of them fit the int32 sums
 constexpr int64_t kLoraMaxSlots = 1 << 20;
-constexpr int64_t kLoraMaxRows = 1 << 26;  // 512 threads per 16 rows stay below 2^32
+constexpr int64_t kLoraMaxRows = 1 << 26;  // 512 threads per 16 rows: 2^31 (with 1024, less than all of them)
 constexpr int kLoraMaxN = (1 << 20) - 1;  // a tile's output rows stay within 32-bit buffer offsets
 struct LoraArgs {
   const float* x = nullptr;

@@ -647,7 +647,7 @@ static hipError_t launch_down_tile(const LoraArgs& g, hipStream_t s) {
   const int64_t tiles = (g.M + kDownRows - 1) / kDownRows;
   const int steps = lora_ldt(g.max_rank) / 16;
   const int rt = steps == 1 || tiles < 256 ? 1 : steps == 2 || tiles < 512 ? 2 : 4;
-  const bool wide = rt == 1 && g.K > 1024;
+  const bool wide = rt == 1 && g.K > 1024 && tiles < 1 << 22;  // a launch is less than 2^32 threads
   auto kern = wide      ? k_lora_down_tile<1, 16>
               : rt == 1 ? k_lora_down_tile<1, 8>
               : rt == 2 ? k_lora_down_tile<2, 8>
