@@ -17,6 +17,7 @@
 // borders at 2^-24 each would misplace one row in several hundred).
 #include "device_common.h"
 #include "kernels.h"
+#include "ref_expf.h"
 
 #include <algorithm>
 
@@ -30,18 +31,9 @@ constexpr int kLastBin = 46 * kBinsPerOctave;  // ids past it have no mass
 constexpr int kMassBits = 44;                  // mass of the row's maximum
 constexpr int kList = 256;                     // ids put in order at once
 
-// The bits of 2^(44 + j/32) less j * 2^47: with n * 2^47 added (n % 32 = j) those of
-// 2^(44 + n/32).
-__device__ const uint64_t kExp2[32] = {
-    0x42b0000000000000ull, 0x42afd9b0d3158574ull, 0x42afb5586cf9890full, 0x42af9301d0125b51ull,
-    0x42af72b83c7d517bull, 0x42af54873168b9aaull, 0x42af387a6e756238ull, 0x42af1e9df51fdee1ull,
-    0x42af06fe0a31b715ull, 0x42aef1a7373aa9cbull, 0x42aedea64c123422ull, 0x42aece086061892dull,
-    0x42aebfdad5362a27ull, 0x42aeb42b569d4f82ull, 0x42aeab07dd485429ull, 0x42aea47eb03a5585ull,
-    0x42aea09e667f3bcdull, 0x42ae9f75e8ec5f74ull, 0x42aea11473eb0187ull, 0x42aea589994cce13ull,
-    0x42aeace5422aa0dbull, 0x42aeb737b0cdc5e5ull, 0x42aec49182a3f090ull, 0x42aed503b23e255dull,
-    0x42aee89f995ad3adull, 0x42aeff76f2fb5e47ull, 0x42af199bdd85529cull, 0x42af3720dcef9069ull,
-    0x42af5818dcfba487ull, 0x42af7c97337b9b5full, 0x42afa4afa2a490daull, 0x42afd0765b6e4540ull,
-};
+// The bits of 2^(j/32) less j * 2^47: with kMassBits << 52 and n * 2^47 added (n % 32 = j)
+// those of 2^(kMassBits + n/32).
+__constant__ uint64_t kSampleExp2Tab[32] = {MH_EXP2_TABLE_32};
 
 // Of a logit d below the maximum (a double, exact): log2 of p over the maximum's, at
 // least -60, in steps of 1/32, and what is left, |rest| <= 1/64.  Adding 1.5 * 2^47
@@ -365,7 +357,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     L.best = 0x7FFFFFFF;
     L.listed = 0;
   }
-  if (t < 32) L.exp2[t] = kExp2[t];
+  if (t < 32) L.exp2[t] = kSampleExp2Tab[t] + ((uint64_t)kMassBits << 52);
   if (t < kList) L.ahead[t] = 0;
   for (int b = t; b < kBins; b += T) L.hist[b] = 0;
   for (int s = t; s < SampleLds<T, IDS>::SEGS; s += T) L.seg[s] = 0;
