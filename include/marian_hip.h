@@ -484,7 +484,7 @@ int marian_hip_residual_rms_norm(const void* x, int64_t ldx, const void* r, int6
  * 2^20, M up to 2^26, slots up to 2^20.  A slot at or past `slots`, or a rank out
  * of range, sets *err (device int, may be NULL) to 1 and counts as no adapter; a
  * row's result does not depend on other rows' adapters (the order of its fp32 sums
- * depends on M: a call picks its kernels by the sizes).
+ * depends on M: a call picks its kernels by the sizes, and by whether out lies over x).
  * x (fp32 [M, K]) is always given, it is what the adapters read; xq / xa are its
  * codes and multipliers (both or neither: then the call quantizes x, and a
  * non-finite x sets *err).  The adapters' products are sums of fp32 with exact bf16
@@ -558,7 +558,7 @@ int marian_hip_candidate_argmax(const int8_t* xq, const float* xa, int64_t M, in
  * whose running kept mass exceeds u of the kept mass (u rounded down to a multiple
  * of 2^-32); logprob[m] (optional) the logarithm of its share of the kept mass.
  * token and logprob may share no memory with each other or an input.  Masses are multiples of 2^-44 of the
- * maximum's, and their sums exact: ids below 2^-45 of it are never drawn, and a
+ * maximum's, at most two of them from the exponential, and their sums exact: ids below 2^-45 of it are never drawn, and a
  * row's result does not depend on the launch or on other rows.  A row of only
  * -inf and NaN gets id 0 and logprob -inf.  A setting or u out of range sets *err
  * (device int, may be NULL) to 1, and the row's maximum is taken.

@@ -437,7 +437,7 @@ __global__ __launch_bounds__(NW * 64) void k_lora_one(GemmArgs g, LoraArgs l) {
 // 15.8 us, 17.7 with a launch of its own for the codes).
 //
 // A workgroup is a chain of round trips (slot, rank, weights, the waves' sums) that two
-// workgroups a CU hide in part: 16384 x 512, rank 32: 17 us, 2.2 TB/s; a call of 4200
+// workgroups a CU hide in part: 16384 x 512, rank 32: 16 us, 2.3 TB/s; a call of 4200
 // rows, K 2048, N 512, rank 24: 37.6 us, 41.1 with four waves a workgroup.
 // ---------------------------------------------------------------------------
 constexpr int kDownRows = 16;
@@ -612,7 +612,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(4))) vo
 // turn: K 2048, N 512, rank 64: 160 rows 15 | 21 and 16 | 61, 320 24 | 22 and 26 | 59, 1000
 // 49 | 25 and 53 | 61; K 512, N 2048, rank 16: 320 12 | 11 and 12 | 21, 500 14 | 11 and 14 | 23,
 // 1000 22 | 12 and 22 | 24; K 512, N 512, rank 16: 1000 11 | 11 and 11 | 22.  Which they are
-// the host cannot see: rows while the worse side of either choice is about alike.
+// the host cannot see.  Past 320 rows the second bound keeps rows in runs near the tiles' time;
+// rows in turn of high rank pay for it, 59 us instead of 26 at
+// 321 of rank 64 and K 2048, up to about 1000, where both take as long.
 static bool lora_few_rows(const LoraArgs& g) {
   return g.M <= 320 || (g.M <= 1024 && g.M * g.max_rank * (g.K + g.N) <= 1 << 25);
 }
@@ -662,7 +664,7 @@ hipError_t launch_lora_down(const LoraArgs& g, hipStream_t s) {
 }
 
 // Every workgroup repeats the M rank first products, four at a time on four or
-// eight waves.  us a call, one launch | two (K 512, N 2048): 1 row of rank 8 8.0 |
+// eight waves: few of them, and few columns.  us a call, one launch | two (K 512, N 2048): 1 row of rank 8 8.0 |
 // 11.1, 4 of 16 8.5 | 11.4, 2 of 64 14.3 | 11.7, 8 of 16 13.8 | 11.2; K 2048, N 512: 2
 // rows of 16 8.1 | 11.3, 4 of 16 11.9 | 11.2, 1 of 64 12.3 | 11.9.
 bool lora_one_launch(int64_t M, int64_t K, int max_rank) {

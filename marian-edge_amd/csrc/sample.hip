@@ -9,9 +9,9 @@
 // what the kernel looks for.  The drawn id is the first in ascending id order
 // whose running kept mass exceeds u times the kept mass.
 //
-// Mass is an integer, 2^44 exp((l - max) / T) rounded to nearest: sums of up to
-// 2^19 of them are exact in 64 bits, so they do not depend on the order in which
-// lanes and atomics add them, and a row's result is the same whatever the launch
+// Mass is an integer, at most 2 from 2^44 exp((l - max) / T) and 2^44 for the maximum:
+// sums of up to 2^19 of them are exact in 64 bits, so they do not depend on the order in
+// which lanes and atomics add them, and a row's result is the same whatever the launch
 // shape.  The exponential is 2^y by a polynomial in 64 bits: a drawn number
 // close to a border of the running mass needs more than fp32's 24 bits (32000
 // borders at 2^-24 each would misplace one row in several hundred).
@@ -35,7 +35,7 @@ constexpr int kList = 256;                     // ids put in order at once
 // those of 2^(kMassBits + n/32).
 __constant__ uint64_t kSampleExp2Tab[32] = {MH_EXP2_TABLE_32};
 
-// Of a logit d below the maximum (a double, exact): log2 of p over the maximum's, at
+// Of a logit d below the maximum (a double): log2 of p over the maximum's, at
 // least -60, in steps of 1/32, and what is left, |rest| <= 1/64.  Adding 1.5 * 2^47
 // rounds to a step and leaves their number in the low word: conversion and rounding
 // instructions take four times an addition's time.  steps is monotone in the logit, so
@@ -52,10 +52,10 @@ __device__ __forceinline__ Octave octave_steps(double d, const Octaves& o) {
   const double t = __builtin_fma(d, o.per_logit, 0x1.8p47);
   return {(int)(uint32_t)__double_as_longlong(t), __builtin_fma(d, o.per_logit, -(t - 0x1.8p47))};
 }
-// round(2^44 2^y) + kMassBias: a table of 2^(j/32) to whose exponent the whole octaves
-// are added, a polynomial of degree 4 (interpolated at Chebyshev nodes, relative error
-// 8e-14), and 2^52 added to their product, which leaves the integer in the low 52
-// bits.  The table's entries fill every LDS bank once: no lane waits for another.
+// 2^44 2^y as an integer, + kMassBias, by a table (P. T. P. Tang's method, ACM TOMS 15, 1989): a
+// table of 2^(j/32) to whose exponent the whole octaves are added, a polynomial of degree
+// 4 (interpolated at Chebyshev nodes, relative error 8e-14, which is 1.4 of 2^44), and 2^52
+// added to their product, which rounds and leaves the integer in the low 52 bits.  The table's entries fill every LDS bank once: no lane waits for another.
 constexpr uint64_t kMassBias = 0x4330000000000000ull;  // of 2^52
 __device__ __forceinline__ uint64_t biased_mass(Octave o, const uint64_t* exp2) {
   const uint64_t e = exp2[o.steps & 31];
@@ -514,6 +514,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
   int drawn = -1;  // in the thread that holds it: the id, its logit, the kept mass
   float drawn_v = 0.0f;
   uint64_t drawn_of = 0;
+  // A top-k that leaves the list a quarter of room for ids that share its last bin: where they
+  // are too many the list was in vain (us, 64 rows, top-k 192 | 200 | 230, list to 128 | 192 |
+  // 256: of 32000 ids 18.8 18.7 19.1 | 18.1 18.8 19.1 | 18.1 18.5 26.2, of 100003 39.8 39.5 39.6 |
+  // 27.6 39.3 39.6 | 27.7 28.1 51.4; of 4000, with few maxima a thread, 11.0 | 16.6 | 16.6 at 192).
   int stage = n <= kList ? LIST_ALL : !by_k ? (by_p ? BORDER_P : DRAW) : top_k <= kList * 3 / 4 ? LIST_TOP : BORDER_K;
 #pragma unroll 1
   while (stage < DRAW) {
@@ -762,6 +766,11 @@ hipError_t launch(const SampleArgs& g, hipStream_t s) {
 
 }  // namespace
 
+// The row in LDS while it fits, four rows a CU up to 4096 ids.  us a call, 256 threads | 1024 |
+// 1024 that read memory for each pass, a nucleus: 1 row of 4096 ids 11.5 | 12.1 | 13.8, 64 of 1000
+// 8.9 | 10.8 | 12.3, 64 of 4096 13.3 | 13.2 | 15.0, 512 of 4096 15.2 | 24.7 | 28.8 (of 200, all in the
+// list, 1 row 10.3 | 7.8 | 8.8, 512 rows 11.3 | 15.6 | 18.9); in LDS | from memory: 64 rows of 5000 ids
+// 13.7 | 15.6, 512 of 5000 25.8 | 30.0, 1 of 32768 24.5 | 27.6, 512 of 32768 61.8 | 71.0.
 hipError_t launch_sample(const SampleArgs& g, hipStream_t s) {
   if (!g.logits || !g.u || !g.token || g.V <= 0 || g.V > kSampleMaxIds || g.rows < 0 || (g.off && !g.cand))
     return hipErrorInvalidValue;

@@ -182,11 +182,13 @@ __device__ __forceinline__ void tile_store(const GemmArgs& g, const Epilogue& e,
 // v_mfma_f32_32x32x16_bf16 takes rows and columns l % 32 from lane l, k 8 (l / 32)
 // .. + 8, and its results lie where the int8 blocks' do.  Each distinct slot of a
 // block's 32 rows is one product with all rows' t; rows of other slots do not take
-// it.  Up to RS steps of 16 ranks (STEPS: exactly) t stays in registers and a slot's
-// weights are requested while the one before it is multiplied, the first slot's
-// before the dequantization; 0: more steps, read as they are needed past the first.
+// it, and one order of sums (from zero, then added) holds for whole blocks too, so
+// that a row's bits do not depend on the rows beside it.  Up to RS steps of 16 ranks
+// (STEPS: exactly) t stays in registers and a slot's weights are requested while the
+// one before it is multiplied, the first slot's before the dequantization; 0: more
+// steps, read as they are needed past the first.
 // ad: lane l's row's adapter of each block.  Bound by the slots of a block, one after
-// another, and the stores: 16384 x 2048, K 512, rank 32, runs of about 26 rows, 58 us; 36
+// another, and the stores: 16384 x 2048, K 512, rank 32, runs of about 26 rows, 54 us; 42
 // without adapters.
 template <int BM, int MB, int NB, bool RELU, int STEPS>
 __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e, const LoraArgs& l,
@@ -287,8 +289,6 @@ __device__ __forceinline__ void lora_store(const GemmArgs& g, const Epilogue& e,
           }
           return p;
         };
-        // Summed from zero and then added, for whole blocks too: a row's order of sums is the
-        // same whatever adapters the rows beside it use.
         const v16f none = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         v16f p = steps(__builtin_amdgcn_mfma_f32_32x32x16_bf16(t[0][2], w0, none, 0, 0, 0));
         const uint32_t m = s.rows >> (4 * half);
