@@ -52,10 +52,11 @@ __device__ __forceinline__ Octave octave_steps(double d, const Octaves& o) {
   const double t = __builtin_fma(d, o.per_logit, 0x1.8p47);
   return {(int)(uint32_t)__double_as_longlong(t), __builtin_fma(d, o.per_logit, -(t - 0x1.8p47))};
 }
-// 2^44 2^y as an integer, + kMassBias, by a table (P. T. P. Tang's method, ACM TOMS 15, 1989): a
-// table of 2^(j/32) to whose exponent the whole octaves are added, a polynomial of degree
-// 4 (interpolated at Chebyshev nodes, relative error 8e-14, which is 1.4 of 2^44), and 2^52
-// added to their product, which rounds and leaves the integer in the low 52 bits.  The table's entries fill every LDS bank once: no lane waits for another.
+// 2^44 2^y as an integer, + kMassBias, by a table (P. T. P. Tang's method, ACM TOMS 15,
+// 1989): 2^(j/32), to whose exponent the whole octaves are added, times a polynomial of
+// degree 4 (interpolated at Chebyshev nodes, relative error 8e-14, which is 1.4 of 2^44),
+// and 2^52 added to the product, which rounds it and leaves the integer in the low 52
+// bits.  The table's entries fill every LDS bank once: no lane waits for another.
 constexpr uint64_t kMassBias = 0x4330000000000000ull;  // of 2^52
 __device__ __forceinline__ uint64_t biased_mass(Octave o, const uint64_t* exp2) {
   const uint64_t e = exp2[o.steps & 31];
