@@ -60,6 +60,9 @@
  *   marian_hip_q8_linear_lora  a Q8 layer with each row's own low-rank adapter
  *   marian_hip_sample_logits, marian_hip_sample_candidates  temperature, top-k,
  *                              top-p and min-p sampling from given numbers
+ *   marian_hip_paged_plan, marian_hip_paged_append, marian_hip_paged_attention
+ *                              a step over a key-value cache in pages
+ *   marian_hip_verify_drafts   drafted ids accepted or replaced, from given numbers
  * The op-level entry points that need intermediate device buffers keep them
  * in library scratch, one set per (device, stream), kept until the process
  * ends: calls on different streams do not share it, and calls on one stream
@@ -86,12 +89,14 @@
 extern "C" {
 #endif
 
-#define MARIAN_HIP_ABI_VERSION 5 /* 2: marian_hip_attention takes head_dim;
+#define MARIAN_HIP_ABI_VERSION 6 /* 2: marian_hip_attention takes head_dim;
                                     3: the Transformer-SSRU engine, shortlisted translate;
                                     4: warmup, reserve, validate_batch, stats
                                        launched_steps and allocations;
                                     5: residual_rms_norm, q8_linear_lora, sample_logits,
-                                       sample_candidates */
+                                       sample_candidates;
+                                    6: paged_plan, paged_append, paged_attention,
+                                       verify_drafts */
 
 enum {
   MARIAN_HIP_OK = 0,
@@ -502,6 +507,116 @@ int marian_hip_q8_linear_lora(const float* x, const int8_t* xq, const float* xa,
                               size_t workspace_bytes, int* err, void* stream);
 /* Bytes of workspace of a call with these sizes (has_xq: xq / xa are given). */
 int marian_hip_q8_linear_lora_workspace(int64_t M, int64_t K, int64_t max_rank, int has_xq, size_t* bytes);
+
+/* ---- One step of many requests over a paged key-value cache (no counterpart in the
+ * reference, whose caches are one block per sentence) ----
+ *
+ * The key cache is [num_pages, kv_heads, page_size, head_dim], the value cache
+ * [num_pages, kv_heads, head_dim, page_size], fp32 or bfloat16; page_size is a power of
+ * two from 8 to 1024, num_pages * page_size below 2^31.  Slot s is place s % page_size of
+ * page s / page_size.  Row b of block_table [requests, max_blocks] names request b's pages
+ * in order.  The rows of a step are packed: request b's are [cu_rows[b], cu_rows[b + 1]).
+ * A step is paged_plan, paged_append and paged_attention in every layer, then
+ * sample_logits or verify_drafts; the next step's lengths are lengths_out, less what
+ * verify_drafts rejected (lengths may shrink between steps: the pages stay). */
+
+/* Pages, slots and rows of a step.  Request b has lengths[b] tokens, held by the first
+ * pages_held[b] entries of its table row, and brings new_tokens[b] rows; a negative
+ * new_tokens[b]: it has ended, its pages go back (in request order, then table order) on
+ * top of the stack free_pages[0 .. *free_count), its length and pages become 0.  Then
+ * requests are served in order, up to the first that needs more pages than there are,
+ * more table entries than max_blocks or more rows than are left of row_cap: that one and
+ * those after it get no rows and keep what they had, and *served tells how many came
+ * before it (requests: all; a scheduler asks again once pages are back).  Pages are taken
+ * from the top of the stack, a request's in order.
+ * lengths_out, pages_held_out and free_count_out (each may be the input that it follows)
+ * hold the state after the step, cu_rows [requests + 1] the rows; for r below
+ * cu_rows[requests], slot_of_row[r], request_of_row[r] and position_of_row[r] (each [row_cap]
+ * and optional) say where row r's keys go and what it is, past that they are -1.  Entries
+ * of block_table and free_pages that nothing was put into stay as they were.
+ * Counts out of range (a negative length, more pages held than max_blocks, a length past
+ * them, a free count past num_pages, more pages given back than there are) set *err
+ * (device int, may be NULL) to 1 and are not served; a page number out of range sets it too
+ * and gives slot -1.  requests 1 to 8192, max_blocks up to 2^18, row_cap up to 2^18. */
+int marian_hip_paged_plan(const int32_t* lengths, const int32_t* new_tokens, const int32_t* pages_held,
+                          int64_t requests, int64_t page_size, int32_t* block_table, int64_t max_blocks,
+                          int32_t* free_pages, const int32_t* free_count, int64_t num_pages,
+                          int32_t* lengths_out, int32_t* pages_held_out, int32_t* free_count_out,
+                          int32_t* cu_rows, int32_t* slot_of_row, int32_t* request_of_row,
+                          int32_t* position_of_row, int64_t row_cap, int32_t* served, int* err,
+                          void* stream);
+
+/* Row r's keys k[r * ldk ..] and values v[r * ldv ..] (kv_heads * head_dim of them, fp32,
+ * or bfloat16 with in_bf16 != 0, at any value-aligned address) into slot slot_of_row[r] of
+ * the caches, rounded to nearest even where the cache is bfloat16 and the rows are not.  A
+ * negative slot: the row is left out; a slot past the cache sets *err and is left out.
+ * Slots of a call differ (of two rows with one slot either's values stay, one by one).
+ * head_dim 48, 64 or 128, kv_heads up to 128, rows up to 2^18; caches 16-byte aligned. */
+int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int in_bf16,
+                            const int32_t* slot_of_row, int64_t rows, int64_t kv_heads, int64_t head_dim,
+                            void* k_cache, void* v_cache, int cache_bf16, int64_t num_pages,
+                            int64_t page_size, int* err, void* stream);
+
+/* Attention of a step's rows over their requests' pages.  Row i of the n rows of request b
+ * stands at position p = lengths[b] - n + i (lengths[b] counts the step's own rows, whose
+ * keys are in the cache already) and sees the keys j <= p; with window > 0 those with
+ * j > p - window or j < sinks.  Query head h reads key head h / (heads / kv_heads).
+ *   out[row, h] = sum_j softmax_j(scale q k_j) v_j   (fp32, [rows, heads * head_dim])
+ * A row that sees no key (p < 0) gets zeros.  Keys and values that a row does not see do
+ * not change its result, whatever they hold; pages that no row sees are not read.  Scores,
+ * weights and sums are fp32, products exact.  The sums' order depends on the sizes of the
+ * call and on the request's own lengths, not on other requests.  q is fp32, or
+ * bfloat16 with q_bf16 != 0 (then the cache is too); ldq a multiple of 8, ldo of 4.
+ * max_rows (at most 64) and max_keys (at most 2^27) bound every request's rows and length:
+ * they choose the split.  A request past them, or whose rows are not within rows, sets *err
+ * (device int, may be NULL) to 1 and its rows are left as they were, as are rows that
+ * are no request's; a page out of range that a row sees sets *err, its keys count as unseen.
+ * heads a multiple of kv_heads, up to 128; head_dim 48, 64 or 128; scale positive.
+ * q, out, the caches and workspace must be 16-byte aligned.  workspace: device memory of
+ * marian_hip_paged_attention_workspace bytes that no other call uses meanwhile, or
+ * NULL for library scratch; a call captured into a graph must bring one where that is not 0. */
+int marian_hip_paged_attention(const void* q, int64_t ldq, int q_bf16, int64_t rows, const void* k_cache,
+                               const void* v_cache, int cache_bf16, int64_t num_pages, int64_t page_size,
+                               const int32_t* block_table, int64_t max_blocks, const int32_t* lengths,
+                               const int32_t* cu_rows, int64_t requests, int64_t max_rows, int64_t max_keys,
+                               int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
+                               int64_t window, int64_t sinks, float* out, int64_t ldo, void* workspace,
+                               size_t workspace_bytes, int* err, void* stream);
+/* Bytes of workspace of a call with these sizes. */
+int marian_hip_paged_attention_workspace(int64_t rows, int64_t requests, int64_t max_rows, int64_t max_keys,
+                                         int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
+                                         int64_t sinks, size_t* bytes);
+
+/* Drafted ids against the target's logits, so that every id that comes out is distributed
+ * as marian_hip_sample_logits would draw it.  Row r of logits (fp32, or bfloat16 with
+ * in_bf16 != 0, as there) is the target's after the drafts before it; drafts[r], for all
+ * rows of a request but its last, is the id drafted there.  The settings (per request, each
+ * array may be NULL) and what they keep are marian_hip_sample_logits's; p is the share of what is
+ * kept of row r.  With draft_logits, q is the share of what the same settings keep of its row
+ * draft_row[r] (draft_row NULL: r), which the draft was drawn from; without, q is 1 (a
+ * draft that was looked up).  In order, a draft is accepted while u[r] * q < p.  At the first
+ * that is not, one id is drawn from max(p - q, 0) over all ids; after the last draft, one
+ * from p of the last row: the first in ascending order whose running sum exceeds u_draw[b]
+ * of the whole (u_draw rounded down to a multiple of 2^-32; weights are multiples of 2^-51).
+ * token[r] (packed as the rows): the accepted drafts, the drawn id, then -1; accepted[b]:
+ * how many drafts, so accepted[b] + 1 ids come out.  A request without rows: accepted 0.
+ * A row of only -inf and NaN accepts nothing and gives id 0.  A setting out of range sets
+ * *err (device int, may be NULL) and keeps the maximum; a draft, draft row or u out of range
+ * sets it and is not accepted; a u_draw out of range sets it and counts as 0; a request
+ * whose rows are not within rows, or more than max_rows, sets it and has accepted 0 and its
+ * tokens left as they were.  token, accepted and workspace share no memory with each other or an input.
+ * workspace: device memory (8-byte aligned) of marian_hip_verify_drafts_workspace bytes that
+ * no other call uses meanwhile, or NULL for library scratch; a call captured into a graph
+ * must bring one.  V up to 524288, rows and draft rows up to 2^18 and 2^31 - 1. */
+int marian_hip_verify_drafts(const void* logits, int64_t ld, int64_t rows, int64_t V, int in_bf16,
+                             const void* draft_logits, int64_t ld_draft, int64_t draft_rows,
+                             const int32_t* draft_row, const int32_t* drafts, const int32_t* cu_rows,
+                             int64_t requests, int64_t max_rows, const float* temperature,
+                             const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
+                             const float* u_draw, int32_t* token, int32_t* accepted, void* workspace,
+                             size_t workspace_bytes, int* err, void* stream);
+/* Bytes of workspace of a call with these rows (drafted: with draft_logits). */
+int marian_hip_verify_drafts_workspace(int64_t rows, int drafted, size_t* bytes);
 
 /* Variable-length attention: query row i belongs to sequence seq_of_row[i]
  * and attends over key rows [cu_k[s], cu_k[s+1]); max_keys bounds every range

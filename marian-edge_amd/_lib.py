@@ -157,6 +157,15 @@ SIGNATURES = {
     "marian_hip_q8_linear_lora_workspace": (C.c_int, [_I64, _I64, _I64, C.c_int, C.POINTER(_SZ)]),
     "marian_hip_sample_logits": (C.c_int, [_P, _I64, _I64, _I64, C.c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "marian_hip_sample_candidates": (C.c_int, [_P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "marian_hip_paged_plan": (C.c_int, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _P,
+                                        _P]),
+    "marian_hip_paged_append": (C.c_int, [_P, _I64, _P, _I64, C.c_int, _P, _I64, _I64, _I64, _P, _P, C.c_int, _I64, _I64, _P, _P]),
+    "marian_hip_paged_attention": (C.c_int, [_P, _I64, C.c_int, _I64, _P, _P, C.c_int, _I64, _I64, _P, _I64, _P, _P, _I64, _I64,
+                                             _I64, _I64, _I64, _I64, C.c_float, _I64, _I64, _P, _I64, _P, _SZ, _P, _P]),
+    "marian_hip_paged_attention_workspace": (C.c_int, [_I64] * 9 + [C.POINTER(_SZ)]),
+    "marian_hip_verify_drafts": (C.c_int, [_P, _I64, _I64, _I64, C.c_int, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _P,
+                                           _P, _P, _P, _P, _P, _SZ, _P, _P]),
+    "marian_hip_verify_drafts_workspace": (C.c_int, [_I64, C.c_int, C.POINTER(_SZ)]),
     "marian_hip_attention": (C.c_int, [_P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, C.c_int, _P, _I64, _P]),
     "marian_hip_vocab_argmax": (C.c_int, [_P, _P, _I64, _I64, _P, _P, _P, _I64, C.c_uint32, _P, _P, _P]),
     "marian_hip_candidate_argmax": (C.c_int, [_P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _P, _I64, _P, _P, _P, _P]),

@@ -21,7 +21,7 @@ INCLUDE = PKG.parent / "include"
 BUILD_DIR = PKG / "_build"
 LIB = PKG / "libmarian_hip.so"
 SOURCES = ["gemm.hip", "attention.hip", "attnseq.hip", "block.hip", "rows.hip", "ssru.hip", "lngemm.hip", "tile.hip", "rmsnorm.hip",
-           "lora.hip", "sample.hip", "engine.hip", "ops.hip"]
+           "lora.hip", "sample.hip", "paged.hip", "paged_attention.hip", "verify.hip", "engine.hip", "ops.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

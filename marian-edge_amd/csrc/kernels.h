@@ -537,6 +537,121 @@ struct SampleArgs {
 };
 hipError_t launch_sample(const SampleArgs& g, hipStream_t s);
 
+// What a row's settings keep: the ids at or before (border_v, border_id) in the order of logits, whose masses are
+// `total`; border_id alone (kKeptOne, total 1).  total 0: the row has no id to draw.  kKeptInf: the ids of infinite
+// logits, taken as 0, and no others.
+constexpr uint32_t kKeptInf = 1u, kKeptOne = 2u;
+struct RowKept {
+  uint64_t total;
+  float max, border_v;
+  int border_id;
+  uint32_t flags;
+};
+// Records of a verification's rows: target rows 0 .. rows - 1 in kept[0 ..), and with draft_logits the draft row of
+// target row r (row draft_row[r], or r, of draft_logits) in kept[rows + r].  Settings are per request, request b's rows
+// cu[b] .. cu[b + 1).  Rows that nothing is drawn from (no request's; of the drafts a request's last) are left out.
+struct KeptArgs : SampleArgs {
+  const int32_t* cu = nullptr;
+  int requests = 0;
+  const void* draft_logits = nullptr;
+  int64_t ld_draft = 0;
+  const int32_t* draft_row = nullptr;
+  int draft_rows = 0;
+  RowKept* kept = nullptr;
+};
+hipError_t launch_kept(const KeptArgs& g, hipStream_t s);
+
+// Drafted ids against the target's rows: drafts[r], r = cu[b] .. cu[b + 1) - 2, is accepted while u[r] q < p, with
+// p and q its shares of what is kept of target row r and its draft row (without draft_logits q = 1).  From the first row
+// whose draft is not, or a request's last, one id is drawn with u_draw[b]: from max(p - q, 0), or p at the last.
+// token[r]: the accepted drafts, the drawn id, -1; accepted[b] how many drafts.
+struct VerifyArgs : KeptArgs {
+  const int32_t* drafts = nullptr;
+  const float* u_draw = nullptr;
+  int max_rows = 0;  // of a request
+  int32_t* accepted = nullptr;
+};
+hipError_t launch_verify(const VerifyArgs& g, hipStream_t s);
+
+// ---- a step over a paged key-value cache ----
+// Key cache [pages, kv_heads, page_size, head_dim], value cache [pages, kv_heads, head_dim, page_size] of fp32 or bf16;
+// page_size = 1 << page_shift keys.  Row b of the block table names request b's pages in order.
+constexpr int kPageShiftMin = 3, kPageShiftMax = 10;  // eight keys are one load of the attention
+constexpr int kPlanMaxRequests = 8192;                // prefix sums in LDS
+constexpr int kPlanMaxRows = 1 << 18;                 // and those of rows and pages in 32 bits
+constexpr int kMaxBlocks = 1 << 18;
+constexpr int kMaxKvHeads = 128;
+
+// One step's pages, slots and rows.  Request b has lengths[b] tokens in its first pages_held[b] table entries and
+// brings new_tokens[b] rows; negative: it has ended, and its pages go back on top of the stack free_pages[0 ..
+// *free_count).  Requests are served in order, up to the first whose pages or rows there is no room for (*served); page
+// after page is taken from the top of the stack.  lengths_out, pages_held_out and free_count_out may be the inputs.
+struct PagedPlanArgs {
+  const int32_t* lengths = nullptr;
+  const int32_t* new_tokens = nullptr;
+  const int32_t* pages_held = nullptr;
+  int32_t* table = nullptr;  // [requests, max_blocks]
+  int32_t* free_pages = nullptr;
+  const int32_t* free_count = nullptr;
+  int requests = 0, page_shift = 0, max_blocks = 0, num_pages = 0, row_cap = 0;
+  int32_t* lengths_out = nullptr;
+  int32_t* pages_held_out = nullptr;
+  int32_t* free_count_out = nullptr;
+  int32_t* cu_rows = nullptr;          // [requests + 1]
+  int32_t* slot_of_row = nullptr;      // [row_cap], -1 past the last row; these three are optional
+  int32_t* request_of_row = nullptr;
+  int32_t* position_of_row = nullptr;
+  int32_t* served = nullptr;
+  int* err = nullptr;                  // set to 1 on counts or pages out of range
+};
+hipError_t launch_paged_plan(const PagedPlanArgs& g, hipStream_t s);
+
+// Row r's keys and values (k + r ldk, v + r ldv: kv_heads * head_dim values) into slot slot_of_row[r] (negative: none).
+struct PagedAppendArgs {
+  const void* k = nullptr;
+  const void* v = nullptr;
+  int64_t ldk = 0, ldv = 0;
+  int in_bf16 = 0, cache_bf16 = 0;
+  const int32_t* slot_of_row = nullptr;
+  int64_t rows = 0;
+  int kv_heads = 0, head_dim = 0, page_shift = 0, num_pages = 0;
+  void* k_cache = nullptr;
+  void* v_cache = nullptr;
+  int* err = nullptr;  // set to 1 on a slot past the cache
+};
+hipError_t launch_paged_append(const PagedAppendArgs& g, hipStream_t s);
+
+// Attention of the rows cu[b] .. cu[b + 1) of each request over its length[b] keys, the last of them the rows' own;
+// head_dim 48, 64 or 128.  workspace: paged_attention_bytes.
+struct PagedAttnArgs {
+  const void* q = nullptr;
+  int64_t ldq = 0;
+  int q_bf16 = 0, cache_bf16 = 0;
+  const void* k = nullptr;
+  const void* v = nullptr;
+  int page_shift = 0, num_pages = 0;
+  const int32_t* table = nullptr;  // [requests, max_blocks]
+  int max_blocks = 0;
+  const int32_t* length = nullptr;
+  const int32_t* cu = nullptr;
+  int requests = 0, rows = 0, max_rows = 0, max_keys = 0;
+  int heads = 0, kv_heads = 0, group = 0, head_dim = 0;
+  float scale_log2e = 0.0f;
+  int window = 0, sinks = 0;
+  float* out = nullptr;
+  int64_t ldo = 0;
+  int* err = nullptr;  // set to 1 on a request or page out of range
+  // Filled by launch_paged_attention.
+  int qtiles = 0, chunks = 0, chunk_tiles = 0;
+  float* part_o = nullptr;   // [rows, heads, chunks, head_dim]
+  float* part_ml = nullptr;  // [rows, heads, chunks, 2]: reference, sum of weights
+};
+constexpr int kPagedMaxRows = 64;          // of a request
+constexpr int kPagedMaxKeys = 1 << 27;
+bool paged_attention_launchable(const PagedAttnArgs& g);  // within a grid's limits
+size_t paged_attention_bytes(const PagedAttnArgs& g);
+hipError_t launch_paged_attention(const PagedAttnArgs& g, void* workspace, hipStream_t s);
+
 // Reduces argmax partials to token ids (op-level argmax).
 // Records the message marian_hip_last_op_error returns on this thread.
 void note_op_error(const char* msg);

@@ -458,6 +458,300 @@ int marian_hip_sample_candidates(const float* logits, const uint32_t* cand, cons
   return op_status(launch_sample(g, (hipStream_t)stream), "sample_candidates");
 }
 
+namespace {
+// A page of the paged cache: a power of two from 8 to 1024 keys.
+int page_shift_of(int64_t page_size) {
+  for (int s = kPageShiftMin; s <= kPageShiftMax; ++s)
+    if (page_size == (int64_t)1 << s) return s;
+  return -1;
+}
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+// Whether any of `outs` shares memory with another of them or with one of `ins`.
+bool any_overlap(const Span* outs, int n_outs, const Span* ins, int n_ins) {
+  for (int i = 0; i < n_outs; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) return true;
+    for (int j = 0; j < n_ins; ++j)
+      if (overlap(outs[i].p, outs[i].bytes, ins[j].p, ins[j].bytes)) return true;
+  }
+  return false;
+}
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// Bytes of `rows` rows of `width` values, ld values apart.
+size_t rows_bytes(int64_t rows, int64_t ld, int64_t width, size_t value) {
+  return rows > 0 ? ((size_t)(rows - 1) * ld + width) * value : 0;
+}
+}  // namespace
+
+int marian_hip_paged_plan(const int32_t* lengths, const int32_t* new_tokens, const int32_t* pages_held,
+                          int64_t requests, int64_t page_size, int32_t* block_table, int64_t max_blocks,
+                          int32_t* free_pages, const int32_t* free_count, int64_t num_pages,
+                          int32_t* lengths_out, int32_t* pages_held_out, int32_t* free_count_out,
+                          int32_t* cu_rows, int32_t* slot_of_row, int32_t* request_of_row,
+                          int32_t* position_of_row, int64_t row_cap, int32_t* served, int* err,
+                          void* stream) {
+  if (!lengths || !new_tokens || !pages_held || !block_table || !free_pages || !free_count || !lengths_out ||
+      !pages_held_out || !free_count_out || !cu_rows || !served)
+    return refuse("paged_plan: an array is missing");
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return refuse("paged_plan: a page is a power of two from 8 to 1024 keys");
+  if (requests <= 0 || requests > kPlanMaxRequests || max_blocks <= 0 || max_blocks > kMaxBlocks || num_pages <= 0 ||
+      num_pages > INT32_MAX >> shift || row_cap < 0 || row_cap > kPlanMaxRows)
+    return refuse("paged_plan: sizes out of range");
+  const size_t w = (size_t)requests * 4, r = (size_t)row_cap * 4;
+  const Span outs[] = {{block_table, w * max_blocks}, {free_pages, (size_t)num_pages * 4}, {lengths_out, w},
+                       {pages_held_out, w}, {free_count_out, 4}, {cu_rows, w + 4}, {slot_of_row, r},
+                       {request_of_row, r}, {position_of_row, r}, {served, 4}};
+  // An output may be the very input that it follows; any other overlap is refused.
+  const Span ins[] = {{lengths == lengths_out ? nullptr : lengths, w}, {new_tokens, w},
+                      {pages_held == pages_held_out ? nullptr : pages_held, w},
+                      {free_count == free_count_out ? nullptr : free_count, 4}};
+  if (any_overlap(outs, 10, ins, 4)) return refuse("paged_plan: an output overlaps an input or another output");
+  PagedPlanArgs g;
+  g.lengths = lengths;
+  g.new_tokens = new_tokens;
+  g.pages_held = pages_held;
+  g.table = block_table;
+  g.free_pages = free_pages;
+  g.free_count = free_count;
+  g.requests = (int)requests;
+  g.page_shift = shift;
+  g.max_blocks = (int)max_blocks;
+  g.num_pages = (int)num_pages;
+  g.row_cap = (int)row_cap;
+  g.lengths_out = lengths_out;
+  g.pages_held_out = pages_held_out;
+  g.free_count_out = free_count_out;
+  g.cu_rows = cu_rows;
+  g.slot_of_row = slot_of_row;
+  g.request_of_row = request_of_row;
+  g.position_of_row = position_of_row;
+  g.served = served;
+  g.err = err;
+  return op_status(launch_paged_plan(g, (hipStream_t)stream), "paged_plan");
+}
+
+namespace {
+// Checks that the cache's sizes and addresses are what the kernels take; the reason, or null.
+const char* paged_cache_refusal(const void* k_cache, const void* v_cache, int64_t num_pages, int shift, int64_t kv_heads,
+                                int64_t head_dim) {
+  if (!k_cache || !v_cache) return "a cache is missing";
+  if (shift < 0) return "a page is a power of two from 8 to 1024 keys";
+  if (num_pages <= 0 || num_pages > INT32_MAX >> shift) return "sizes out of range";
+  if (kv_heads <= 0 || kv_heads > kMaxKvHeads) return "sizes out of range";
+  if (head_dim != 48 && head_dim != 64 && head_dim != 128) return "head_dim is 48, 64 or 128";
+  if (!aligned16(k_cache) || !aligned16(v_cache)) return "the caches must be 16-byte aligned";
+  return nullptr;
+}
+int refuse_as(const char* op, const char* why) {
+  g_op_error = std::string(op) + ": " + why;
+  return MARIAN_HIP_ERR_INVALID_INPUT;
+}
+}  // namespace
+
+int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int in_bf16,
+                            const int32_t* slot_of_row, int64_t rows, int64_t kv_heads, int64_t head_dim,
+                            void* k_cache, void* v_cache, int cache_bf16, int64_t num_pages,
+                            int64_t page_size, int* err, void* stream) {
+  const int shift = page_shift_of(page_size);
+  if (const char* why = paged_cache_refusal(k_cache, v_cache, num_pages, shift, kv_heads, head_dim))
+    return refuse_as("paged_append", why);
+  if (!k || !v || !slot_of_row) return refuse("paged_append: an array is missing");
+  const int64_t width = kv_heads * head_dim;
+  if (rows < 0 || rows > kPlanMaxRows || ldk < width || ldv < width || ldk > kMaxStride || ldv > kMaxStride)
+    return refuse("paged_append: sizes out of range");
+  const size_t value = in_bf16 ? 2 : 4, cache = (size_t)num_pages * page_size * width * (cache_bf16 ? 2 : 4);
+  if ((uintptr_t)k % value || (uintptr_t)v % value) return refuse("paged_append: k or v is not aligned to its values");
+  const Span outs[] = {{k_cache, cache}, {v_cache, cache}};
+  const Span ins[] = {{k, rows_bytes(rows, ldk, width, value)}, {v, rows_bytes(rows, ldv, width, value)},
+                      {slot_of_row, (size_t)rows * 4}};
+  if (any_overlap(outs, 2, ins, 3)) return refuse("paged_append: a cache overlaps an input or the other cache");
+  PagedAppendArgs g;
+  g.k = k;
+  g.v = v;
+  g.ldk = ldk;
+  g.ldv = ldv;
+  g.in_bf16 = in_bf16 ? 1 : 0;
+  g.cache_bf16 = cache_bf16 ? 1 : 0;
+  g.slot_of_row = slot_of_row;
+  g.rows = rows;
+  g.kv_heads = (int)kv_heads;
+  g.head_dim = (int)head_dim;
+  g.page_shift = shift;
+  g.num_pages = (int)num_pages;
+  g.k_cache = k_cache;
+  g.v_cache = v_cache;
+  g.err = err;
+  return op_status(launch_paged_append(g, (hipStream_t)stream), "paged_append");
+}
+
+namespace {
+// The sizes of a paged attention call; the reason why they are refused, or null.
+const char* paged_attention_sizes(PagedAttnArgs& g, int64_t rows, int64_t requests, int64_t max_rows, int64_t max_keys,
+                                  int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks) {
+  if (rows < 0 || rows > kPlanMaxRows || requests < 0 || requests > kPlanMaxRequests || max_rows <= 0 ||
+      max_rows > kPagedMaxRows || max_keys <= 0 || max_keys > kPagedMaxKeys || window < 0 || window > INT32_MAX / 2 ||
+      sinks < 0 || sinks > INT32_MAX / 2)
+    return "sizes out of range";
+  if (kv_heads <= 0 || kv_heads > kMaxKvHeads || heads <= 0 || heads > kMaxKvHeads || heads % kv_heads)
+    return "heads is a multiple of kv_heads, both at most 128";
+  if (head_dim != 48 && head_dim != 64 && head_dim != 128) return "head_dim is 48, 64 or 128";
+  g.rows = (int)rows;
+  g.requests = (int)requests;
+  g.max_rows = (int)max_rows;
+  g.max_keys = (int)max_keys;
+  g.heads = (int)heads;
+  g.kv_heads = (int)kv_heads;
+  g.group = (int)(heads / kv_heads);
+  g.head_dim = (int)head_dim;
+  g.window = (int)window;
+  g.sinks = (int)sinks;
+  if (!paged_attention_launchable(g)) return "too many requests, rows and heads for one call";
+  return nullptr;
+}
+}  // namespace
+
+int marian_hip_paged_attention_workspace(int64_t rows, int64_t requests, int64_t max_rows, int64_t max_keys,
+                                         int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
+                                         int64_t sinks, size_t* bytes) {
+  PagedAttnArgs g;
+  if (!bytes) return refuse("paged_attention_workspace: bytes is missing");
+  if (const char* why = paged_attention_sizes(g, rows, requests, max_rows, max_keys, heads, kv_heads, head_dim, window, sinks))
+    return refuse_as("paged_attention_workspace", why);
+  *bytes = paged_attention_bytes(g);
+  return MARIAN_HIP_OK;
+}
+
+int marian_hip_paged_attention(const void* q, int64_t ldq, int q_bf16, int64_t rows, const void* k_cache,
+                               const void* v_cache, int cache_bf16, int64_t num_pages, int64_t page_size,
+                               const int32_t* block_table, int64_t max_blocks, const int32_t* lengths,
+                               const int32_t* cu_rows, int64_t requests, int64_t max_rows, int64_t max_keys,
+                               int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
+                               int64_t window, int64_t sinks, float* out, int64_t ldo, void* workspace,
+                               size_t workspace_bytes, int* err, void* stream) {
+  PagedAttnArgs g;
+  const int shift = page_shift_of(page_size);
+  if (const char* why = paged_attention_sizes(g, rows, requests, max_rows, max_keys, heads, kv_heads, head_dim, window, sinks))
+    return refuse_as("paged_attention", why);
+  if (const char* why = paged_cache_refusal(k_cache, v_cache, num_pages, shift, kv_heads, head_dim))
+    return refuse_as("paged_attention", why);
+  if (!q || !block_table || !lengths || !cu_rows || !out) return refuse("paged_attention: an array is missing");
+  const int64_t width = heads * head_dim;
+  if (max_blocks <= 0 || max_blocks > kMaxBlocks || ldq < width || ldo < width || ldq > kMaxStride || ldo > kMaxStride ||
+      ldq % 8 || ldo % 4)
+    return refuse("paged_attention: sizes or strides out of range");
+  if (!(scale > 0.0f) || !(scale <= 1e30f)) return refuse("paged_attention: scale is not positive and finite");
+  if (q_bf16 && !cache_bf16) return refuse("paged_attention: bfloat16 queries need a bfloat16 cache");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace))
+    return refuse("paged_attention: q, out and workspace must be 16-byte aligned");
+  const size_t bytes = paged_attention_bytes(g), cache = (size_t)num_pages * page_size * kv_heads * head_dim * (cache_bf16 ? 2 : 4);
+  const Span outs[] = {{out, rows_bytes(rows, ldo, width, 4)}, {workspace, workspace_bytes}};
+  const Span ins[] = {{q, rows_bytes(rows, ldq, width, q_bf16 ? 2 : 4)}, {k_cache, cache}, {v_cache, cache},
+                      {block_table, (size_t)requests * max_blocks * 4}, {lengths, (size_t)requests * 4},
+                      {cu_rows, (size_t)(requests + 1) * 4}};
+  if (any_overlap(outs, 2, ins, 6)) return refuse("paged_attention: out or the workspace overlaps an input or each other");
+  if (rows == 0 || requests == 0) return MARIAN_HIP_OK;
+  hipStream_t s = (hipStream_t)stream;
+  if (workspace) {
+    if (workspace_bytes < bytes) return refuse("paged_attention: the workspace is too small");
+  } else if (bytes) {
+    // A graph would go on using scratch that a later call may replace.
+    if (capturing(s)) return refuse("paged_attention: a call that is captured into a graph needs a workspace");
+    workspace = op_scratch(3, bytes, s);
+    if (!workspace) return op_status(hipErrorOutOfMemory, "paged_attention scratch");
+  }
+  g.q = q;
+  g.ldq = ldq;
+  g.q_bf16 = q_bf16 ? 1 : 0;
+  g.cache_bf16 = cache_bf16 ? 1 : 0;
+  g.k = k_cache;
+  g.v = v_cache;
+  g.page_shift = shift;
+  g.num_pages = (int)num_pages;
+  g.table = block_table;
+  g.max_blocks = (int)max_blocks;
+  g.length = lengths;
+  g.cu = cu_rows;
+  g.scale_log2e = scale * 1.4426950408889634f;
+  g.out = out;
+  g.ldo = ldo;
+  g.err = err;
+  return op_status(launch_paged_attention(g, workspace, s), "paged_attention");
+}
+
+namespace {
+size_t verify_bytes(int64_t rows, bool drafted) { return (size_t)rows * (drafted ? 2 : 1) * sizeof(RowKept); }
+}  // namespace
+
+int marian_hip_verify_drafts_workspace(int64_t rows, int drafted, size_t* bytes) {
+  if (!bytes) return refuse("verify_drafts_workspace: bytes is missing");
+  if (rows < 0 || rows > kPlanMaxRows) return refuse("verify_drafts_workspace: sizes out of range");
+  *bytes = verify_bytes(rows, drafted != 0);
+  return MARIAN_HIP_OK;
+}
+
+int marian_hip_verify_drafts(const void* logits, int64_t ld, int64_t rows, int64_t V, int in_bf16,
+                             const void* draft_logits, int64_t ld_draft, int64_t draft_rows,
+                             const int32_t* draft_row, const int32_t* drafts, const int32_t* cu_rows,
+                             int64_t requests, int64_t max_rows, const float* temperature,
+                             const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
+                             const float* u_draw, int32_t* token, int32_t* accepted, void* workspace,
+                             size_t workspace_bytes, int* err, void* stream) {
+  if (!logits || !drafts || !cu_rows || !u || !u_draw || !token || !accepted)
+    return refuse("verify_drafts: an array is missing");
+  if (rows < 0 || rows > kPlanMaxRows || V <= 0 || V > kSampleMaxIds || ld < V || ld > kMaxStride || requests < 0 ||
+      requests > kPlanMaxRequests || max_rows <= 0 || max_rows > kPlanMaxRows)
+    return refuse("verify_drafts: sizes out of range");
+  if (draft_logits && (draft_rows < 0 || draft_rows > INT32_MAX || ld_draft < V || ld_draft > kMaxStride))
+    return refuse("verify_drafts: sizes of the draft rows out of range");
+  if (!draft_logits && draft_row) return refuse("verify_drafts: draft_row without draft_logits");
+  if ((uintptr_t)workspace & 7) return refuse("verify_drafts: the workspace must be 8-byte aligned");
+  const size_t value = in_bf16 ? 2 : 4, bytes = verify_bytes(rows, draft_logits != nullptr);
+  const size_t w = (size_t)requests * 4, r = (size_t)rows * 4;
+  const Span outs[] = {{token, r}, {accepted, w}, {workspace, workspace_bytes}};
+  const Span ins[] = {{logits, rows_bytes(rows, ld, V, value)}, {draft_logits, rows_bytes(draft_rows, ld_draft, V, value)},
+                      {draft_row, r}, {drafts, r}, {cu_rows, w + 4}, {temperature, w}, {top_k, w}, {top_p, w}, {min_p, w},
+                      {u, r}, {u_draw, w}};
+  if (any_overlap(outs, 3, ins, 11)) return refuse("verify_drafts: an output or the workspace overlaps another array");
+  if (requests == 0) return MARIAN_HIP_OK;
+  hipStream_t s = (hipStream_t)stream;
+  if (workspace) {
+    if (workspace_bytes < bytes) return refuse("verify_drafts: the workspace is too small");
+  } else if (bytes) {
+    if (capturing(s)) return refuse("verify_drafts: a call that is captured into a graph needs a workspace");
+    workspace = op_scratch(3, bytes, s);
+    if (!workspace) return op_status(hipErrorOutOfMemory, "verify_drafts scratch");
+  }
+  VerifyArgs g;
+  g.logits = logits;
+  g.ld = ld;
+  g.bf16 = in_bf16 ? 1 : 0;
+  g.rows = (int)rows;
+  g.V = (int)V;
+  g.temperature = temperature;
+  g.top_k = top_k;
+  g.top_p = top_p;
+  g.min_p = min_p;
+  g.u = u;
+  g.token = token;
+  g.err = err;
+  g.cu = cu_rows;
+  g.requests = (int)requests;
+  g.draft_logits = draft_logits;
+  g.ld_draft = ld_draft;
+  g.draft_row = draft_row;
+  g.draft_rows = (int)draft_rows;
+  g.kept = (RowKept*)workspace;
+  g.drafts = drafts;
+  g.u_draw = u_draw;
+  g.max_rows = (int)max_rows;
+  g.accepted = accepted;
+  return op_status(launch_verify(g, s), "verify_drafts");
+}
+
 int marian_hip_attention(const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,
                          const int32_t* seq_of_row, const uint32_t* cu_k, int64_t n_seqs,
                          int64_t rows, int64_t heads, int64_t head_dim, int64_t max_keys,

@@ -17,9 +17,10 @@
 // borders at 2^-24 each would misplace one row in several hundred).
 #include "device_common.h"
 #include "kernels.h"
-#include "ref_expf.h"
+#include "mass.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mh {
 namespace {
@@ -28,85 +29,7 @@ constexpr uint32_t kNothing = 0x007FFFFFu;     // argmax_order of -inf: ids that
 constexpr int kBins = 2048;
 constexpr int kBinsPerOctave = 32;             // of p, in the histograms over log2 p
 constexpr int kLastBin = 46 * kBinsPerOctave;  // ids past it have no mass
-constexpr int kMassBits = 44;                  // mass of the row's maximum
 constexpr int kList = 256;                     // ids put in order at once
-
-// The bits of 2^(j/32) less j * 2^47: with kMassBits << 52 and n * 2^47 added (n % 32 = j)
-// those of 2^(kMassBits + n/32).
-__constant__ uint64_t kSampleExp2Tab[32] = {MH_EXP2_TABLE_32};
-
-// Of a logit d below the maximum (a double): log2 of p over the maximum's, at
-// least -60, in steps of 1/32, and what is left, |rest| <= 1/64.  Adding 1.5 * 2^47
-// rounds to a step and leaves their number in the low word: conversion and rounding
-// instructions take four times an addition's time.  steps is monotone in the logit, so
-// -steps is the histogram's bin.
-struct Octaves {
-  double per_logit, least;  // steps' scale (not 0, so that -inf stays below the rest); the d of -60
-};
-struct Octave {
-  int steps;
-  double rest;
-};
-__device__ __forceinline__ Octave octave_steps(double d, const Octaves& o) {
-  d = fmax(d, o.least);
-  const double t = __builtin_fma(d, o.per_logit, 0x1.8p47);
-  return {(int)(uint32_t)__double_as_longlong(t), __builtin_fma(d, o.per_logit, -(t - 0x1.8p47))};
-}
-// 2^44 2^y as an integer, + kMassBias, by a table (P. T. P. Tang's method, ACM TOMS 15,
-// 1989): 2^(j/32), to whose exponent the whole octaves are added, times a polynomial of
-// degree 4 (interpolated at Chebyshev nodes, relative error 8e-14, which is 1.4 of 2^44),
-// and 2^52 added to the product, which rounds it and leaves the integer in the low 52
-// bits.  The table's entries fill every LDS bank once: no lane waits for another.
-constexpr uint64_t kMassBias = 0x4330000000000000ull;  // of 2^52
-__device__ __forceinline__ uint64_t biased_mass(Octave o, const uint64_t* exp2) {
-  const uint64_t e = exp2[o.steps & 31];
-  double p = __builtin_fma(0x1.3b2b1bee88b09p-7, o.rest, 0x1.c6b167e571135p-5);
-  p = __builtin_fma(p, o.rest, 0x1.ebfbdff8131c3p-3);
-  p = __builtin_fma(p, o.rest, 0x1.62e42fef6d01ap-1);
-  p = __builtin_fma(p, o.rest, 0x1.0000000000000p+0);
-  const double scale = __hiloint2double((int)((uint32_t)(e >> 32) + ((uint32_t)o.steps << 15)), (int)(uint32_t)e);
-  return (uint64_t)__double_as_longlong(__builtin_fma(p, scale, 0x1p52));
-}
-__device__ __forceinline__ uint64_t mass_of_steps(Octave o, const uint64_t* exp2) {
-  return biased_mass(o, exp2) & 0x000FFFFFFFFFFFFFull;
-}
-
-// Inclusive prefix sums over the wave, in 12 additions that move the lanes
-// themselves (the compiler moves them first: 36 instructions).  The hardware asks for
-// two instructions between a lane's result and the next step's read of it.
-__device__ __forceinline__ uint64_t wave_scan_mass(uint64_t v) {
-  uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
-#define STEP(CTRL)                                                                           \
-  "v_add_co_u32_dpp %0, vcc, %0, %0 " CTRL " bank_mask:0xf bound_ctrl:0\n\t"                 \
-  "v_addc_co_u32_dpp %1, vcc, %1, %1, vcc " CTRL " bank_mask:0xf bound_ctrl:0\n\ts_nop 0\n\t"
-  asm("s_nop 1\n\t" STEP("row_shr:1 row_mask:0xf") STEP("row_shr:2 row_mask:0xf") STEP("row_shr:4 row_mask:0xf")
-          STEP("row_shr:8 row_mask:0xf") STEP("row_bcast:15 row_mask:0xa") STEP("row_bcast:31 row_mask:0xc")
-              "s_nop 0"
-      : "+v"(lo), "+v"(hi)
-      :
-      : "vcc");
-#undef STEP
-  return ((uint64_t)hi << 32) | lo;
-}
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
-  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32) |
-         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
-}
-
-template <class V>
-__device__ __forceinline__ V lds_add(V* p, V v) {
-  return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-}
-
-// Ids in descending order of this pair: logit, then ascending id.
-__device__ __forceinline__ uint64_t pair_of(float v, uint32_t id) {
-  return ((uint64_t)argmax_order(v) << 32) | (0xFFFFFFFFu - id);
-}
-__device__ __forceinline__ float order_logit(uint32_t k) {  // inverse of argmax_order
-  return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
-}
-__device__ __forceinline__ float pair_logit(uint64_t p) { return order_logit((uint32_t)(p >> 32)); }
-__device__ __forceinline__ int pair_id(uint64_t p) { return (int)(0xFFFFFFFFu - (uint32_t)p); }
 
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
@@ -210,13 +133,35 @@ __device__ __forceinline__ Found locate(Lds& L, Need&& need_of) {
 // whose number is not known before, cost more to gather than that saves: 24.0 and 27.8).
 enum Stage { LIST_ALL, LIST_TOP, BORDER_K, BORDER_P, DRAW, DRAWN };
 
-template <int T, int IDS, bool BF16>
-__global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
+//
+// KEPT: nothing is drawn; a row's record (RowKept) says what its request's settings keep.  Workgroup r is target row r,
+// workgroup rows + r the draft row that goes with it.
+template <int T, int IDS, bool BF16, bool KEPT>
+__global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs, SampleArgs> g) {
   constexpr int NW = T / 64, NJ = IDS / (4 * T);  // slots of four ids per thread
   static_assert(NJ * 4 * T == IDS && T >= kList && kBins % T == 0, "whole slots");
   __shared__ __attribute__((aligned(16))) SampleLds<T, IDS> L;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t row = blockIdx.x;
+  int64_t set = row;  // of the settings
+  if constexpr (KEPT) {
+    const int r = (int)(row < g.rows ? row : row - g.rows);
+    if (t == 0) L.found = -1;
+    wg_lds_barrier();
+    int last = 0;
+    for (int b = t; b < g.requests; b += T) {
+      const int end = g.cu[b + 1];
+      if (g.cu[b] <= r && r < end) {
+        L.found = b;
+        L.best = end - 1;
+      }
+    }
+    wg_lds_barrier();
+    set = __builtin_amdgcn_readfirstlane(L.found);
+    last = __builtin_amdgcn_readfirstlane(L.best);
+    if (set < 0 || (row >= g.rows && r == last)) return;  // no request's, or a request's last row: nothing was drafted after it
+    wg_lds_barrier();  // found and best are used again
+  }
 
   // ---- the row and its settings (uniform) ----
   uint32_t o0 = 0;
@@ -229,20 +174,31 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     n = (int)min(max(len, (int64_t)0), (int64_t)g.V);
   }
   {
-    const int64_t first = g.off ? (int64_t)o0 : row * g.ld;
+    int64_t first = g.off ? (int64_t)o0 : row * g.ld;
+    if constexpr (KEPT) {
+      if (row >= g.rows) {
+        const int r = (int)(row - g.rows), at = g.draft_row ? g.draft_row[r] : r;
+        if ((uint32_t)at >= (uint32_t)g.draft_rows) return;  // refused where the drafts are looked at
+        g.logits = g.draft_logits;
+        first = at * g.ld_draft;
+      }
+    }
     base = BF16 ? (const void*)((const uint16_t*)g.logits + first) : (const void*)((const float*)g.logits + first);
   }
-  const float temp = g.temperature ? g.temperature[row] : 1.0f;
-  const int top_k = g.top_k ? g.top_k[row] : 0;
-  const float top_p = g.top_p ? g.top_p[row] : 1.0f;
-  const float min_p = g.min_p ? g.min_p[row] : 0.0f;
-  const float u = g.u[row];
+  const float temp = g.temperature ? g.temperature[set] : 1.0f;
+  const int top_k = g.top_k ? g.top_k[set] : 0;
+  const float top_p = g.top_p ? g.top_p[set] : 1.0f;
+  const float min_p = g.min_p ? g.min_p[set] : 0.0f;
+  const float u = KEPT ? 0.0f : g.u[row];
   const bool valid = temp >= 0.0f && top_p >= 0.0f && min_p >= 0.0f && min_p <= 1.0f && u >= 0.0f && u < 1.0f;
   auto finish = [&](int id, float logprob) {  // one thread
     g.token[row] = id < 0 ? -1 : g.off ? (int32_t)g.cand[(int64_t)o0 + id] : id;
     if (g.logprob) g.logprob[row] = logprob;
   };
   if (!valid && t == 0 && g.err) *g.err = 1;
+  auto record = [&](uint64_t total, float max, float v, int id, bool only, bool one) {  // one thread
+    if constexpr (KEPT) g.kept[row] = RowKept{total, max, v, id, (only ? kKeptInf : 0u) | (one ? kKeptOne : 0u)};
+  };
   if (n == 0) {
     if (t == 0) finish(-1, -INFINITY);
     return;
@@ -367,7 +323,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
 #pragma unroll
   for (int i = 1; i < NW; ++i) lmax = fmaxf(lmax, L.wmax[i]);
   if (lmax == -INFINITY) {  // only -inf and NaN
-    if (t == 0) finish(0, -INFINITY);
+    if (t == 0) {
+      if constexpr (KEPT) record(0, lmax, lmax, -1, false, false);
+      else finish(0, -INFINITY);
+    }
     return;
   }
   if (!valid || temp == 0.0f || top_k == 1 || top_p == 0.0f) {  // the maximum's lowest id
@@ -380,7 +339,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     if (best != 0x7FFFFFFF)
       __hip_atomic_fetch_min(&L.best, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     wg_lds_barrier();
-    if (t == 0) finish(L.best, 0.0f);
+    if (t == 0) {
+      if constexpr (KEPT) record(1, lmax, lmax, L.best, lmax == INFINITY, true);
+      else finish(L.best, 0.0f);
+    }
     return;
   }
   if (lmax == INFINITY) {
@@ -657,6 +619,11 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
     uint32_t kept = 0;  // the first so many
 #pragma unroll
     for (int i = 0; i < kList / 64; ++i) kept += L.kept[i];
+    if constexpr (KEPT) {
+      scan_threads((uint32_t)t < kept ? m : 0ull, total);
+      if (t == 0) record(total, lmax, pair_logit(L.sorted[kept - 1]), pair_id(L.sorted[kept - 1]), only_inf, false);
+      return;
+    }
     // The draw, in ascending ids: the places of a list of all, else sorted once more.
     if (stage == LIST_ALL) {
       pair = L.entry[min((uint32_t)t, listed - 1)];
@@ -726,6 +693,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
       if (!find) {
         total = run;
         need = need_u(total);
+        if constexpr (KEPT) {
+          if (t == 0) record(total, lmax, border_v, border_id, only_inf, false);
+          return;
+        }
       }
     }
     if (wave == seg % NW) {  // the wave that holds the group
@@ -760,8 +731,14 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs g) {
 
 template <int T, int IDS>
 hipError_t launch(const SampleArgs& g, hipStream_t s) {
-  auto kern = g.bf16 ? k_sample<T, IDS, true> : k_sample<T, IDS, false>;
+  auto kern = g.bf16 ? k_sample<T, IDS, true, false> : k_sample<T, IDS, false, false>;
   hipLaunchKernelGGL(kern, dim3((unsigned)g.rows), dim3(T), 0, s, g);
+  return hipGetLastError();
+}
+template <int T, int IDS>
+hipError_t launch_keep(const KeptArgs& g, hipStream_t s) {
+  auto kern = g.bf16 ? k_sample<T, IDS, true, true> : k_sample<T, IDS, false, true>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(g.draft_logits ? 2 * g.rows : g.rows)), dim3(T), 0, s, g);
   return hipGetLastError();
 }
 
@@ -779,6 +756,13 @@ hipError_t launch_sample(const SampleArgs& g, hipStream_t s) {
   if (g.V <= 4096) return launch<256, 4096>(g, s);
   if (g.V <= 32768) return launch<1024, 32768>(g, s);
   return launch<1024, 0>(g, s);
+}
+
+hipError_t launch_kept(const KeptArgs& g, hipStream_t s) {
+  if (g.rows == 0) return hipSuccess;
+  if (g.V <= 4096) return launch_keep<256, 4096>(g, s);
+  if (g.V <= 32768) return launch_keep<1024, 32768>(g, s);
+  return launch_keep<1024, 0>(g, s);
 }
 
 }  // namespace mh

@@ -173,6 +173,75 @@ def sample_candidates(logits, cand, cand_offsets, max_cands: int, u, token, temp
         _p(top_p), _p(min_p), u.ptr, token.ptr, _p(logprob), _p(err), stream), "sample_candidates")
 
 
+def paged_plan(lengths, new_tokens, page_size: int, block_table, pages_held, free_pages, free_count, lengths_out,
+               pages_held_out, free_count_out, cu_rows, served, slot_of_row=None, request_of_row=None, position_of_row=None,
+               row_cap=None, err=None, stream=None) -> None:
+    """marian_hip_paged_plan: pages, slots and rows of a step.  lengths_out, pages_held_out and free_count_out may be
+    the inputs.  row_cap: the most rows of the step (the length of the row maps that are given)."""
+    requests, max_blocks = block_table.shape
+    if row_cap is None:
+        row_cap = next((m.shape[0] for m in (slot_of_row, request_of_row, position_of_row) if m is not None), 0)
+    _lib.check(_lib.load().marian_hip_paged_plan(
+        lengths.ptr, new_tokens.ptr, pages_held.ptr, requests, int(page_size), block_table.ptr, max_blocks, free_pages.ptr,
+        free_count.ptr, free_pages.shape[0], lengths_out.ptr, pages_held_out.ptr, free_count_out.ptr, cu_rows.ptr,
+        _p(slot_of_row), _p(request_of_row), _p(position_of_row), int(row_cap), served.ptr, _p(err), stream), "paged_plan")
+
+
+def paged_append(k, v, slot_of_row, k_cache, v_cache, ldk=None, ldv=None, bf16: bool = False, cache_bf16: bool = False,
+                 err=None, stream=None) -> None:
+    """marian_hip_paged_append: rows k and v into their slots of k_cache [pages, kv_heads, page_size, head_dim] and
+    v_cache [pages, kv_heads, head_dim, page_size]; bf16: of the rows."""
+    pages, kv_heads, page_size, head_dim = k_cache.shape
+    _lib.check(_lib.load().marian_hip_paged_append(
+        k.ptr, ldk or k.shape[1], v.ptr, ldv or v.shape[1], int(bf16), slot_of_row.ptr, slot_of_row.shape[0], kv_heads,
+        head_dim, k_cache.ptr, v_cache.ptr, int(cache_bf16), pages, page_size, _p(err), stream), "paged_append")
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, cu_rows, out, heads: int, max_rows: int, max_keys: int,
+                    scale: float, window: int = 0, sinks: int = 0, bf16: bool = False, cache_bf16: bool = False, ldq=None,
+                    ldo=None, workspace=None, err=None, stream=None) -> None:
+    """marian_hip_paged_attention: the step's rows q over their requests' pages; bf16: of q.  workspace: a byte
+    buffer of paged_attention_workspace bytes, needed when the call is captured into a graph."""
+    pages, kv_heads, page_size, head_dim = k_cache.shape
+    requests, max_blocks = block_table.shape
+    _lib.check(_lib.load().marian_hip_paged_attention(
+        q.ptr, ldq or q.shape[1], int(bf16), q.shape[0], k_cache.ptr, v_cache.ptr, int(cache_bf16), pages, page_size,
+        block_table.ptr, max_blocks, lengths.ptr, cu_rows.ptr, requests, int(max_rows), int(max_keys), int(heads), kv_heads,
+        head_dim, float(scale), int(window), int(sinks), out.ptr, ldo or out.shape[1], _p(workspace),
+        workspace.nbytes if workspace is not None else 0, _p(err), stream), "paged_attention")
+
+
+def paged_attention_workspace(rows: int, requests: int, max_rows: int, max_keys: int, heads: int, kv_heads: int,
+                              head_dim: int, window: int = 0, sinks: int = 0) -> int:
+    """Bytes of workspace of paged_attention."""
+    n = C.c_size_t(0)
+    _lib.check(_lib.load().marian_hip_paged_attention_workspace(
+        rows, requests, max_rows, max_keys, heads, kv_heads, head_dim, window, sinks, C.byref(n)), "paged_attention_workspace")
+    return n.value
+
+
+def verify_drafts(logits, drafts, cu_rows, u, u_draw, token, accepted, max_rows=None, draft_logits=None, draft_row=None,
+                  temperature=None, top_k=None, top_p=None, min_p=None, bf16: bool = False, ids=None, workspace=None, err=None,
+                  stream=None) -> None:
+    """marian_hip_verify_drafts; ids: the row's ids when fewer than the strides; max_rows: the most rows of a
+    request (the rows of all when not given).  workspace: a byte buffer of verify_drafts_workspace bytes, needed when the call is
+    captured into a graph."""
+    rows, ld = logits.shape
+    draft_rows, ld_draft = draft_logits.shape if draft_logits is not None else (0, 0)
+    _lib.check(_lib.load().marian_hip_verify_drafts(
+        logits.ptr, ld, rows, ids or ld, int(bf16), _p(draft_logits), ld_draft, draft_rows, _p(draft_row), drafts.ptr,
+        cu_rows.ptr, accepted.shape[0], int(max_rows or max(rows, 1)), _p(temperature), _p(top_k), _p(top_p), _p(min_p), u.ptr,
+        u_draw.ptr, token.ptr, accepted.ptr, _p(workspace), workspace.nbytes if workspace is not None else 0, _p(err), stream),
+        "verify_drafts")
+
+
+def verify_drafts_workspace(rows: int, drafted: bool) -> int:
+    """Bytes of workspace of verify_drafts (drafted: with draft_logits)."""
+    n = C.c_size_t(0)
+    _lib.check(_lib.load().marian_hip_verify_drafts_workspace(rows, int(drafted), C.byref(n)), "verify_drafts_workspace")
+    return n.value
+
+
 def attention(q, k, v, seq_of_row, cu, out, heads: int, max_keys: int, ldq=None, ldkv=None,
               ldo=None, bf16: bool = False, packed_self: bool = True, head_dim: int = 64,
               stream=None) -> None:

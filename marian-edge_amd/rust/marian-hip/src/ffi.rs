@@ -6,7 +6,7 @@
 
 use std::ffi::{c_char, c_int};
 
-pub const MARIAN_HIP_ABI_VERSION: u32 = 5;
+pub const MARIAN_HIP_ABI_VERSION: u32 = 6;
 
 pub const OK: c_int = 0;
 pub const ERR_INVALID_INPUT: c_int = -1;
