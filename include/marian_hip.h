@@ -566,7 +566,7 @@ int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t l
  * not change its result, whatever they hold; pages that no row sees are not read.  Scores,
  * weights and sums are fp32, products exact.  The sums' order depends on the sizes of the
  * call and on the request's own lengths, not on other requests.  q is fp32, or
- * bfloat16 with q_bf16 != 0 (then the cache is too); ldq a multiple of 8, ldo of 4.
+ * bfloat16 with q_bf16 != 0 (then the cache must be too); ldq a multiple of 8, ldo of 4.
  * max_rows (at most 64) and max_keys (at most 2^27) bound every request's rows and length:
  * they choose the split.  A request past them, or whose rows are not within rows, sets *err
  * (device int, may be NULL) to 1 and its rows are left as they were, as are rows that
@@ -583,9 +583,9 @@ int marian_hip_paged_attention(const void* q, int64_t ldq, int q_bf16, int64_t r
                                int64_t window, int64_t sinks, float* out, int64_t ldo, void* workspace,
                                size_t workspace_bytes, int* err, void* stream);
 /* Bytes of workspace of a call with these sizes. */
-int marian_hip_paged_attention_workspace(int64_t rows, int64_t requests, int64_t max_rows, int64_t max_keys,
-                                         int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
-                                         int64_t sinks, size_t* bytes);
+int marian_hip_paged_attention_workspace(int64_t requests, int64_t max_rows, int64_t max_keys, int64_t heads,
+                                         int64_t kv_heads, int64_t head_dim, int q_bf16, int cache_bf16,
+                                         int64_t window, int64_t sinks, size_t* bytes);
 
 /* Drafted ids against the target's logits, so that every id that comes out is distributed
  * as marian_hip_sample_logits would draw it.  Row r of logits (fp32, or bfloat16 with

@@ -642,15 +642,15 @@ struct PagedAttnArgs {
   int64_t ldo = 0;
   int* err = nullptr;  // set to 1 on a request or page out of range
   // Filled by launch_paged_attention.
-  int qtiles = 0, chunks = 0, chunk_tiles = 0;
-  float* part_o = nullptr;   // [rows, heads, chunks, head_dim]
-  float* part_ml = nullptr;  // [rows, heads, chunks, 2]: reference, sum of weights
+  int qtiles = 0, whole = 0, workers = 0, min_tiles = 0;
+  float* part_o = nullptr;   // [workers, 2, columns of a query tile, head_dim]
+  float* part_ml = nullptr;  // [workers, 2, columns, 2]: reference, sum of weights
 };
 constexpr int kPagedMaxRows = 64;          // of a request
 constexpr int kPagedMaxKeys = 1 << 27;
 bool paged_attention_launchable(const PagedAttnArgs& g);  // within a grid's limits
 size_t paged_attention_bytes(const PagedAttnArgs& g);
-hipError_t launch_paged_attention(const PagedAttnArgs& g, void* workspace, hipStream_t s);
+hipError_t launch_paged_attention(const PagedAttnArgs& g, void* workspace, size_t workspace_bytes, hipStream_t s);
 
 // Reduces argmax partials to token ids (op-level argmax).
 // Records the message marian_hip_last_op_error returns on this thread.

@@ -590,16 +590,19 @@ int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t l
 
 namespace {
 // The sizes of a paged attention call; the reason why they are refused, or null.
-const char* paged_attention_sizes(PagedAttnArgs& g, int64_t rows, int64_t requests, int64_t max_rows, int64_t max_keys,
-                                  int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks) {
-  if (rows < 0 || rows > kPlanMaxRows || requests < 0 || requests > kPlanMaxRequests || max_rows <= 0 ||
+const char* paged_attention_sizes(PagedAttnArgs& g, int64_t requests, int64_t max_rows, int64_t max_keys, int64_t heads,
+                                  int64_t kv_heads, int64_t head_dim, int q_bf16, int cache_bf16, int64_t window,
+                                  int64_t sinks) {
+  if (requests < 0 || requests > kPlanMaxRequests || max_rows <= 0 ||
       max_rows > kPagedMaxRows || max_keys <= 0 || max_keys > kPagedMaxKeys || window < 0 || window > INT32_MAX / 2 ||
       sinks < 0 || sinks > INT32_MAX / 2)
     return "sizes out of range";
   if (kv_heads <= 0 || kv_heads > kMaxKvHeads || heads <= 0 || heads > kMaxKvHeads || heads % kv_heads)
     return "heads is a multiple of kv_heads, both at most 128";
   if (head_dim != 48 && head_dim != 64 && head_dim != 128) return "head_dim is 48, 64 or 128";
-  g.rows = (int)rows;
+  if (q_bf16 && !cache_bf16) return "bfloat16 queries need a bfloat16 cache";
+  g.q_bf16 = q_bf16 ? 1 : 0;
+  g.cache_bf16 = cache_bf16 ? 1 : 0;
   g.requests = (int)requests;
   g.max_rows = (int)max_rows;
   g.max_keys = (int)max_keys;
@@ -614,12 +617,13 @@ const char* paged_attention_sizes(PagedAttnArgs& g, int64_t rows, int64_t reques
 }
 }  // namespace
 
-int marian_hip_paged_attention_workspace(int64_t rows, int64_t requests, int64_t max_rows, int64_t max_keys,
-                                         int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
-                                         int64_t sinks, size_t* bytes) {
+int marian_hip_paged_attention_workspace(int64_t requests, int64_t max_rows, int64_t max_keys, int64_t heads,
+                                         int64_t kv_heads, int64_t head_dim, int q_bf16, int cache_bf16,
+                                         int64_t window, int64_t sinks, size_t* bytes) {
   PagedAttnArgs g;
   if (!bytes) return refuse("paged_attention_workspace: bytes is missing");
-  if (const char* why = paged_attention_sizes(g, rows, requests, max_rows, max_keys, heads, kv_heads, head_dim, window, sinks))
+  if (const char* why = paged_attention_sizes(g, requests, max_rows, max_keys, heads, kv_heads, head_dim, q_bf16, cache_bf16,
+                                              window, sinks))
     return refuse_as("paged_attention_workspace", why);
   *bytes = paged_attention_bytes(g);
   return MARIAN_HIP_OK;
@@ -634,17 +638,17 @@ int marian_hip_paged_attention(const void* q, int64_t ldq, int q_bf16, int64_t r
                                size_t workspace_bytes, int* err, void* stream) {
   PagedAttnArgs g;
   const int shift = page_shift_of(page_size);
-  if (const char* why = paged_attention_sizes(g, rows, requests, max_rows, max_keys, heads, kv_heads, head_dim, window, sinks))
+  if (const char* why = paged_attention_sizes(g, requests, max_rows, max_keys, heads, kv_heads, head_dim, q_bf16, cache_bf16,
+                                              window, sinks))
     return refuse_as("paged_attention", why);
   if (const char* why = paged_cache_refusal(k_cache, v_cache, num_pages, shift, kv_heads, head_dim))
     return refuse_as("paged_attention", why);
   if (!q || !block_table || !lengths || !cu_rows || !out) return refuse("paged_attention: an array is missing");
   const int64_t width = heads * head_dim;
-  if (max_blocks <= 0 || max_blocks > kMaxBlocks || ldq < width || ldo < width || ldq > kMaxStride || ldo > kMaxStride ||
+  if (rows < 0 || rows > kPlanMaxRows || max_blocks <= 0 || max_blocks > kMaxBlocks || ldq < width || ldo < width || ldq > kMaxStride || ldo > kMaxStride ||
       ldq % 8 || ldo % 4)
     return refuse("paged_attention: sizes or strides out of range");
   if (!(scale > 0.0f) || !(scale <= 1e30f)) return refuse("paged_attention: scale is not positive and finite");
-  if (q_bf16 && !cache_bf16) return refuse("paged_attention: bfloat16 queries need a bfloat16 cache");
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace))
     return refuse("paged_attention: q, out and workspace must be 16-byte aligned");
   const size_t bytes = paged_attention_bytes(g), cache = (size_t)num_pages * page_size * kv_heads * head_dim * (cache_bf16 ? 2 : 4);
@@ -662,11 +666,11 @@ int marian_hip_paged_attention(const void* q, int64_t ldq, int q_bf16, int64_t r
     if (capturing(s)) return refuse("paged_attention: a call that is captured into a graph needs a workspace");
     workspace = op_scratch(3, bytes, s);
     if (!workspace) return op_status(hipErrorOutOfMemory, "paged_attention scratch");
+    workspace_bytes = bytes;
   }
   g.q = q;
   g.ldq = ldq;
-  g.q_bf16 = q_bf16 ? 1 : 0;
-  g.cache_bf16 = cache_bf16 ? 1 : 0;
+  g.rows = (int)rows;
   g.k = k_cache;
   g.v = v_cache;
   g.page_shift = shift;
@@ -679,7 +683,7 @@ int marian_hip_paged_attention(const void* q, int64_t ldq, int q_bf16, int64_t r
   g.out = out;
   g.ldo = ldo;
   g.err = err;
-  return op_status(launch_paged_attention(g, workspace, s), "paged_attention");
+  return op_status(launch_paged_attention(g, workspace, workspace_bytes, s), "paged_attention");
 }
 
 namespace {

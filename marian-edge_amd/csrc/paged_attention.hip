@@ -8,6 +8,7 @@
 // of w_j e^-m v_j; parts of the keys join by rescaling each to the largest m.
 #include "device_common.h"
 #include "kernels.h"
+#include "mass.h"
 
 #include <algorithm>
 
@@ -19,8 +20,6 @@ constexpr int kWaves = 4;
 // Scores (in octaves) may pass the reference by so much before the sums are rescaled: weights up to 2^8.
 constexpr float kSlack = 8.0f;
 
-typedef short s8v __attribute__((ext_vector_type(8)));
-typedef short s4v __attribute__((ext_vector_type(4)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 
@@ -71,9 +70,9 @@ __device__ __forceinline__ void split3(float a, float b, int& hi, int& mid, int&
 __device__ __forceinline__ f4v mfma32(v4i a, v4i b, f4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f4v mfma16(v2i a, v2i b, f4v c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4v, a), __builtin_bit_cast(s4v, b), c, 0, 0, 0);
-}
+// Half a product: four values a lane, the other four zero.  (The product of 16 in the same chain of sums read the ones of
+// 32 before they were done, in one build of this file.)
+__device__ __forceinline__ f4v mfma_half(v2i a, v2i b, f4v c) { return mfma32(v4i{a[0], a[1], 0, 0}, v4i{b[0], b[1], 0, 0}, c); }
 
 // The operands of one tile, in the order of the matrix instructions' lanes.  A wave's lane is (m, g) = (lane % 16,
 // lane / 16).  S^T = K Q^T comes in two products of 16 keys, row 4a + i of product t being key 8a + 4t + i of the
@@ -186,7 +185,7 @@ struct Query<D, true, QP> {
     for (int j = QP - 1; j >= 0; --j) {  // the small parts first
 #pragma unroll
       for (int s = 0; s < KS; ++s) c = mfma32(x.k[t][s], q[j][s], c);
-      if constexpr (HALF) c = mfma16(x.kh[t], qh[j], c);
+      if constexpr (HALF) c = mfma_half(x.kh[t], qh[j], c);
     }
     return c;
   }
@@ -249,225 +248,405 @@ __device__ __forceinline__ void add_values(f4v (&o)[D / 16], const Tile<D, false
       for (int d = 0; d < D / 16; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[t][d][i], w[4 * t + i], o[d], 0, 0, 0);
 }
 
-// One workgroup: a request, a key head, 16 NT (row, query head) pairs and one chunk of the tiles that they see; its
-// waves take turns at the tiles and join at the end.
+// Registers a thread of an instance needs, as waves a SIMD: workgroups a compute unit, one wave of each on a SIMD.
 template <int D, bool CB16, int QP, int NT>
-__global__ __launch_bounds__(kWaves * 64) void k_paged_attention(PagedAttnArgs g) {
+constexpr int waves_a_simd() {
+  if (D == 128) return NT == 1 ? (CB16 && QP == 1 ? 3 : 2) : (CB16 && QP == 1 ? 2 : 1);
+  if (D == 64 && (!CB16 || QP == 3)) return NT == 1 ? (CB16 ? 4 : 3) : 2;
+  return NT == 1 ? 4 : 3;
+}
+
+// Work is counted in tiles of a (request, query tile, key head), in that order, head fastest: one at least for each that has
+// rows, so that rows that see nothing are written too.
+template <int NT>
+__device__ __forceinline__ int64_t request_tiles(const PagedAttnArgs& g, const Request& r) {
+  const int cols = r.n * g.group, pos0 = r.len - r.n;
+  int64_t all = 0;
+  for (int col0 = 0; col0 < cols; col0 += 16 * NT)
+    all += max(1, span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles);
+  return all * g.kv_heads;
+}
+
+template <class T>
+__device__ __forceinline__ T uniform(T v) {
+  static_assert(sizeof(T) == 4, "one register");
+  return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+}
+
+// Where a workgroup's share of all tiles begins: request b, `into` tiles into it, `quota` tiles to take.
+struct Share {
+  int b;
+  int64_t into, quota;
+};
+constexpr int kThreads = kWaves * 64;
+struct ShareLds {
+  int64_t sum[kPlanMaxRequests / kThreads + 1], wave[kWaves], into;
+  int b;
+};
+__device__ __forceinline__ int64_t quota_of(const PagedAttnArgs& g, int64_t total) {
+  return max((total + g.workers - 1) / g.workers, (int64_t)g.min_tiles);
+}
+template <int NT>
+__device__ __forceinline__ Share share_of(const PagedAttnArgs& g, int worker, ShareLds& L) {
+  const int t = threadIdx.x, lane = t & 63, wave = uniform(t >> 6);
+  const int steps = (g.requests + kThreads - 1) / kThreads;
+  int64_t mine = 0, upto = 0, total = 0;
+  auto step = [&](int i) {  // this thread's request's tiles, and their running sum within the step
+    const int b = i * kThreads + t;
+    mine = b < g.requests ? request_tiles<NT>(g, request_of(g, b, worker == 0)) : 0;
+    upto = (int64_t)wave_scan_mass((uint64_t)mine);
+    if (lane == 63) L.wave[wave] = upto;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      upto += w < wave ? L.wave[w] : 0;
+      all += L.wave[w];
+    }
+    return all;
+  };
+  if (t == 0) L.b = g.requests;
+  for (int i = 0; i < steps; ++i) {
+    const int64_t all = step(i);
+    if (steps > 1) {
+      if (t == 0) L.sum[i] = all;
+      __syncthreads();
+    }
+    total += all;
+  }
+  const int64_t quota = quota_of(g, total);
+  int64_t at = (int64_t)worker * quota;
+  int i = 0;
+  if (steps > 1) {
+    for (; i < steps - 1 && at >= L.sum[i]; ++i) at -= L.sum[i];
+    step(i);
+  }
+  if (mine && upto - mine <= at && at < upto) {
+    L.b = i * kThreads + t;
+    L.into = at - (upto - mine);
+  }
+  __syncthreads();
+  return {uniform(L.b), uniform64(L.into), quota};
+}
+
+// A workgroup of four waves takes tiles of one (request, query tile of 16 NT (row, head) pairs, key head) after another:
+// either all of one (g.whole), or its share of all the call's tiles, the same number for every workgroup and as many
+// workgroups as run at once: then the caches' lengths may differ as they like, and a sequence is split where shares
+// meet.  The waves take turns at the tiles of a sequence and join at its end; what is not a whole sequence goes to
+// the workspace: part 0 of a workgroup is the end or middle of a sequence, part 1 the beginning of one.
+template <int D, bool CB16, int QP, int NT>
+__global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k_paged_attention(PagedAttnArgs g) {
   constexpr int DT = D / 16;
   __shared__ __attribute__((aligned(16))) float lds_o[kWaves][DT * 64 * 4];
   __shared__ float lds_m[kWaves][NT][16], lds_l[kWaves][NT][16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ ShareLds share;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int m = lane & 15, grp = lane >> 4;
-  int id = blockIdx.x;
-  const int chunk = id % g.chunks;
-  id /= g.chunks;
-  const int head = id % g.kv_heads;
-  id /= g.kv_heads;
-  const int qt = id % g.qtiles, b = id / g.qtiles;
-  const Request rq = request_of(g, b, chunk == 0 && head == 0 && qt == 0 && threadIdx.x == 0);
-  const int cols = rq.n * g.group, col0 = qt * 16 * NT;
-  if (col0 >= cols) return;
-  const int pos0 = rq.len - rq.n;
-  const Span span = span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks);
-  const int t0 = chunk * g.chunk_tiles, t1 = min(span.tiles, t0 + g.chunk_tiles);
-  if (t0 >= t1 && chunk > 0) return;
-
-  Query<D, CB16, QP> q[NT];
-  int pos[NT];      // of the lane's column
-  f4v o[NT][DT];
-  float ref[NT], sum[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int col = col0 + 16 * n + m, i = min(col, cols - 1) / g.group, hq = head * g.group + min(col, cols - 1) % g.group;
-    q[n].load(g.q, (int64_t)(rq.row0 + i) * g.ldq + hq * D, col < cols, g.q_bf16, grp);
-    pos[n] = pos0 + i;
-    ref[n] = -INFINITY;
-    sum[n] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[n][d] = f4v{0, 0, 0, 0};
+  int b, qt = 0, head = 0;
+  int64_t left;  // tiles to take
+  int t0 = 0;
+  if (g.whole) {
+    int id = blockIdx.x;
+    head = id % g.kv_heads;
+    id /= g.kv_heads;
+    qt = id % g.qtiles;
+    b = id / g.qtiles;
+    left = 0x7FFFFFFF;
+  } else {
+    const Share s = share_of<NT>(g, blockIdx.x, share);
+    b = s.b;
+    left = s.quota;
+    if (b >= g.requests) return;
+    // The query tile and head that the share begins in.
+    const Request rq = request_of(g, b, false);
+    const int cols = rq.n * g.group, pos0 = rq.len - rq.n;
+    int64_t into = s.into;
+    for (;; ++qt) {
+      const int col0 = qt * 16 * NT;
+      const int tiles = max(1, span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles);
+      if (into < (int64_t)tiles * g.kv_heads || col0 + 16 * NT >= cols) {
+        head = (int)(into / tiles);
+        t0 = (int)(into % tiles);
+        break;
+      }
+      into -= (int64_t)tiles * g.kv_heads;
+    }
   }
-
   const int ps = 1 << g.page_shift;
-  const int32_t* table = g.table + (int64_t)b * g.max_blocks;
-  // Page of key group a (8 keys) of a tile; keys past the request's last give the last one's.
-  auto page_at = [&](int tile, int a) -> int {
-    return table[min(tile * kTileKeys + 8 * a, rq.len - 1) >> g.page_shift];
-  };
   auto in_range = [&](int page) { return (uint32_t)page < (uint32_t)g.num_pages; };
-  auto block = [&](int page) -> int64_t { return ((int64_t)(in_range(page) ? page : 0) * g.kv_heads + head) * D << g.page_shift; };
 
-  Tile<D, CB16> x;
-  int it = t0 + wave;
-  int page_k = 0, page_v = 0, next_k = 0, next_v = 0;
-  auto load_k = [&](int tile, int page) {
-    const int key = tile * kTileKeys + 8 * (m >> 2) + (m & 3);
-    x.load_k((const char*)g.k, block(page) + (int64_t)(key & (ps - 1)) * D, grp);
-  };
-  if (it < t1) {
-    const int tile = span.tile(it);
-    page_k = page_at(tile, m >> 2);
-    page_v = page_at(tile, grp);
-    load_k(tile, page_k);
-    if (it + kWaves < t1) {
-      next_k = page_at(span.tile(it + kWaves), m >> 2);
-      next_v = page_at(span.tile(it + kWaves), grp);
+  for (;;) {
+    const Request rq = request_of(g, b, g.whole && head == 0 && qt == 0 && threadIdx.x == 0);
+    const int cols = uniform(rq.n * g.group), col0 = qt * 16 * NT;
+    if (col0 >= cols) {  // no (more) rows
+      if (g.whole || ++b >= g.requests) return;
+      qt = head = t0 = 0;
+      continue;
     }
-  }
+    const int pos0 = rq.len - rq.n;
+    const Span span = span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks);
+    const int t1 = (int)min((int64_t)max(1, span.tiles), t0 + left);
+    const bool alone = t0 == 0 && t1 >= span.tiles;
+    left -= t1 - t0;
+
+    Query<D, CB16, QP> q[NT];
+    int pos[NT];  // of the lane's column
+    f4v o[NT][DT];
+    float ref[NT], sum[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int col = col0 + 16 * n + m, i = min(col, cols - 1) / g.group, hq = head * g.group + min(col, cols - 1) % g.group;
+      q[n].load(g.q, (int64_t)(rq.row0 + i) * g.ldq + hq * D, col < cols, g.q_bf16, grp);
+      pos[n] = pos0 + i;
+      ref[n] = -INFINITY;
+      sum[n] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[n][d] = f4v{0, 0, 0, 0};
+    }
+
+    const int32_t* table = g.table + (int64_t)b * g.max_blocks;
+    // Page of key group a (8 keys) of a tile; keys past the request's last give the last one's.
+    auto page_at = [&](int tile, int a) -> int {
+      return table[min(tile * kTileKeys + 8 * a, rq.len - 1) >> g.page_shift];
+    };
+    auto block = [&](int page) -> int64_t { return ((int64_t)(in_range(page) ? page : 0) * g.kv_heads + head) * D << g.page_shift; };
+
+    Tile<D, CB16> x;
+    const int last = min(t1, span.tiles);
+    int it = t0 + wave;
+    int page_k = 0, page_v = 0, next_k = 0, next_v = 0;
+    auto load_k = [&](int tile, int page) {
+      const int key = tile * kTileKeys + 8 * (m >> 2) + (m & 3);
+      x.load_k((const char*)g.k, block(page) + (int64_t)(key & (ps - 1)) * D, grp);
+    };
+    if (it < last) {
+      const int tile = span.tile(it);
+      page_k = page_at(tile, m >> 2);
+      page_v = page_at(tile, grp);
+      load_k(tile, page_k);
+      const int next = span.tile(min(it + kWaves, last - 1));
+      next_k = page_at(next, m >> 2);
+      next_v = page_at(next, grp);
+    }
 #pragma unroll 1
-  for (; it < t1; it += kWaves) {
-    const int tile = span.tile(it), key0 = tile * kTileKeys;
-    const int kg = key0 + 8 * grp;  // this lane's first key
-    x.load_v((const char*)g.v, block(page_v) + ((int64_t)m << g.page_shift) + (kg & (ps - 1)), g.page_shift);
-    f4v s[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) s[n][t] = q[n].scores(x, t);
-    const int page = page_v;
-    if (it + kWaves < t1) {
-      load_k(span.tile(it + kWaves), next_k);
-      page_v = next_v;
-      if (it + 2 * kWaves < t1) {
-        next_k = page_at(span.tile(it + 2 * kWaves), m >> 2);
-        next_v = page_at(span.tile(it + 2 * kWaves), grp);
-      }
-    }
-    // Tiles that not every row sees whole: keys out of sight leave the sums alone, whatever they hold.
-    const bool whole = key0 + kTileKeys - 1 <= span.first_pos &&
-                       (g.window <= 0 || key0 > span.last_pos - g.window || key0 + kTileKeys <= g.sinks);
-    const bool bad = !in_range(page);
-    if (!whole || __any(bad)) {
-      uint32_t some = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = kg + i;
-        const bool any = key <= span.last_pos && (g.window <= 0 || key > span.first_pos - g.window || key < g.sinks);
-        some |= any ? 1u << i : 0u;
-      }
-      if (bad && some && g.err) *g.err = 1;
-      if (bad) some = 0;
-      x.keep_v(some);
+    for (; it < last; it += kWaves) {
+      const int tile = span.tile(it), key0 = tile * kTileKeys;
+      const int kg = key0 + 8 * grp;  // this lane's first key
+      x.load_v((const char*)g.v, block(page_v) + ((int64_t)m << g.page_shift) + (kg & (ps - 1)), g.page_shift);
+      f4v s[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
+        for (int t = 0; t < 2; ++t) s[n][t] = q[n].scores(x, t);
+      const int page = page_v;
+      // The next tile's keys, and the pages of the one after (at the end some tile once more: behind a branch the
+      // values' wait would have to cover these loads too).
+      load_k(span.tile(min(it + kWaves, last - 1)), next_k);
+      page_v = next_v;
+      const int after = span.tile(min(it + 2 * kWaves, last - 1));
+      next_k = page_at(after, m >> 2);
+      next_v = page_at(after, grp);
+      // Tiles that not every row sees whole: keys out of sight leave the sums alone, whatever they hold.
+      const bool whole = key0 + kTileKeys - 1 <= span.first_pos &&
+                         (g.window <= 0 || key0 > span.last_pos - g.window || key0 + kTileKeys <= g.sinks);
+      const bool bad = !in_range(page);
+      if (!whole || __any(bad)) {
+        uint32_t some = 0;
+#pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int key = kg + i;
-          const bool see = (some >> i & 1) && key <= pos[n] && (g.window <= 0 || key > pos[n] - g.window || key < g.sinks);
-          s[n][i >> 2][i & 3] = see ? s[n][i >> 2][i & 3] : -INFINITY;
+          const bool any = key <= span.last_pos && (g.window <= 0 || key > span.first_pos - g.window || key < g.sinks);
+          some |= any ? 1u << i : 0u;
         }
+        if (bad && some && g.err) *g.err = 1;
+        if (bad) some = 0;
+        x.keep_v(some);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = kg + i;
+            const bool see = (some >> i & 1) && key <= pos[n] && (g.window <= 0 || key > pos[n] - g.window || key < g.sinks);
+            s[n][i >> 2][i & 3] = see ? s[n][i >> 2][i & 3] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                          fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3]))) * g.scale_log2e;
+        if (__any(top > ref[n] + kSlack)) {
+          top = fmaxf(top, xor_lane_f<16>(top));
+          top = fmaxf(top, xor_lane_f<32>(top));
+          const float to = fmaxf(ref[n], top);
+          const float by = to > -INFINITY ? exp2_fast(ref[n] - to) : 1.0f;
+          ref[n] = to;
+          sum[n] *= by;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[n][d] *= by;
+        }
+        const float base = ref[n] > -INFINITY ? -ref[n] : 0.0f;
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = exp2_fast(__builtin_fmaf(s[n][i >> 2][i & 3], g.scale_log2e, base));
+        sum[n] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        add_values<D>(o[n], x, w);
+      }
     }
+
+    // ---- the waves' parts, then the rows' or the share's ----
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
-                        fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3]))) * g.scale_log2e;
-      if (__any(top > ref[n] + kSlack)) {
-        top = fmaxf(top, xor_lane_f<16>(top));
-        top = fmaxf(top, xor_lane_f<32>(top));
-        const float to = fmaxf(ref[n], top);
-        const float by = to > -INFINITY ? exp2_fast(ref[n] - to) : 1.0f;
-        ref[n] = to;
-        sum[n] *= by;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[n][d] *= by;
+      sum[n] += xor_lane_f<16>(sum[n]);
+      sum[n] += xor_lane_f<32>(sum[n]);
+      if (lane < 16) {
+        lds_m[wave][n][m] = ref[n];
+        lds_l[wave][n][m] = sum[n];
       }
-      const float base = ref[n] > -INFINITY ? -ref[n] : 0.0f;
-      float w[8];
+    }
+    __syncthreads();
+    const int64_t part = (int64_t)blockIdx.x * 2 + (t0 > 0 ? 0 : 1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = exp2_fast(__builtin_fmaf(s[n][i >> 2][i & 3], g.scale_log2e, base));
-      sum[n] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-      add_values<D>(o[n], x, w);
+    for (int n = 0; n < NT; ++n) {
+      float top = lds_m[0][n][m];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][n][m]);
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float r = lds_m[w][n][m];
+        total += r > -INFINITY ? lds_l[w][n][m] * exp2_fast(r - top) : lds_l[w][n][m];
+      }
+      const float by = ref[n] > -INFINITY ? exp2_fast(ref[n] - top) : 1.0f;
+      if (n) __syncthreads();
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *(f4v*)&lds_o[wave][(d * 64 + lane) * 4] = o[n][d] * by;
+      __syncthreads();
+      const int col = col0 + 16 * n + m;
+      const int i = col / g.group, hq = head * g.group + col % g.group;
+      // A row that sees no key gives zeros; one whose weights are all zero what the formula gives, 0 / 0.
+      const bool sees = pos0 + i >= 0;
+      for (int d = wave; d < DT; d += kWaves) {
+        f4v v = *(const f4v*)&lds_o[0][(d * 64 + lane) * 4];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) v += *(const f4v*)&lds_o[w][(d * 64 + lane) * 4];
+        if (col >= cols) continue;
+        if (alone) {
+          v = sees ? v / total : f4v{0, 0, 0, 0};
+          *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 16 * d + 4 * grp) = v;
+        } else {
+          const int64_t at = part * (16 * NT) + 16 * n + m;
+          *(f4v*)(g.part_o + at * D + 16 * d + 4 * grp) = v;
+          if (d == 0 && grp == 0) *(float2*)(g.part_ml + 2 * at) = make_float2(top, total);
+        }
+      }
+    }
+    if (g.whole || left <= 0) return;
+    t0 = 0;
+    if (++head == g.kv_heads) {
+      head = 0;
+      ++qt;
     }
   }
+}
 
-  // ---- the waves' parts, then the row's or the chunk's ----
-  const bool alone = span.tiles <= g.chunk_tiles;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    sum[n] += xor_lane_f<16>(sum[n]);
-    sum[n] += xor_lane_f<32>(sum[n]);
-    if (lane < 16) {
-      lds_m[wave][n][m] = ref[n];
-      lds_l[wave][n][m] = sum[n];
-    }
+// Joins the parts of a sequence's columns, a wave each: the largest reference first, then the parts' sums, four dimensions
+// a lane and as many parts at once as fit.
+template <int D, int NT>
+__global__ __launch_bounds__(kThreads) void k_paged_join(PagedAttnArgs g) {
+  constexpr int QUADS = D / 4, AT_ONCE = 64 / QUADS;  // D = 48: 5 parts, and four lanes idle
+  __shared__ int64_t before_w[kWaves], total_w[kWaves];
+  const int t = threadIdx.x, lane = t & 63, wave = uniform(t >> 6);
+  int id = blockIdx.x;
+  const int col_in = id % (16 * NT / kWaves) * kWaves + wave;
+  id /= 16 * NT / kWaves;
+  const int head = id % g.kv_heads;
+  id /= g.kv_heads;
+  const int qt = id % g.qtiles, b = id / g.qtiles;
+  const Request rq = request_of(g, b, false);
+  const int cols = rq.n * g.group, col = qt * 16 * NT + col_in;
+  if (col - wave >= cols) return;
+  int64_t before = 0, total = 0;
+  for (int r = t; r < g.requests; r += kThreads) {
+    const int64_t n = request_tiles<NT>(g, request_of(g, r, false));
+    total += n;
+    before += r < b ? n : 0;
+  }
+  before = (int64_t)wave_scan_mass((uint64_t)before);
+  total = (int64_t)wave_scan_mass((uint64_t)total);
+  if (lane == 63) {
+    before_w[wave] = before;
+    total_w[wave] = total;
   }
   __syncthreads();
+  if (col >= cols) return;
+  before = total = 0;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float top = lds_m[0][n][m];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][n][m]);
-    float total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float r = lds_m[w][n][m];
-      total += r > -INFINITY ? lds_l[w][n][m] * exp2_fast(r - top) : lds_l[w][n][m];
-    }
-    const float by = ref[n] > -INFINITY ? exp2_fast(ref[n] - top) : 1.0f;
-    if (n) __syncthreads();
-#pragma unroll
-    for (int d = 0; d < DT; ++d) *(f4v*)&lds_o[wave][(d * 64 + lane) * 4] = o[n][d] * by;
-    __syncthreads();
-    const int col = col0 + 16 * n + m;
-    const int i = col / g.group, hq = head * g.group + col % g.group;
-    const int64_t row = rq.row0 + i;
-    // A row that sees no key gives zeros; one whose weights are all zero what the formula gives, 0 / 0.
-    const bool sees = pos0 + i >= 0;
-    for (int d = wave; d < DT; d += kWaves) {
-      f4v v = *(const f4v*)&lds_o[0][(d * 64 + lane) * 4];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) v += *(const f4v*)&lds_o[w][(d * 64 + lane) * 4];
-      if (col >= cols) continue;
-      if (alone) {
-        v = sees ? v / total : f4v{0, 0, 0, 0};
-        *(f4v*)(g.out + row * g.ldo + hq * D + 16 * d + 4 * grp) = v;
-      } else {
-        const int64_t at = (row * g.heads + hq) * g.chunks + chunk;
-        *(f4v*)(g.part_o + at * D + 16 * d + 4 * grp) = v;
-        if (d == 0 && grp == 0) *(float2*)(g.part_ml + 2 * at) = make_float2(top, total);
-      }
-    }
+  for (int w = 0; w < kWaves; ++w) {
+    before += before_w[w];
+    total += total_w[w];
   }
-}
-
-// Joins the chunks of one (row, query head): a wave each.
-template <int D>
-__global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs g, int nt16) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int per = g.max_rows * g.heads;
-  const int b = (int)(item / per), i = (int)(item % per) / g.heads, hq = (int)(item % g.heads);
-  if (b >= g.requests) return;
-  const Request rq = request_of(g, b, false);
-  if (i >= rq.n) return;
-  const int cols = rq.n * g.group, qt = (i * g.group + hq % g.group) / nt16, col0 = qt * nt16, pos0 = rq.len - rq.n;
-  const Span span = span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + nt16) - 1) / g.group, g.window, g.sinks);
-  if (span.tiles <= g.chunk_tiles) return;  // written already
-  const int chunks = (span.tiles + g.chunk_tiles - 1) / g.chunk_tiles;
-  const int64_t row = rq.row0 + i, at = (row * g.heads + hq) * g.chunks;
-  const float2* ml = (const float2*)g.part_ml + at;
+  const int64_t quota = quota_of(g, total);
+  const int pos0 = rq.len - rq.n;
+  int tiles = 0;
+  for (int j = 0; j <= qt; ++j) {
+    const int col0 = j * 16 * NT;
+    tiles = max(1, span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles);
+    before += (int64_t)tiles * (j < qt ? g.kv_heads : head);
+  }
+  const int64_t first = before / quota, last = (before + tiles - 1) / quota;
+  if (first == last) return;  // in one share: written already
+  const int parts = (int)(last - first) + 1;
+  auto place = [&](int p) -> int64_t { return ((first + p) * 2 + (p == 0 ? 1 : 0)) * (16 * NT) + col_in; };
+  const float2* ml = (const float2*)g.part_ml;
   float top = -INFINITY;
-  for (int c = lane; c < chunks; c += 64) top = fmaxf(top, ml[c].x);
+  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[place(p)].x);
   top = wave_max(top);
   const float base = top > -INFINITY ? top : 0.0f;
-  constexpr int PER = (D + 63) / 64;
-  float total = 0.0f, v[PER] = {};
-#pragma unroll 4
-  for (int c = 0; c < chunks; ++c) {
-    const float2 e = ml[c];
-    const float by = e.x > -INFINITY ? exp2_fast(e.x - base) : 1.0f;
-    total += e.y * by;
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (j * 64 + lane < D) v[j] += g.part_o[(at + c) * D + j * 64 + lane] * by;
+  const int quad = lane % QUADS, row = lane / QUADS;
+  f4v v = {0, 0, 0, 0};
+  float sum = 0.0f;
+  if (row < AT_ONCE) {
+#pragma unroll 8
+    for (int p = row; p < parts; p += AT_ONCE) {
+      const int64_t at = place(p);
+      const float2 e = ml[at];
+      const f4v x = *(const f4v*)(g.part_o + at * D + 4 * quad);
+      const float by = e.x > -INFINITY ? exp2_fast(e.x - base) : 1.0f;
+      sum += e.y * by;
+      v += x * by;
+    }
   }
+  const f4v own = v;
+  const float own_sum = sum;
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (j * 64 + lane < D) g.out[row * g.ldo + hq * D + j * 64 + lane] = pos0 + i >= 0 ? v[j] / total : 0.0f;
+  for (int r = 1; r < AT_ONCE; ++r) {  // into the first lanes
+    const int from = (lane + r * QUADS) & 63;
+    sum += __shfl(own_sum, from);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] += __shfl(own[c], from);
+  }
+  if (lane < QUADS) {
+    const int i = col / g.group, hq = head * g.group + col % g.group;
+    *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 4 * quad) = pos0 + i >= 0 ? v / sum : f4v{0, 0, 0, 0};
+  }
 }
 
-// How a call is split: by sizes that the host knows.
+constexpr int kComputeUnits = 256;
+constexpr int kMinTiles = 2 * kWaves;  // of a share
+constexpr int kWholeKeys = 512;  // caches up to this long are one workgroup's
+template <int D>
+int instance_waves(const PagedAttnArgs& g, int nt) {
+  if (!g.cache_bf16) return nt == 1 ? waves_a_simd<D, false, 1, 1>() : waves_a_simd<D, false, 1, 2>();
+  if (g.q_bf16) return nt == 1 ? waves_a_simd<D, true, 1, 1>() : waves_a_simd<D, true, 1, 2>();
+  return nt == 1 ? waves_a_simd<D, true, 3, 1>() : waves_a_simd<D, true, 3, 2>();
+}
+
+// How a call is laid out, by sizes that the host knows.
 struct Plan {
-  int nt, qtiles, chunks, chunk_tiles;
+  int nt, qtiles, whole, workers;
 };
 Plan plan_of(const PagedAttnArgs& g) {
   Plan p;
@@ -476,57 +655,58 @@ Plan plan_of(const PagedAttnArgs& g) {
   p.qtiles = (cols + 16 * p.nt - 1) / (16 * p.nt);
   int64_t keys = g.max_keys;
   if (g.window > 0) keys = std::min<int64_t>(keys, (int64_t)g.window + g.max_rows + g.sinks + 2 * kTileKeys);
-  const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
-  const int64_t groups = (int64_t)std::max(1, g.requests) * g.kv_heads * p.qtiles;
-  const int64_t want = std::max<int64_t>(1, 2048 / groups);  // workgroups: eight a compute unit
-  p.chunk_tiles = (int)std::max<int64_t>(2 * kWaves, (tiles + want - 1) / want);
-  p.chunks = (int)std::max<int64_t>(1, (tiles + p.chunk_tiles - 1) / p.chunk_tiles);
+  p.whole = keys <= kWholeKeys;
+  const int waves = g.head_dim == 48    ? instance_waves<48>(g, p.nt)
+                    : g.head_dim == 64 ? instance_waves<64>(g, p.nt)
+                                       : instance_waves<128>(g, p.nt);
+  const int64_t tiles = (int64_t)std::max(1, g.requests) * g.kv_heads * p.qtiles * ((keys + kTileKeys - 1) / kTileKeys + 1);
+  p.workers = (int)std::min<int64_t>((int64_t)kComputeUnits * waves, (tiles + kMinTiles - 1) / kMinTiles);
   return p;
 }
 
 template <int D, bool CB16, int QP, int NT>
-hipError_t launch(const PagedAttnArgs& g, int64_t blocks, hipStream_t s) {
-  hipLaunchKernelGGL((k_paged_attention<D, CB16, QP, NT>), dim3((unsigned)blocks), dim3(kWaves * 64), 0, s, g);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || g.chunks == 1) return e;
-  const int64_t items = (int64_t)g.requests * g.max_rows * g.heads;
-  hipLaunchKernelGGL((k_paged_join<D>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, g, 16 * NT);
+hipError_t launch(const PagedAttnArgs& g, hipStream_t s) {
+  const int64_t sequences = (int64_t)g.requests * g.qtiles * g.kv_heads;
+  hipLaunchKernelGGL((k_paged_attention<D, CB16, QP, NT>), dim3((unsigned)(g.whole ? sequences : g.workers)), dim3(kThreads), 0, s, g);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || g.whole) return e;
+  hipLaunchKernelGGL((k_paged_join<D, NT>), dim3((unsigned)(sequences * (16 * NT / kWaves))), dim3(kThreads), 0, s, g);
   return hipGetLastError();
 }
 template <int D>
-hipError_t launch_d(const PagedAttnArgs& g, int nt, int64_t blocks, hipStream_t s) {
-  if (!g.cache_bf16) return nt == 1 ? launch<D, false, 1, 1>(g, blocks, s) : launch<D, false, 1, 2>(g, blocks, s);
-  if (g.q_bf16) return nt == 1 ? launch<D, true, 1, 1>(g, blocks, s) : launch<D, true, 1, 2>(g, blocks, s);
-  return nt == 1 ? launch<D, true, 3, 1>(g, blocks, s) : launch<D, true, 3, 2>(g, blocks, s);
+hipError_t launch_d(const PagedAttnArgs& g, int nt, hipStream_t s) {
+  if (!g.cache_bf16) return nt == 1 ? launch<D, false, 1, 1>(g, s) : launch<D, false, 1, 2>(g, s);
+  if (g.q_bf16) return nt == 1 ? launch<D, true, 1, 1>(g, s) : launch<D, true, 1, 2>(g, s);
+  return nt == 1 ? launch<D, true, 3, 1>(g, s) : launch<D, true, 3, 2>(g, s);
 }
 
 }  // namespace
 
 bool paged_attention_launchable(const PagedAttnArgs& g) {
   const Plan p = plan_of(g);
-  return (int64_t)g.requests * g.kv_heads * p.qtiles * p.chunks <= 0x7FFFFF &&  // 2^31 threads
-         (int64_t)g.requests * g.max_rows * g.heads <= 0x1FFFFFF;
+  return (int64_t)g.requests * p.qtiles * g.kv_heads * (16 * p.nt / kWaves) <= 0x7FFFFF;  // 2^31 threads
 }
 
 size_t paged_attention_bytes(const PagedAttnArgs& g) {
   const Plan p = plan_of(g);
-  return p.chunks == 1 ? 0 : (size_t)g.rows * g.heads * p.chunks * (g.head_dim + 2) * sizeof(float);
+  return p.whole ? 0 : (size_t)p.workers * 2 * 16 * p.nt * (g.head_dim + 2) * sizeof(float);
 }
 
-hipError_t launch_paged_attention(const PagedAttnArgs& args, void* workspace, hipStream_t s) {
+hipError_t launch_paged_attention(const PagedAttnArgs& args, void* workspace, size_t workspace_bytes, hipStream_t s) {
   PagedAttnArgs g = args;
   if (g.requests == 0 || g.rows == 0) return hipSuccess;
+  const size_t bytes = paged_attention_bytes(g);
+  if (!paged_attention_launchable(g) || (bytes && (!workspace || workspace_bytes < bytes))) return hipErrorInvalidValue;
   const Plan p = plan_of(g);
   g.qtiles = p.qtiles;
-  g.chunks = p.chunks;
-  g.chunk_tiles = p.chunk_tiles;
+  g.whole = p.whole;
+  g.workers = p.workers;
+  g.min_tiles = kMinTiles;
   g.part_o = (float*)workspace;
-  g.part_ml = g.part_o + (size_t)g.rows * g.heads * p.chunks * g.head_dim;
-  const int64_t blocks = (int64_t)g.requests * g.kv_heads * p.qtiles * p.chunks;
-  if (!paged_attention_launchable(g)) return hipErrorInvalidValue;
-  if (g.head_dim == 48) return launch_d<48>(g, p.nt, blocks, s);
-  if (g.head_dim == 64) return launch_d<64>(g, p.nt, blocks, s);
-  if (g.head_dim == 128) return launch_d<128>(g, p.nt, blocks, s);
+  g.part_ml = g.part_o + (size_t)p.workers * 2 * 16 * p.nt * g.head_dim;
+  if (g.head_dim == 48) return launch_d<48>(g, p.nt, s);
+  if (g.head_dim == 64) return launch_d<64>(g, p.nt, s);
+  if (g.head_dim == 128) return launch_d<128>(g, p.nt, s);
   return hipErrorInvalidValue;
 }
 

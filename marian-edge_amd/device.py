@@ -211,12 +211,13 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, cu_rows, out, hea
         workspace.nbytes if workspace is not None else 0, _p(err), stream), "paged_attention")
 
 
-def paged_attention_workspace(rows: int, requests: int, max_rows: int, max_keys: int, heads: int, kv_heads: int,
-                              head_dim: int, window: int = 0, sinks: int = 0) -> int:
-    """Bytes of workspace of paged_attention."""
+def paged_attention_workspace(requests: int, max_rows: int, max_keys: int, heads: int, kv_heads: int, head_dim: int,
+                              window: int = 0, sinks: int = 0, bf16: bool = False, cache_bf16: bool = False) -> int:
+    """Bytes of workspace of paged_attention with these sizes and types."""
     n = C.c_size_t(0)
     _lib.check(_lib.load().marian_hip_paged_attention_workspace(
-        rows, requests, max_rows, max_keys, heads, kv_heads, head_dim, window, sinks, C.byref(n)), "paged_attention_workspace")
+        requests, max_rows, max_keys, heads, kv_heads, head_dim, int(bf16), int(cache_bf16), window, sinks, C.byref(n)),
+        "paged_attention_workspace")
     return n.value
 
 

@@ -171,3 +171,26 @@ def test_large_scores(dev, types):
     cache = po.Cache(rng, lengths, 1, 64, 16, TYPES[types][1])
     q = queries(rng, rows, 2, 64, types, size=30.0)
     check(run(dev, q, cache, lengths, rows, 2, types, scale=0.5), q, cache, lengths, rows, scale=0.5)
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("heads, kv_heads, d, rows", [(8, 8, 64, 1), (8, 2, 128, 3), (8, 8, 48, 1), (24, 1, 128, 1)])
+def test_workspace_is_as_large_as_it_says(dev, types, heads, kv_heads, d, rows):
+    """A call writes nothing past the bytes it asks for (a long cache in shares of all workgroups), and gives what it
+    gives with library scratch."""
+    rng = np.random.default_rng(d)
+    lengths, rows = [9000, 4000, 2], [rows] * 3
+    q_bf16, c_bf16 = TYPES[types]
+    cache = po.Cache(rng, lengths, kv_heads, d, 16, c_bf16)
+    q = queries(rng, rows, heads, d, types)
+    need = dev.paged_attention_workspace(3, max(rows), max(lengths), heads, kv_heads, d, bf16=q_bf16, cache_bf16=c_bf16)
+    assert need > 0
+    whole = dev.DeviceArray.from_host(np.full(need + 4096, 0x5A, np.uint8))
+
+    class Part:
+        ptr, nbytes = whole.ptr, need
+
+    got = run(dev, q, cache, lengths, rows, heads, types, workspace=Part)
+    after = whole.host()
+    assert (after[need:] == 0x5A).all() and (after[:need] != 0x5A).any()
+    assert np.array_equal(got, run(dev, q, cache, lengths, rows, heads, types))

@@ -135,11 +135,13 @@ def test_calls_without_work(pkg, lib):
 def test_workspace_sizes(pkg, lib):
     n = C.c_size_t(0)
     size = lib.marian_hip_paged_attention_workspace
-    assert size(1, 1, 1, 64, 8, 8, 64, 0, 0, C.byref(n)) == pkg._lib.OK and n.value == 0  # one piece
-    assert size(1, 1, 1, 100000, 8, 8, 64, 0, 0, C.byref(n)) == pkg._lib.OK and n.value > 8 * 64 * 4
-    assert size(1, 1, 1, 100000, 8, 8, 64, 0, 0, None) == pkg._lib.ERR_INVALID_INPUT
-    for bad in ((-1, 1, 1, 64, 8, 8, 64, 0, 0), (1, 1, 65, 64, 8, 8, 64, 0, 0), (1, 1, 1, 64, 8, 3, 64, 0, 0),
-                (1, 1, 1, 64, 8, 8, 65, 0, 0), (1, 1, 1, 64, 8, 8, 64, -1, 0)):
+    assert size(1, 1, 64, 8, 8, 64, 1, 1, 0, 0, C.byref(n)) == pkg._lib.OK and n.value == 0  # one piece
+    for q16, c16 in ((0, 0), (0, 1), (1, 1)):
+        assert size(1, 1, 100000, 8, 8, 64, q16, c16, 0, 0, C.byref(n)) == pkg._lib.OK and n.value > 8 * 64 * 4
+        assert size(1, 1, 100000, 8, 8, 64, q16, c16, 100, 4, C.byref(n)) == pkg._lib.OK and n.value == 0  # a short window
+    assert size(1, 1, 100000, 8, 8, 64, 1, 1, 0, 0, None) == pkg._lib.ERR_INVALID_INPUT
+    for bad in ((-1, 1, 64, 8, 8, 64, 1, 1, 0, 0), (1, 65, 64, 8, 8, 64, 1, 1, 0, 0), (1, 1, 64, 8, 3, 64, 1, 1, 0, 0),
+                (1, 1, 64, 8, 8, 65, 1, 1, 0, 0), (1, 1, 64, 8, 8, 64, 1, 1, -1, 0), (1, 1, 64, 8, 8, 64, 1, 0, 0, 0)):
         assert size(*bad, C.byref(n)) == pkg._lib.ERR_INVALID_INPUT
     of_rows = lib.marian_hip_verify_drafts_workspace
     assert of_rows(10, 0, C.byref(n)) == pkg._lib.OK
