@@ -642,9 +642,10 @@ struct PagedAttnArgs {
   int64_t ldo = 0;
   int* err = nullptr;  // set to 1 on a request or page out of range
   // Filled by launch_paged_attention.
-  int qtiles = 0, whole = 0, workers = 0, min_tiles = 0;
+  int qtiles = 0, whole = 0, workers = 0;
   float* part_o = nullptr;   // [workers, 2, columns of a query tile, head_dim]
   float* part_ml = nullptr;  // [workers, 2, columns, 2]: reference, sum of weights
+  int2* begun = nullptr;     // [sequences]: the workgroup that begins it, parts
 };
 constexpr int kPagedMaxRows = 64;          // of a request
 constexpr int kPagedMaxKeys = 1 << 27;

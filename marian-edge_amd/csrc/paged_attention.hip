@@ -17,6 +17,15 @@ namespace {
 
 constexpr int kTileKeys = 32;  // keys a wave takes at once
 constexpr int kWaves = 4;
+constexpr int kMinTiles = 2 * kWaves;  // of a share
+// What splitting sequences costs (another beginning and end in every workgroup, a second launch, about 10 us), as tiles
+// that one workgroup works on meanwhile: 0.11 us for 8 KB of keys and values.
+constexpr int kSplitCost = 64;
+constexpr int kRate = 64;  // workgroups that read as fast as the whole chip does
+template <int D, bool CB16, int NT>
+constexpr int split_cost() {
+  return kSplitCost * 8 / (D / 8 * (CB16 ? 1 : 2)) / NT;
+}
 // Scores (in octaves) may pass the reference by so much before the sums are rescaled: weights up to 2^8.
 constexpr float kSlack = 8.0f;
 
@@ -256,14 +265,18 @@ constexpr int waves_a_simd() {
   return NT == 1 ? 4 : 3;
 }
 
-// Work is counted in tiles of a (request, query tile, key head), in that order, head fastest: one at least for each that has
-// rows, so that rows that see nothing are written too.
+// A sequence is what one query tile and key head of a request see.  Work is counted in its tiles and kBegin more for its
+// beginning and end, in the order request, query tile, head.
+constexpr int kBegin = 8;
 template <int NT>
-__device__ __forceinline__ int64_t request_tiles(const PagedAttnArgs& g, const Request& r) {
+__device__ __forceinline__ int64_t request_tiles(const PagedAttnArgs& g, const Request& r, int& longest) {
   const int cols = r.n * g.group, pos0 = r.len - r.n;
   int64_t all = 0;
-  for (int col0 = 0; col0 < cols; col0 += 16 * NT)
-    all += max(1, span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles);
+  for (int col0 = 0; col0 < cols; col0 += 16 * NT) {
+    const int n = kBegin + span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles;
+    longest = max(longest, n);
+    all += n;
+  }
   return all * g.kv_heads;
 }
 
@@ -276,7 +289,8 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
   return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
 }
 
-// Where a workgroup's share of all tiles begins: request b, `into` tiles into it, `quota` tiles to take.
+// Where a workgroup's share of all tiles begins: request b, `into` tiles into it, `quota` tiles to take; quota 0: every
+// sequence is one workgroup's.
 struct Share {
   int b;
   int64_t into, quota;
@@ -284,19 +298,17 @@ struct Share {
 constexpr int kThreads = kWaves * 64;
 struct ShareLds {
   int64_t sum[kPlanMaxRequests / kThreads + 1], wave[kWaves], into;
-  int b;
+  int b, longest[kWaves];
 };
-__device__ __forceinline__ int64_t quota_of(const PagedAttnArgs& g, int64_t total) {
-  return max((total + g.workers - 1) / g.workers, (int64_t)g.min_tiles);
-}
 template <int NT>
-__device__ __forceinline__ Share share_of(const PagedAttnArgs& g, int worker, ShareLds& L) {
+__device__ __forceinline__ Share share_of(const PagedAttnArgs& g, int worker, int cost, ShareLds& L) {
   const int t = threadIdx.x, lane = t & 63, wave = uniform(t >> 6);
   const int steps = (g.requests + kThreads - 1) / kThreads;
   int64_t mine = 0, upto = 0, total = 0;
+  int longest = 0;
   auto step = [&](int i) {  // this thread's request's tiles, and their running sum within the step
     const int b = i * kThreads + t;
-    mine = b < g.requests ? request_tiles<NT>(g, request_of(g, b, worker == 0)) : 0;
+    mine = b < g.requests ? request_tiles<NT>(g, request_of(g, b, worker == 0), longest) : 0;
     upto = (int64_t)wave_scan_mass((uint64_t)mine);
     if (lane == 63) L.wave[wave] = upto;
     __syncthreads();
@@ -317,14 +329,24 @@ __device__ __forceinline__ Share share_of(const PagedAttnArgs& g, int worker, Sh
     }
     total += all;
   }
-  const int64_t quota = quota_of(g, total);
+  longest = (int)wave_max((float)longest);  // at most 2^22: exact
+  if (lane == 0) L.longest[wave] = longest;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) longest = max(longest, L.longest[w]);
+  longest = uniform(longest);
+  total = uniform64(total);
+  // Unsplit, the longest sequence ends last, and by so much later as it is longer than what the others do on average.
+  const int64_t at_rate = total / kRate, even = total / min((int64_t)g.workers, (int64_t)g.requests * g.qtiles * g.kv_heads);
+  if (max((int64_t)longest, at_rate) + max(longest - even, (int64_t)0) <= at_rate + cost) return {0, 0, 0};
+  const int64_t quota = max((total + g.workers - 1) / g.workers, (int64_t)kMinTiles + kBegin);
   int64_t at = (int64_t)worker * quota;
   int i = 0;
   if (steps > 1) {
     for (; i < steps - 1 && at >= L.sum[i]; ++i) at -= L.sum[i];
     step(i);
   }
-  if (mine && upto - mine <= at && at < upto) {
+  if (worker < g.workers && mine && upto - mine <= at && at < upto) {
     L.b = i * kThreads + t;
     L.into = at - (upto - mine);
   }
@@ -332,11 +354,11 @@ __device__ __forceinline__ Share share_of(const PagedAttnArgs& g, int worker, Sh
   return {uniform(L.b), uniform64(L.into), quota};
 }
 
-// A workgroup of four waves takes tiles of one (request, query tile of 16 NT (row, head) pairs, key head) after another:
-// either all of one (g.whole), or its share of all the call's tiles, the same number for every workgroup and as many
-// workgroups as run at once: then the caches' lengths may differ as they like, and a sequence is split where shares
-// meet.  The waves take turns at the tiles of a sequence and join at its end; what is not a whole sequence goes to
-// the workspace: part 0 of a workgroup is the end or middle of a sequence, part 1 the beginning of one.
+// A workgroup of four waves takes tiles of one sequence, in turns, and joins the waves' sums at its end.  With few keys
+// (g.whole), and where no sequence is long beside the rest, a sequence is one workgroup's.  Otherwise as many
+// workgroups as run at once take the same number of tiles each, one sequence after another, whatever their lengths; what
+// is not a whole sequence goes to the workspace: part 0 of a workgroup is the end or middle of a sequence, part 1 the
+// beginning of one.
 template <int D, bool CB16, int QP, int NT>
 __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k_paged_attention(PagedAttnArgs g) {
   constexpr int DT = D / 16;
@@ -346,30 +368,34 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int m = lane & 15, grp = lane >> 4;
   int b, qt = 0, head = 0;
-  int64_t left;  // tiles to take
-  int t0 = 0;
-  if (g.whole) {
+  int64_t quota = 0, left = 0;  // of work to take: in all, still
+  int u0 = 0;                   // of the sequence's work, where this part begins
+  if (!g.whole) {
+    const Share s = share_of<NT>(g, blockIdx.x, split_cost<D, CB16, NT>(), share);
+    b = s.b;
+    quota = left = s.quota;
+    if (b >= g.requests) return;
+  }
+  if (quota == 0) {
     int id = blockIdx.x;
     head = id % g.kv_heads;
     id /= g.kv_heads;
     qt = id % g.qtiles;
     b = id / g.qtiles;
+    if (b >= g.requests) return;
     left = 0x7FFFFFFF;
   } else {
-    const Share s = share_of<NT>(g, blockIdx.x, share);
-    b = s.b;
-    left = s.quota;
-    if (b >= g.requests) return;
+    const Share s = {b, uniform64(share.into), quota};
     // The query tile and head that the share begins in.
     const Request rq = request_of(g, b, false);
     const int cols = rq.n * g.group, pos0 = rq.len - rq.n;
     int64_t into = s.into;
     for (;; ++qt) {
       const int col0 = qt * 16 * NT;
-      const int tiles = max(1, span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles);
+      const int tiles = kBegin + span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles;
       if (into < (int64_t)tiles * g.kv_heads || col0 + 16 * NT >= cols) {
         head = (int)(into / tiles);
-        t0 = (int)(into % tiles);
+        u0 = (int)(into % tiles);
         break;
       }
       into -= (int64_t)tiles * g.kv_heads;
@@ -382,15 +408,19 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
     const Request rq = request_of(g, b, g.whole && head == 0 && qt == 0 && threadIdx.x == 0);
     const int cols = uniform(rq.n * g.group), col0 = qt * 16 * NT;
     if (col0 >= cols) {  // no (more) rows
-      if (g.whole || ++b >= g.requests) return;
-      qt = head = t0 = 0;
+      if (quota == 0 || ++b >= g.requests) return;
+      qt = head = u0 = 0;
       continue;
     }
     const int pos0 = rq.len - rq.n;
     const Span span = span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks);
-    const int t1 = (int)min((int64_t)max(1, span.tiles), t0 + left);
-    const bool alone = t0 == 0 && t1 >= span.tiles;
-    left -= t1 - t0;
+    const int all = kBegin + span.tiles, u1 = (int)min((int64_t)all, u0 + left);
+    const int t0 = max(0, u0 - kBegin), last = max(0, u1 - kBegin);  // of its tiles
+    const bool alone = u0 == 0 && u1 == all;
+    if (!g.whole && u0 == 0 && threadIdx.x == 0)  // its rest is the next workgroups'
+      g.begun[((int64_t)b * g.qtiles + qt) * g.kv_heads + head] =
+          make_int2(blockIdx.x, alone ? 1 : (int)((quota - left + all + quota - 1) / quota));
+    left -= u1 - u0;
 
     Query<D, CB16, QP> q[NT];
     int pos[NT];  // of the lane's column
@@ -415,7 +445,6 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
     auto block = [&](int page) -> int64_t { return ((int64_t)(in_range(page) ? page : 0) * g.kv_heads + head) * D << g.page_shift; };
 
     Tile<D, CB16> x;
-    const int last = min(t1, span.tiles);
     int it = t0 + wave;
     int page_k = 0, page_v = 0, next_k = 0, next_v = 0;
     auto load_k = [&](int tile, int page) {
@@ -507,7 +536,7 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
       }
     }
     __syncthreads();
-    const int64_t part = (int64_t)blockIdx.x * 2 + (t0 > 0 ? 0 : 1);
+    const int64_t part = (int64_t)blockIdx.x * 2 + (u0 > 0 ? 0 : 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float top = lds_m[0][n][m];
@@ -543,8 +572,8 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
         }
       }
     }
-    if (g.whole || left <= 0) return;
-    t0 = 0;
+    if (quota == 0 || left <= 0) return;
+    u0 = 0;
     if (++head == g.kv_heads) {
       head = 0;
       ++qt;
@@ -552,91 +581,72 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
   }
 }
 
-// Joins the parts of a sequence's columns, a wave each: the largest reference first, then the parts' sums, four dimensions
-// a lane and as many parts at once as fit.
+// Joins the parts of a sequence's columns, 1 << lg_cols columns a workgroup: the largest reference first, then the parts'
+// sums, four dimensions a lane, as many parts at once as fit, and the parts shared among a column's waves.
 template <int D, int NT>
-__global__ __launch_bounds__(kThreads) void k_paged_join(PagedAttnArgs g) {
+__global__ __launch_bounds__(kThreads) void k_paged_join(PagedAttnArgs g, int lg_cols) {
   constexpr int QUADS = D / 4, AT_ONCE = 64 / QUADS;  // D = 48: 5 parts, and four lanes idle
-  __shared__ int64_t before_w[kWaves], total_w[kWaves];
-  const int t = threadIdx.x, lane = t & 63, wave = uniform(t >> 6);
-  int id = blockIdx.x;
-  const int col_in = id % (16 * NT / kWaves) * kWaves + wave;
-  id /= 16 * NT / kWaves;
-  const int head = id % g.kv_heads;
-  id /= g.kv_heads;
-  const int qt = id % g.qtiles, b = id / g.qtiles;
+  __shared__ f4v lds_o[kWaves][QUADS];
+  __shared__ float lds_l[kWaves];
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  const int groups = 16 * NT >> lg_cols, seq = blockIdx.x / groups, split = wave >> lg_cols, splits = kWaves >> lg_cols;
+  const int base_col = blockIdx.x % groups << lg_cols, col_in = base_col + (wave & ((1 << lg_cols) - 1));
+  const int head = seq % g.kv_heads, qt = seq / g.kv_heads % g.qtiles, b = seq / g.kv_heads / g.qtiles;
   const Request rq = request_of(g, b, false);
-  const int cols = rq.n * g.group, col = qt * 16 * NT + col_in;
-  if (col - wave >= cols) return;
-  int64_t before = 0, total = 0;
-  for (int r = t; r < g.requests; r += kThreads) {
-    const int64_t n = request_tiles<NT>(g, request_of(g, r, false));
-    total += n;
-    before += r < b ? n : 0;
-  }
-  before = (int64_t)wave_scan_mass((uint64_t)before);
-  total = (int64_t)wave_scan_mass((uint64_t)total);
-  if (lane == 63) {
-    before_w[wave] = before;
-    total_w[wave] = total;
-  }
-  __syncthreads();
-  if (col >= cols) return;
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += before_w[w];
-    total += total_w[w];
-  }
-  const int64_t quota = quota_of(g, total);
-  const int pos0 = rq.len - rq.n;
-  int tiles = 0;
-  for (int j = 0; j <= qt; ++j) {
-    const int col0 = j * 16 * NT;
-    tiles = max(1, span_of(pos0 + col0 / g.group, pos0 + (min(cols, col0 + 16 * NT) - 1) / g.group, g.window, g.sinks).tiles);
-    before += (int64_t)tiles * (j < qt ? g.kv_heads : head);
-  }
-  const int64_t first = before / quota, last = (before + tiles - 1) / quota;
-  if (first == last) return;  // in one share: written already
-  const int parts = (int)(last - first) + 1;
-  auto place = [&](int p) -> int64_t { return ((first + p) * 2 + (p == 0 ? 1 : 0)) * (16 * NT) + col_in; };
+  const int cols = uniform(rq.n * g.group) - qt * 16 * NT;
+  if (base_col >= cols) return;
+  const int2 begun = g.begun[seq];
+  const int first = uniform(begun.x), parts = uniform(begun.y);
+  if (parts < 2) return;
+  auto place = [&](int p) -> int64_t { return ((int64_t)(first + p) * 2 + (p == 0 ? 1 : 0)) * (16 * NT) + col_in; };
   const float2* ml = (const float2*)g.part_ml;
-  float top = -INFINITY;
-  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[place(p)].x);
-  top = wave_max(top);
-  const float base = top > -INFINITY ? top : 0.0f;
   const int quad = lane % QUADS, row = lane / QUADS;
   f4v v = {0, 0, 0, 0};
   float sum = 0.0f;
-  if (row < AT_ONCE) {
+  if (col_in < cols) {
+    float top = -INFINITY;
+    for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[place(p)].x);
+    top = wave_max(top);
+    const float base = top > -INFINITY ? top : 0.0f;
+    if (row < AT_ONCE) {
 #pragma unroll 8
-    for (int p = row; p < parts; p += AT_ONCE) {
-      const int64_t at = place(p);
-      const float2 e = ml[at];
-      const f4v x = *(const f4v*)(g.part_o + at * D + 4 * quad);
-      const float by = e.x > -INFINITY ? exp2_fast(e.x - base) : 1.0f;
-      sum += e.y * by;
-      v += x * by;
+      for (int p = split * AT_ONCE + row; p < parts; p += splits * AT_ONCE) {
+        const int64_t at = place(p);
+        const float2 e = ml[at];
+        const f4v x = *(const f4v*)(g.part_o + at * D + 4 * quad);
+        const float by = e.x > -INFINITY ? exp2_fast(e.x - base) : 1.0f;
+        sum += e.y * by;
+        v += x * by;
+      }
+    }
+    const f4v own = v;
+    const float own_sum = sum;
+#pragma unroll
+    for (int r = 1; r < AT_ONCE; ++r) {  // into the first lanes
+      const int from = (lane + r * QUADS) & 63;
+      sum += __shfl(own_sum, from);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __shfl(own[i], from);
     }
   }
-  const f4v own = v;
-  const float own_sum = sum;
-#pragma unroll
-  for (int r = 1; r < AT_ONCE; ++r) {  // into the first lanes
-    const int from = (lane + r * QUADS) & 63;
-    sum += __shfl(own_sum, from);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] += __shfl(own[c], from);
+  if (splits > 1) {
+    if (lane < QUADS) lds_o[wave][lane] = v;
+    if (lane == 0) lds_l[wave] = sum;
+    __syncthreads();
+    if (split > 0) return;
+    for (int w = 1; w < splits; ++w) {
+      v += lds_o[wave + (w << lg_cols)][quad];
+      sum += lds_l[wave + (w << lg_cols)];
+    }
   }
-  if (lane < QUADS) {
-    const int i = col / g.group, hq = head * g.group + col % g.group;
-    *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 4 * quad) = pos0 + i >= 0 ? v / sum : f4v{0, 0, 0, 0};
+  if (col_in < cols && lane < QUADS) {
+    const int col = qt * 16 * NT + col_in, i = col / g.group, hq = head * g.group + col % g.group;
+    *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 4 * quad) =
+        rq.len - rq.n + i >= 0 ? v / sum : f4v{0, 0, 0, 0};
   }
 }
 
 constexpr int kComputeUnits = 256;
-constexpr int kMinTiles = 2 * kWaves;  // of a share
-constexpr int kWholeKeys = 512;  // caches up to this long are one workgroup's
 template <int D>
 int instance_waves(const PagedAttnArgs& g, int nt) {
   if (!g.cache_bf16) return nt == 1 ? waves_a_simd<D, false, 1, 1>() : waves_a_simd<D, false, 1, 2>();
@@ -655,22 +665,27 @@ Plan plan_of(const PagedAttnArgs& g) {
   p.qtiles = (cols + 16 * p.nt - 1) / (16 * p.nt);
   int64_t keys = g.max_keys;
   if (g.window > 0) keys = std::min<int64_t>(keys, (int64_t)g.window + g.max_rows + g.sinks + 2 * kTileKeys);
-  p.whole = keys <= kWholeKeys;
+  const int64_t sequences = (int64_t)g.requests * p.qtiles * g.kv_heads;
   const int waves = g.head_dim == 48    ? instance_waves<48>(g, p.nt)
                     : g.head_dim == 64 ? instance_waves<64>(g, p.nt)
                                        : instance_waves<128>(g, p.nt);
-  const int64_t tiles = (int64_t)std::max(1, g.requests) * g.kv_heads * p.qtiles * ((keys + kTileKeys - 1) / kTileKeys + 1);
-  p.workers = (int)std::min<int64_t>((int64_t)kComputeUnits * waves, (tiles + kMinTiles - 1) / kMinTiles);
+  const int64_t tiles_most = (keys + kTileKeys - 1) / kTileKeys;
+  const int cost = kSplitCost * 8 / (g.head_dim / 8 * (g.cache_bf16 ? 1 : 2)) / p.nt;
+  const int64_t tiles = (int64_t)std::max(1, g.requests) * g.kv_heads * p.qtiles * (tiles_most + kBegin + 1);
+  p.workers = (int)std::min<int64_t>((int64_t)kComputeUnits * waves, (tiles + kMinTiles + kBegin - 1) / (kMinTiles + kBegin));
+  p.whole = tiles_most <= cost || sequences >= 4 * kComputeUnits * waves;
   return p;
 }
 
 template <int D, bool CB16, int QP, int NT>
 hipError_t launch(const PagedAttnArgs& g, hipStream_t s) {
   const int64_t sequences = (int64_t)g.requests * g.qtiles * g.kv_heads;
-  hipLaunchKernelGGL((k_paged_attention<D, CB16, QP, NT>), dim3((unsigned)(g.whole ? sequences : g.workers)), dim3(kThreads), 0, s, g);
+  hipLaunchKernelGGL((k_paged_attention<D, CB16, QP, NT>), dim3((unsigned)(g.whole ? sequences : std::max<int64_t>(sequences, g.workers))),
+                     dim3(kThreads), 0, s, g);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || g.whole) return e;
-  hipLaunchKernelGGL((k_paged_join<D, NT>), dim3((unsigned)(sequences * (16 * NT / kWaves))), dim3(kThreads), 0, s, g);
+  const int lg_cols = sequences < kComputeUnits ? 0 : 2;
+  hipLaunchKernelGGL((k_paged_join<D, NT>), dim3((unsigned)(sequences * (16 * NT >> lg_cols))), dim3(kThreads), 0, s, g, lg_cols);
   return hipGetLastError();
 }
 template <int D>
@@ -684,12 +699,13 @@ hipError_t launch_d(const PagedAttnArgs& g, int nt, hipStream_t s) {
 
 bool paged_attention_launchable(const PagedAttnArgs& g) {
   const Plan p = plan_of(g);
-  return (int64_t)g.requests * p.qtiles * g.kv_heads * (16 * p.nt / kWaves) <= 0x7FFFFF;  // 2^31 threads
+  return (int64_t)g.requests * p.qtiles * g.kv_heads * (p.whole ? 1 : 8 * p.nt) <= 0x7FFFFF;  // 2^31 threads
 }
 
 size_t paged_attention_bytes(const PagedAttnArgs& g) {
   const Plan p = plan_of(g);
-  return p.whole ? 0 : (size_t)p.workers * 2 * 16 * p.nt * (g.head_dim + 2) * sizeof(float);
+  const size_t sequences = (size_t)g.requests * p.qtiles * g.kv_heads;
+  return p.whole ? 0 : (size_t)p.workers * 2 * 16 * p.nt * (g.head_dim + 2) * sizeof(float) + sequences * sizeof(int2);
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& args, void* workspace, size_t workspace_bytes, hipStream_t s) {
@@ -701,9 +717,9 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, void* workspace, si
   g.qtiles = p.qtiles;
   g.whole = p.whole;
   g.workers = p.workers;
-  g.min_tiles = kMinTiles;
   g.part_o = (float*)workspace;
   g.part_ml = g.part_o + (size_t)p.workers * 2 * 16 * p.nt * g.head_dim;
+  g.begun = (int2*)(g.part_ml + (size_t)p.workers * 2 * 16 * p.nt * 2);
   if (g.head_dim == 48) return launch_d<48>(g, p.nt, s);
   if (g.head_dim == 64) return launch_d<64>(g, p.nt, s);
   if (g.head_dim == 128) return launch_d<128>(g, p.nt, s);
