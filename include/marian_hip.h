@@ -615,8 +615,8 @@ int marian_hip_verify_drafts(const void* logits, int64_t ld, int64_t rows, int64
                              const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
                              const float* u_draw, int32_t* token, int32_t* accepted, void* workspace,
                              size_t workspace_bytes, int* err, void* stream);
-/* Bytes of workspace of a call with these rows (drafted: with draft_logits). */
-int marian_hip_verify_drafts_workspace(int64_t rows, int drafted, size_t* bytes);
+/* Bytes of workspace of a call with these sizes (drafted: with draft_logits). */
+int marian_hip_verify_drafts_workspace(int64_t rows, int64_t requests, int64_t V, int drafted, size_t* bytes);
 
 /* Variable-length attention: query row i belongs to sequence seq_of_row[i]
  * and attends over key rows [cu_k[s], cu_k[s+1]); max_keys bounds every range

@@ -165,7 +165,7 @@ SIGNATURES = {
     "marian_hip_paged_attention_workspace": (C.c_int, [_I64] * 6 + [C.c_int] * 2 + [_I64] * 2 + [C.POINTER(_SZ)]),
     "marian_hip_verify_drafts": (C.c_int, [_P, _I64, _I64, _I64, C.c_int, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _P,
                                            _P, _P, _P, _P, _P, _SZ, _P, _P]),
-    "marian_hip_verify_drafts_workspace": (C.c_int, [_I64, C.c_int, C.POINTER(_SZ)]),
+    "marian_hip_verify_drafts_workspace": (C.c_int, [_I64, _I64, _I64, C.c_int, C.POINTER(_SZ)]),
     "marian_hip_attention": (C.c_int, [_P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, C.c_int, _P, _I64, _P]),
     "marian_hip_vocab_argmax": (C.c_int, [_P, _P, _I64, _I64, _P, _P, _P, _I64, C.c_uint32, _P, _P, _P]),
     "marian_hip_candidate_argmax": (C.c_int, [_P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _P, _I64, _P, _P, _P, _P]),

@@ -543,6 +543,7 @@ hipError_t launch_sample(const SampleArgs& g, hipStream_t s);
 constexpr uint32_t kKeptInf = 1u, kKeptOne = 2u;
 struct RowKept {
   uint64_t total;
+  double draft_share;  // of the id drafted there
   float max, border_v;
   int border_id;
   uint32_t flags;
@@ -557,7 +558,9 @@ struct KeptArgs : SampleArgs {
   int64_t ld_draft = 0;
   const int32_t* draft_row = nullptr;
   int draft_rows = 0;
+  const int32_t* drafts = nullptr;
   RowKept* kept = nullptr;
+  int32_t* done = nullptr;  // [requests], set to 0
 };
 hipError_t launch_kept(const KeptArgs& g, hipStream_t s);
 
@@ -566,12 +569,13 @@ hipError_t launch_kept(const KeptArgs& g, hipStream_t s);
 // whose draft is not, or a request's last, one id is drawn with u_draw[b]: from max(p - q, 0), or p at the last.
 // token[r]: the accepted drafts, the drawn id, -1; accepted[b] how many drafts.
 struct VerifyArgs : KeptArgs {
-  const int32_t* drafts = nullptr;
   const float* u_draw = nullptr;
+  uint64_t* seg = nullptr;  // [requests, groups of 256 ids]
   int max_rows = 0;  // of a request
   int32_t* accepted = nullptr;
 };
-hipError_t launch_verify(const VerifyArgs& g, hipStream_t s);
+size_t verify_bytes(int64_t rows, int64_t requests, int64_t V, bool drafted);
+hipError_t launch_verify(const VerifyArgs& g, void* workspace, size_t workspace_bytes, hipStream_t s);
 
 // ---- a step over a paged key-value cache ----
 // Key cache [pages, kv_heads, page_size, head_dim], value cache [pages, kv_heads, head_dim, page_size] of fp32 or bf16;
@@ -649,7 +653,6 @@ struct PagedAttnArgs {
 };
 constexpr int kPagedMaxRows = 64;          // of a request
 constexpr int kPagedMaxKeys = 1 << 27;
-bool paged_attention_launchable(const PagedAttnArgs& g);  // within a grid's limits
 size_t paged_attention_bytes(const PagedAttnArgs& g);
 hipError_t launch_paged_attention(const PagedAttnArgs& g, void* workspace, size_t workspace_bytes, hipStream_t s);
 

@@ -5,6 +5,7 @@
 #pragma once
 
 #include "device_common.h"
+#include "kernels.h"
 #include "ref_expf.h"
 
 namespace mh {
@@ -88,6 +89,19 @@ __device__ __forceinline__ float order_logit(uint32_t k) {  // inverse of argmax
 }
 __device__ __forceinline__ float pair_logit(uint64_t p) { return order_logit((uint32_t)(p >> 32)); }
 __device__ __forceinline__ int pair_id(uint64_t p) { return (int)(0xFFFFFFFFu - (uint32_t)p); }
+
+__device__ __forceinline__ Octaves octaves_of(float temperature) {
+  const double per_logit = fmax(1.4426950408889634 / (double)temperature, 0x1p-900);
+  return {per_logit, -60.0 / per_logit};
+}
+
+// The mass of an id with logit v among what a row's settings keep.
+__device__ __forceinline__ double kept_mass(const RowKept& k, const Octaves& scale, float v, int id, const uint64_t* exp2) {
+  if (k.flags & kKeptOne) return id == k.border_id ? 1.0 : 0.0;
+  if (k.flags & kKeptInf) v = v == INFINITY ? 0.0f : -INFINITY;
+  if (!(v > k.border_v || (v == k.border_v && id <= k.border_id))) return 0.0;
+  return (double)mass_of_steps(octave_steps((double)v - (double)k.max, scale), exp2);
+}
 
 }  // namespace
 }  // namespace mh

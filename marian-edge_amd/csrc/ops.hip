@@ -612,7 +612,6 @@ const char* paged_attention_sizes(PagedAttnArgs& g, int64_t requests, int64_t ma
   g.head_dim = (int)head_dim;
   g.window = (int)window;
   g.sinks = (int)sinks;
-  if (!paged_attention_launchable(g)) return "too many requests, rows and heads for one call";
   return nullptr;
 }
 }  // namespace
@@ -686,14 +685,11 @@ int marian_hip_paged_attention(const void* q, int64_t ldq, int q_bf16, int64_t r
   return op_status(launch_paged_attention(g, workspace, workspace_bytes, s), "paged_attention");
 }
 
-namespace {
-size_t verify_bytes(int64_t rows, bool drafted) { return (size_t)rows * (drafted ? 2 : 1) * sizeof(RowKept); }
-}  // namespace
-
-int marian_hip_verify_drafts_workspace(int64_t rows, int drafted, size_t* bytes) {
+int marian_hip_verify_drafts_workspace(int64_t rows, int64_t requests, int64_t V, int drafted, size_t* bytes) {
   if (!bytes) return refuse("verify_drafts_workspace: bytes is missing");
-  if (rows < 0 || rows > kPlanMaxRows) return refuse("verify_drafts_workspace: sizes out of range");
-  *bytes = verify_bytes(rows, drafted != 0);
+  if (rows < 0 || rows > kPlanMaxRows || requests < 0 || requests > kPlanMaxRequests || V <= 0 || V > kSampleMaxIds)
+    return refuse("verify_drafts_workspace: sizes out of range");
+  *bytes = verify_bytes(rows, requests, V, drafted != 0);
   return MARIAN_HIP_OK;
 }
 
@@ -713,7 +709,7 @@ int marian_hip_verify_drafts(const void* logits, int64_t ld, int64_t rows, int64
     return refuse("verify_drafts: sizes of the draft rows out of range");
   if (!draft_logits && draft_row) return refuse("verify_drafts: draft_row without draft_logits");
   if ((uintptr_t)workspace & 7) return refuse("verify_drafts: the workspace must be 8-byte aligned");
-  const size_t value = in_bf16 ? 2 : 4, bytes = verify_bytes(rows, draft_logits != nullptr);
+  const size_t value = in_bf16 ? 2 : 4, bytes = verify_bytes(rows, requests, V, draft_logits != nullptr);
   const size_t w = (size_t)requests * 4, r = (size_t)rows * 4;
   const Span outs[] = {{token, r}, {accepted, w}, {workspace, workspace_bytes}};
   const Span ins[] = {{logits, rows_bytes(rows, ld, V, value)}, {draft_logits, rows_bytes(draft_rows, ld_draft, V, value)},
@@ -728,6 +724,7 @@ int marian_hip_verify_drafts(const void* logits, int64_t ld, int64_t rows, int64
     if (capturing(s)) return refuse("verify_drafts: a call that is captured into a graph needs a workspace");
     workspace = op_scratch(3, bytes, s);
     if (!workspace) return op_status(hipErrorOutOfMemory, "verify_drafts scratch");
+    workspace_bytes = bytes;
   }
   VerifyArgs g;
   g.logits = logits;
@@ -748,12 +745,11 @@ int marian_hip_verify_drafts(const void* logits, int64_t ld, int64_t rows, int64
   g.ld_draft = ld_draft;
   g.draft_row = draft_row;
   g.draft_rows = (int)draft_rows;
-  g.kept = (RowKept*)workspace;
   g.drafts = drafts;
   g.u_draw = u_draw;
   g.max_rows = (int)max_rows;
   g.accepted = accepted;
-  return op_status(launch_verify(g, s), "verify_drafts");
+  return op_status(launch_verify(g, workspace, workspace_bytes, s), "verify_drafts");
 }
 
 int marian_hip_attention(const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv,

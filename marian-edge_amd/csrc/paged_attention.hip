@@ -679,6 +679,7 @@ Plan plan_of(const PagedAttnArgs& g) {
 
 template <int D, bool CB16, int QP, int NT>
 hipError_t launch(const PagedAttnArgs& g, hipStream_t s) {
+  // At most 2^23 workgroups: 8192 requests, 64 rows each, 128 heads.
   const int64_t sequences = (int64_t)g.requests * g.qtiles * g.kv_heads;
   hipLaunchKernelGGL((k_paged_attention<D, CB16, QP, NT>), dim3((unsigned)(g.whole ? sequences : std::max<int64_t>(sequences, g.workers))),
                      dim3(kThreads), 0, s, g);
@@ -697,11 +698,6 @@ hipError_t launch_d(const PagedAttnArgs& g, int nt, hipStream_t s) {
 
 }  // namespace
 
-bool paged_attention_launchable(const PagedAttnArgs& g) {
-  const Plan p = plan_of(g);
-  return (int64_t)g.requests * p.qtiles * g.kv_heads * (p.whole ? 1 : 8 * p.nt) <= 0x7FFFFF;  // 2^31 threads
-}
-
 size_t paged_attention_bytes(const PagedAttnArgs& g) {
   const Plan p = plan_of(g);
   const size_t sequences = (size_t)g.requests * p.qtiles * g.kv_heads;
@@ -712,7 +708,7 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, void* workspace, si
   PagedAttnArgs g = args;
   if (g.requests == 0 || g.rows == 0) return hipSuccess;
   const size_t bytes = paged_attention_bytes(g);
-  if (!paged_attention_launchable(g) || (bytes && (!workspace || workspace_bytes < bytes))) return hipErrorInvalidValue;
+  if (bytes && (!workspace || workspace_bytes < bytes)) return hipErrorInvalidValue;
   const Plan p = plan_of(g);
   g.qtiles = p.qtiles;
   g.whole = p.whole;

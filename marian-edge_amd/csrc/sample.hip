@@ -159,7 +159,9 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
     wg_lds_barrier();
     set = __builtin_amdgcn_readfirstlane(L.found);
     last = __builtin_amdgcn_readfirstlane(L.best);
-    if (set < 0 || (row >= g.rows && r == last)) return;  // no request's, or a request's last row: nothing was drafted after it
+    if (set < 0) return;  // no request's
+    if (t == 0 && row < g.rows && r == g.cu[set]) g.done[set] = 0;
+    if (row >= g.rows && r == last) return;  // nothing was drafted after a request's last row
     wg_lds_barrier();  // found and best are used again
   }
 
@@ -196,8 +198,17 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
     if (g.logprob) g.logprob[row] = logprob;
   };
   if (!valid && t == 0 && g.err) *g.err = 1;
-  auto record = [&](uint64_t total, float max, float v, int id, bool only, bool one) {  // one thread
-    if constexpr (KEPT) g.kept[row] = RowKept{total, max, v, id, (only ? kKeptInf : 0u) | (one ? kKeptOne : 0u)};
+  // The record, and the draft's share in it (one thread).
+  const uint64_t* exp2 = L.exp2;
+  auto record = [&](uint64_t total, float max, float v, int id, bool only, bool one) {
+    if constexpr (KEPT) {
+      RowKept k = {total, 0.0, max, v, id, (only ? kKeptInf : 0u) | (one ? kKeptOne : 0u)};
+      const int r = (int)(row < g.rows ? row : row - g.rows), draft = g.drafts[r];
+      if (total && (uint32_t)draft < (uint32_t)g.V)
+        k.draft_share = kept_mass(k, octaves_of(temp), BF16 ? bf16_to_f32(((const uint16_t*)base)[draft]) : ((const float*)base)[draft],
+                                  draft, exp2) / (double)total;
+      g.kept[row] = k;
+    }
   };
   if (n == 0) {
     if (t == 0) finish(-1, -INFINITY);
@@ -354,7 +365,7 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
   }
   const double per_logit = 1.4426950408889634 / (double)temp;  // octaves of p
   auto octave = [&](float v) -> double { return ((double)v - (double)lmax) * per_logit; };
-  const Octaves scale = {fmax(per_logit, 0x1p-900), -60.0 / fmax(per_logit, 0x1p-900)};
+  const Octaves scale = octaves_of(temp);
   auto steps_of = [&](float v) -> Octave { return octave_steps((double)v - (double)lmax, scale); };
   auto mass_of = [&](float v) -> uint64_t { return mass_of_steps(steps_of(v), L.exp2); };
   auto bin_of = [&](float v) -> int { return -steps_of(v).steps; };
@@ -487,7 +498,7 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
     // ---- the list: all ids at their own places, or those of the stage's bins (of a
     // part of one when it is crowded) ----
     uint32_t listed = n;
-    uint64_t need = 0;
+    uint64_t need = 0, above = 0;  // of BORDER_P: the mass to reach in the list, and the mass ahead of it
     if (stage == LIST_ALL) {
       each([&](int, int i, f4v v) {
 #pragma unroll
@@ -498,6 +509,7 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
     } else {
       int first = 0, last = 0, shift = -1;  // shift: of a part's number
       uint64_t lo = 0, hi = ~0ull;          // pairs looked at
+      above = 0;
 #pragma unroll 1
       for (;;) {
         if (shift >= 0) {
@@ -538,6 +550,7 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
           first = stage == LIST_TOP ? 0 : f.bin;
         }
         need -= f.before;
+        above += f.before;
         if (last >= 0) {
           const float least = least_of(last), most = first ? most_of(first) : INFINITY;
           each([&](int, int i, f4v v) {
@@ -609,6 +622,12 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
       wg_lds_barrier();
       border_v = pair_logit(L.sorted[L.border]);
       border_id = pair_id(L.sorted[L.border]);
+      if constexpr (KEPT) {
+        if (least_v <= border_v) {
+          if (t == (int)L.border) record(above + before + m, lmax, border_v, border_id, only_inf, false);
+          return;
+        }
+      }
       stage = DRAW;
       continue;
     }

@@ -236,10 +236,10 @@ def verify_drafts(logits, drafts, cu_rows, u, u_draw, token, accepted, max_rows=
         "verify_drafts")
 
 
-def verify_drafts_workspace(rows: int, drafted: bool) -> int:
+def verify_drafts_workspace(rows: int, requests: int, ids: int, drafted: bool) -> int:
     """Bytes of workspace of verify_drafts (drafted: with draft_logits)."""
     n = C.c_size_t(0)
-    _lib.check(_lib.load().marian_hip_verify_drafts_workspace(rows, int(drafted), C.byref(n)), "verify_drafts_workspace")
+    _lib.check(_lib.load().marian_hip_verify_drafts_workspace(rows, requests, ids, int(drafted), C.byref(n)), "verify_drafts_workspace")
     return n.value
 
 

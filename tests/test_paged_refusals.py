@@ -93,7 +93,6 @@ def attention_args(**change):
     (dict(out=at(0)), "overlaps"), (dict(out=at(1) + 1024), "overlaps"), (dict(out=at(3)), "overlaps"), (dict(ws=at(2)), "overlaps"),
     (dict(ws=at(6) + 1024), "overlaps"), (dict(ws=at(4)), "overlaps"),
     (dict(max_keys=1 << 20, blocks=1 << 17, ws_bytes=16), "too small"),
-    (dict(requests=8192, max_rows=64, heads=128, kv_heads=128, ldq=8192, ldo=8192), "too many"),
 ])
 def test_attention_refuses(pkg, lib, change, why):
     assert lib.marian_hip_paged_attention(*attention_args(**change)) == pkg._lib.ERR_INVALID_INPUT
@@ -144,7 +143,9 @@ def test_workspace_sizes(pkg, lib):
                 (1, 1, 64, 8, 8, 65, 1, 1, 0, 0), (1, 1, 64, 8, 8, 64, 1, 1, -1, 0), (1, 1, 64, 8, 8, 64, 1, 0, 0, 0)):
         assert size(*bad, C.byref(n)) == pkg._lib.ERR_INVALID_INPUT
     of_rows = lib.marian_hip_verify_drafts_workspace
-    assert of_rows(10, 0, C.byref(n)) == pkg._lib.OK
+    assert of_rows(10, 3, 1000, 0, C.byref(n)) == pkg._lib.OK
     one = n.value
-    assert of_rows(10, 1, C.byref(n)) == pkg._lib.OK and n.value == 2 * one > 0
-    assert of_rows(-1, 1, C.byref(n)) == pkg._lib.ERR_INVALID_INPUT and of_rows(1, 1, None) == pkg._lib.ERR_INVALID_INPUT
+    assert of_rows(10, 3, 1000, 1, C.byref(n)) == pkg._lib.OK and n.value > one > 0
+    for bad in ((-1, 3, 1000, 1), (10, -1, 1000, 1), (10, 8193, 1000, 1), (10, 3, 0, 1), (10, 3, 1 << 20, 1)):
+        assert of_rows(*bad, C.byref(n)) == pkg._lib.ERR_INVALID_INPUT
+    assert of_rows(1, 1, 1, 1, None) == pkg._lib.ERR_INVALID_INPUT
