@@ -354,6 +354,61 @@ __device__ __forceinline__ Share share_of(const PagedAttnArgs& g, int worker, in
   return {uniform(L.b), uniform64(L.into), quota};
 }
 
+// One column's keys one after the other, a wave's lanes (m, g): the column of query m, dimensions d % 4 == g of the score
+// and 16 d + 4 g .. 4 g + 3 of the sums, which are kept in `o` (LDS).
+template <int D, bool CB16>
+struct Slow {
+  const PagedAttnArgs& g;
+  const Span& span;
+  const int32_t* table;
+  f4v* o;
+  int head, lane;
+  float ref, sum;
+  __device__ __forceinline__ float value(const void* p, int64_t i) const {
+    return CB16 ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i];
+  }
+  __device__ void sum_keys(int64_t query, int pos, int first, int last) {
+    const int grp = lane >> 4, place_mask = (1 << g.page_shift) - 1;
+    ref = -INFINITY;
+    sum = 0.0f;
+#pragma unroll 1
+    for (int d = 0; d < D / 16; ++d) o[d * 64 + lane] = f4v{0, 0, 0, 0};
+#pragma unroll 1
+    for (int it = first; it < last; it += kWaves) {
+#pragma unroll 1
+      for (int i = 0; i < kTileKeys; ++i) {
+        const int key = span.tile(it) * kTileKeys + i;
+        if (key > span.last_pos) break;
+        const int page = table[key >> g.page_shift], place = key & place_mask;
+        const bool there = (uint32_t)page < (uint32_t)g.num_pages;
+        const int64_t block = ((int64_t)(there ? page : 0) * g.kv_heads + head) * D << g.page_shift;
+        float score = 0.0f;
+#pragma unroll 1
+        for (int d = grp; d < D; d += 4) {
+          const float a = g.q_bf16 ? bf16_to_f32(((const uint16_t*)g.q)[query + d]) : ((const float*)g.q)[query + d];
+          score = __builtin_fmaf(a, value(g.k, block + (int64_t)place * D + d), score);
+        }
+        score += xor_lane_f<16>(score);
+        score += xor_lane_f<32>(score);
+        score *= g.scale_log2e;
+        if (!there || key > pos || (g.window > 0 && key <= pos - g.window && key >= g.sinks)) continue;
+        const float to = score > ref ? score : ref;
+        const float by = to > -INFINITY ? exp2_fast(ref - to) : 1.0f, w = exp2_fast(score - (to > -INFINITY ? to : 0.0f));
+        ref = to;
+        sum = sum * by + w;
+#pragma unroll 1
+        for (int d = 0; d < D / 16; ++d) {
+          f4v v = o[d * 64 + lane] * by;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = __builtin_fmaf(w, value(g.v, block + ((int64_t)(16 * d + 4 * grp + e) << g.page_shift) + place), v[e]);
+          o[d * 64 + lane] = v;
+        }
+      }
+    }
+  }
+};
+
 // A workgroup of four waves takes tiles of one sequence, in turns, and joins the waves' sums at its end.  With few keys
 // (g.whole), and where no sequence is long beside the rest, a sequence is one workgroup's.  Otherwise as many
 // workgroups as run at once take the same number of tiles each, one sequence after another, whatever their lengths; what
@@ -365,6 +420,7 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
   __shared__ __attribute__((aligned(16))) float lds_o[kWaves][DT * 64 * 4];
   __shared__ float lds_m[kWaves][NT][16], lds_l[kWaves][NT][16];
   __shared__ ShareLds share;
+  __shared__ int lds_odd[kWaves];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int m = lane & 15, grp = lane >> 4;
   int b, qt = 0, head = 0;
@@ -526,49 +582,89 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
     }
 
     // ---- the waves' parts, then the rows' or the share's ----
+    // The lane, unknown to the compiler: it would keep what follows from it in registers all along.
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const int lm = l & 15, lg = l >> 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       sum[n] += xor_lane_f<16>(sum[n]);
       sum[n] += xor_lane_f<32>(sum[n]);
-      if (lane < 16) {
-        lds_m[wave][n][m] = ref[n];
-        lds_l[wave][n][m] = sum[n];
+      if (l < 16) {
+        lds_m[wave][n][lm] = ref[n];
+        lds_l[wave][n][lm] = sum[n];
       }
     }
+    // Infinities and NaN: a weight of zero times one that a row does not see, or a part of a product, makes a NaN of what is
+    // none.  Sums with any are formed again, key by key in the formula's own terms, as slow as that is.
+    float zero = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      zero = __builtin_fmaf(sum[n], 0.0f, zero);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(o[n][d][i], 0.0f, zero);
+    }
+    const bool odd = __any(zero != 0.0f);
+    if (l == 0) lds_odd[wave] = odd;
     __syncthreads();
+    if (lds_odd[0] | lds_odd[1] | lds_odd[2] | lds_odd[3]) {
+      if (odd) {
+        Slow<D, CB16> slow = {g, span, table, (f4v*)lds_o[wave], head, l};
+#pragma unroll 1
+        for (int n = 0; n < NT; ++n) {
+          const int col = min(col0 + 16 * n + lm, cols - 1);
+          slow.sum_keys((int64_t)(rq.row0 + col / g.group) * g.ldq + (head * g.group + col % g.group) * D, pos0 + col / g.group,
+                        t0 + wave, last);
+          if (l < 16) {
+            lds_m[wave][n][l] = slow.ref;
+            lds_l[wave][n][l] = slow.sum;
+          }
+#pragma unroll
+          for (int k = 0; k < NT; ++k) {
+            if (k != n) continue;
+            ref[k] = slow.ref;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[k][d] = slow.o[d * 64 + l];
+          }
+        }
+      }
+      __syncthreads();
+    }
     const int64_t part = (int64_t)blockIdx.x * 2 + (u0 > 0 ? 0 : 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float top = lds_m[0][n][m];
+      float top = lds_m[0][n][lm];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][n][m]);
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][n][lm]);
       float total = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float r = lds_m[w][n][m];
-        total += r > -INFINITY ? lds_l[w][n][m] * exp2_fast(r - top) : lds_l[w][n][m];
+        const float r = lds_m[w][n][lm];
+        total += r > -INFINITY ? lds_l[w][n][lm] * exp2_fast(r - top) : lds_l[w][n][lm];
       }
       const float by = ref[n] > -INFINITY ? exp2_fast(ref[n] - top) : 1.0f;
       if (n) __syncthreads();
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *(f4v*)&lds_o[wave][(d * 64 + lane) * 4] = o[n][d] * by;
+      for (int d = 0; d < DT; ++d) *(f4v*)&lds_o[wave][(d * 64 + l) * 4] = o[n][d] * by;
       __syncthreads();
-      const int col = col0 + 16 * n + m;
+      const int col = col0 + 16 * n + lm;
       const int i = col / g.group, hq = head * g.group + col % g.group;
       // A row that sees no key gives zeros; one whose weights are all zero what the formula gives, 0 / 0.
       const bool sees = pos0 + i >= 0;
       for (int d = wave; d < DT; d += kWaves) {
-        f4v v = *(const f4v*)&lds_o[0][(d * 64 + lane) * 4];
+        f4v v = *(const f4v*)&lds_o[0][(d * 64 + l) * 4];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) v += *(const f4v*)&lds_o[w][(d * 64 + lane) * 4];
+        for (int w = 1; w < kWaves; ++w) v += *(const f4v*)&lds_o[w][(d * 64 + l) * 4];
         if (col >= cols) continue;
         if (alone) {
           v = sees ? v / total : f4v{0, 0, 0, 0};
-          *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 16 * d + 4 * grp) = v;
+          *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 16 * d + 4 * lg) = v;
         } else {
-          const int64_t at = part * (16 * NT) + 16 * n + m;
-          *(f4v*)(g.part_o + at * D + 16 * d + 4 * grp) = v;
-          if (d == 0 && grp == 0) *(float2*)(g.part_ml + 2 * at) = make_float2(top, total);
+          const int64_t at = part * (16 * NT) + 16 * n + lm;
+          *(f4v*)(g.part_o + at * D + 16 * d + 4 * lg) = v;
+          if (d == 0 && lg == 0) *(float2*)(g.part_ml + 2 * at) = make_float2(top, total);
         }
       }
     }

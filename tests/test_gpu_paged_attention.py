@@ -194,3 +194,46 @@ def test_workspace_is_as_large_as_it_says(dev, types, heads, kv_heads, d, rows):
     after = whole.host()
     assert (after[need:] == 0x5A).all() and (after[:need] != 0x5A).any()
     assert np.array_equal(got, run(dev, q, cache, lengths, rows, heads, types))
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("d, length", [(48, 40), (64, 300), (128, 5000)])
+def test_rows_that_do_not_see_infinities_and_nan(dev, types, d, length):
+    """NaN and infinities in the last row's key and value, among the tile that the rows before it see a part of: their
+    results are the finite ones, and the last row's what the formula makes of them."""
+    rng = np.random.default_rng(d)
+    q_bf16, c_bf16 = TYPES[types]
+    lengths, rows = [length, 33], [3, 1]
+    for where, bad in (("v", math.nan), ("v", math.inf), ("k", math.nan), ("k", -math.inf)):
+        cache = po.Cache(rng, lengths, 2, d, 16, c_bf16)
+        q = queries(rng, rows, 4, d, types)
+        j = length - 1
+        page, place = cache.table[0, j // 16], j % 16
+        value = to_bf16(np.float32([bad]))[0][0] if c_bf16 else np.float32(bad)
+        if where == "v":
+            cache.v_cache[page, 0, 5, place] = value
+        else:
+            cache.k_cache[page, 0, place, 5] = value
+        got = run(dev, q, cache, lengths, rows, 4, types)
+        sees = got[2].copy()
+        got[2, :2] = 0  # of the first key head's queries, which see it: below
+        part = q.copy()
+        want, bound = po.attention(part[:3], cache.k[0], cache.v[0], length, scale=1.0 / math.sqrt(d))
+        want[2, :2] = 0
+        assert (np.abs(got[:3] - want) <= bound).all(), (where, bad)
+        check(got[3:], q[3:], type("C", (), dict(k=cache.k[1:], v=cache.v[1:])), lengths[1:], rows[1:])
+        if where == "v":  # one value of the weighted sum
+            assert np.isnan(sees[:2, 5]).all() if math.isnan(bad) else (sees[:2, 5] == bad).all()
+            others = np.arange(d) != 5
+            full, bound = po.attention(part[:3], cache.k[0], cache.v[0], length, scale=1.0 / math.sqrt(d))
+            assert (np.abs(sees[:2] - full[2, :2]) <= bound[2, :2])[:, others].all()
+        elif math.isnan(bad):
+            assert np.isnan(sees[:2]).all()
+        else:  # a score of one infinity: all weight on its key (not a number), or none
+            for h in range(2):
+                if part[2, h, 5] < 0:
+                    assert np.isnan(sees[h]).all()
+                else:
+                    k = cache.k[0].copy()
+                    w = np.exp((k[:-1, 0].astype(np.float64) @ part[2, h].astype(np.float64)) / math.sqrt(d))
+                    np.testing.assert_allclose(sees[h], (w @ cache.v[0][:-1, 0]) / w.sum(), rtol=0, atol=1e-4)
