@@ -18,8 +18,10 @@ namespace {
 constexpr int kTileKeys = 32;  // keys a wave takes at once
 constexpr int kWaves = 4;
 constexpr int kMinTiles = 2 * kWaves;  // of a share
-// What splitting sequences costs (another beginning and end in every workgroup, a second launch, about 10 us), as tiles
-// that one workgroup works on meanwhile: 0.11 us for 8 KB of keys and values.
+// What splitting sequences costs (another beginning and end in every workgroup, a second launch, 7 to 10 us), as tiles
+// that one workgroup works on meanwhile: 0.11 us for 8 KB of keys and values.  us, unsplit | split, 8 key heads of 64, bf16:
+// 1 request of 1024 keys 9.5 | 12.1, of 2048 13.6 | 12.4, of 4000 22.5 | 13.2; 64 ragged ones of up to 1024 17.7 | 21.5, of up
+// to 2048 29.6 | 33.2; 24 of up to 16000 121 | 85; with 6 rows of 4 heads of 128 each, up to 8192 keys, 289 | 211.
 constexpr int kSplitCost = 64;
 constexpr int kRate = 64;  // workgroups that read as fast as the whole chip does
 template <int D, bool CB16, int NT>
@@ -79,9 +81,9 @@ __device__ __forceinline__ void split3(float a, float b, int& hi, int& mid, int&
 __device__ __forceinline__ f4v mfma32(v4i a, v4i b, f4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
 }
-// Half a product: four values a lane, the other four zero.  (The product of 16 in the same chain of sums read the ones of
+// An operand of half a product: four values a lane, the other four zero.  (The product of 16 in the same chain of sums read the ones of
 // 32 before they were done, in one build of this file.)
-__device__ __forceinline__ f4v mfma_half(v2i a, v2i b, f4v c) { return mfma32(v4i{a[0], a[1], 0, 0}, v4i{b[0], b[1], 0, 0}, c); }
+__device__ __forceinline__ v4i half(v2i a) { return v4i{a[0], a[1], 0, 0}; }
 
 // The operands of one tile, in the order of the matrix instructions' lanes.  A wave's lane is (m, g) = (lane % 16,
 // lane / 16).  S^T = K Q^T comes in two products of 16 keys, row 4a + i of product t being key 8a + 4t + i of the
@@ -95,7 +97,7 @@ struct Tile<D, true> {
   static constexpr int KS = D / 32, DT = D / 16;
   static constexpr bool HALF = D % 32 != 0;  // 16 dimensions more
   v4i k[2][KS];
-  v2i kh[2];
+  v4i kh[2];
   v4i v[DT];
   __device__ __forceinline__ void load_k(const char* kc, int64_t at, int g) {  // at: element of the row's first dimension
 #pragma unroll
@@ -103,7 +105,7 @@ struct Tile<D, true> {
       const char* p = kc + 2 * (at + t * 4 * D);
 #pragma unroll
       for (int s = 0; s < KS; ++s) k[t][s] = *(const v4i*)(p + 64 * s + 16 * g);
-      if constexpr (HALF) kh[t] = *(const v2i*)(p + 64 * KS + 8 * g);
+      if constexpr (HALF) kh[t] = half(*(const v2i*)(p + 64 * KS + 8 * g));
     }
   }
   __device__ __forceinline__ void load_v(const char* vc, int64_t at, int page_shift) {  // at: element of (dimension m, key 8g)
@@ -157,13 +159,13 @@ struct Query<D, true, QP> {
   static constexpr int KS = D / 32;
   static constexpr bool HALF = D % 32 != 0;
   v4i q[QP][KS];
-  v2i qh[QP];
+  v4i qh[QP];
   __device__ __forceinline__ void load(const void* base, int64_t at, bool there, int, int g) {
     if constexpr (QP == 1) {
       const uint16_t* p = (const uint16_t*)base + at;
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[0][s] = there ? *(const v4i*)(p + 32 * s + 8 * g) : v4i{0, 0, 0, 0};
-      if constexpr (HALF) qh[0] = there ? *(const v2i*)(p + 32 * KS + 4 * g) : v2i{0, 0};
+      if constexpr (HALF) qh[0] = half(there ? *(const v2i*)(p + 32 * KS + 4 * g) : v2i{0, 0});
     } else {
       const float* p = (const float*)base + at;
 #pragma unroll
@@ -180,11 +182,11 @@ struct Query<D, true, QP> {
       }
       if constexpr (HALF) {
         const f4v a = there ? *(const f4v*)(p + 32 * KS + 4 * g) : f4v{0, 0, 0, 0};
-        int w[3][2];
-        split3(a[0], a[1], w[0][0], w[1][0], w[2][0]);
-        split3(a[2], a[3], w[0][1], w[1][1], w[2][1]);
+        int x[3], y[3];
+        split3(a[0], a[1], x[0], x[1], x[2]);
+        split3(a[2], a[3], y[0], y[1], y[2]);
 #pragma unroll
-        for (int j = 0; j < 3; ++j) qh[j] = v2i{w[j][0], w[j][1]};
+        for (int j = 0; j < 3; ++j) qh[j] = v4i{x[j], y[j], 0, 0};
       }
     }
   }
@@ -194,7 +196,7 @@ struct Query<D, true, QP> {
     for (int j = QP - 1; j >= 0; --j) {  // the small parts first
 #pragma unroll
       for (int s = 0; s < KS; ++s) c = mfma32(x.k[t][s], q[j][s], c);
-      if constexpr (HALF) c = mfma_half(x.kh[t], qh[j], c);
+      if constexpr (HALF) c = mfma32(x.kh[t], qh[j], c);
     }
     return c;
   }
@@ -765,10 +767,14 @@ Plan plan_of(const PagedAttnArgs& g) {
   const int waves = g.head_dim == 48    ? instance_waves<48>(g, p.nt)
                     : g.head_dim == 64 ? instance_waves<64>(g, p.nt)
                                        : instance_waves<128>(g, p.nt);
-  const int64_t tiles_most = (keys + kTileKeys - 1) / kTileKeys;
+  const int64_t tiles_most = (keys + kTileKeys - 1) / kTileKeys, work = sequences * (tiles_most + kBegin);
   const int cost = kSplitCost * 8 / (g.head_dim / 8 * (g.cache_bf16 ? 1 : 2)) / p.nt;
-  const int64_t tiles = (int64_t)std::max(1, g.requests) * g.kv_heads * p.qtiles * (tiles_most + kBegin + 1);
-  p.workers = (int)std::min<int64_t>((int64_t)kComputeUnits * waves, (tiles + kMinTiles + kBegin - 1) / (kMinTiles + kBegin));
+  // Few sequences are cut into as few parts as fill the chip's memory (us, one request of 131000 keys with two | three
+  // workgroups a compute unit 101.6 | 106.3), many by as many workgroups as run at once (61 requests of up to 4001 keys,
+  // two | four: 91.1 | 89.7).
+  const int64_t at_once = (int64_t)kComputeUnits * (sequences < kComputeUnits ? std::min(waves, 2) : waves);
+  p.workers = (int)std::max<int64_t>(1, std::min(at_once, (work + kMinTiles + kBegin - 1) / (kMinTiles + kBegin)));
+  // No second launch where a sequence is not worth splitting at its longest, or there are many.
   p.whole = tiles_most <= cost || sequences >= 4 * kComputeUnits * waves;
   return p;
 }
