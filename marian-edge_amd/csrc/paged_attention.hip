@@ -369,6 +369,17 @@ struct Slow {
   __device__ __forceinline__ float value(const void* p, int64_t i) const {
     return CB16 ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i];
   }
+  __device__ __forceinline__ float query_at(int64_t i) const {
+    return g.q_bf16 ? bf16_to_f32(((const uint16_t*)g.q)[i]) : ((const float*)g.q)[i];
+  }
+  __device__ bool finite(int64_t query) const {
+    float z = 0.0f;
+#pragma unroll 4
+    for (int d = lane >> 4; d < D; d += 4) z = __builtin_fmaf(query_at(query + d), 0.0f, z);
+    z += xor_lane_f<16>(z);
+    z += xor_lane_f<32>(z);
+    return z == 0.0f;
+  }
   __device__ void sum_keys(int64_t query, int pos, int first, int last) {
     const int grp = lane >> 4, place_mask = (1 << g.page_shift) - 1;
     ref = -INFINITY;
@@ -385,11 +396,9 @@ struct Slow {
         const bool there = (uint32_t)page < (uint32_t)g.num_pages;
         const int64_t block = ((int64_t)(there ? page : 0) * g.kv_heads + head) * D << g.page_shift;
         float score = 0.0f;
-#pragma unroll 1
-        for (int d = grp; d < D; d += 4) {
-          const float a = g.q_bf16 ? bf16_to_f32(((const uint16_t*)g.q)[query + d]) : ((const float*)g.q)[query + d];
-          score = __builtin_fmaf(a, value(g.k, block + (int64_t)place * D + d), score);
-        }
+#pragma unroll 4
+        for (int d = grp; d < D; d += 4)
+          score = __builtin_fmaf(query_at(query + d), value(g.k, block + (int64_t)place * D + d), score);
         score += xor_lane_f<16>(score);
         score += xor_lane_f<32>(score);
         score *= g.scale_log2e;
@@ -398,7 +407,7 @@ struct Slow {
         const float by = to > -INFINITY ? exp2_fast(ref - to) : 1.0f, w = exp2_fast(score - (to > -INFINITY ? to : 0.0f));
         ref = to;
         sum = sum * by + w;
-#pragma unroll 1
+#pragma unroll 2
         for (int d = 0; d < D / 16; ++d) {
           f4v v = o[d * 64 + lane] * by;
 #pragma unroll
@@ -598,17 +607,19 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
       }
     }
     // Infinities and NaN: a weight of zero times one that a row does not see, or a part of a product, makes a NaN of what is
-    // none.  Sums with any are formed again, key by key in the formula's own terms, as slow as that is.
-    float zero = 0.0f;
+    // none.  Columns with any, but for those whose query is the cause, are formed again, key by key in the formula's own
+    // terms, as slow as that is.
+    float zero[NT], any_zero = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      zero = __builtin_fmaf(sum[n], 0.0f, zero);
+      zero[n] = sum[n] * 0.0f;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(o[n][d][i], 0.0f, zero);
+        for (int i = 0; i < 4; ++i) zero[n] = __builtin_fmaf(o[n][d][i], 0.0f, zero[n]);
+      any_zero += zero[n];
     }
-    const bool odd = __any(zero != 0.0f);
+    const bool odd = __any(any_zero != 0.0f);
     if (l == 0) lds_odd[wave] = odd;
     __syncthreads();
     if (lds_odd[0] | lds_odd[1] | lds_odd[2] | lds_odd[3]) {
@@ -616,16 +627,23 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
         Slow<D, CB16> slow = {g, span, table, (f4v*)lds_o[wave], head, l};
 #pragma unroll 1
         for (int n = 0; n < NT; ++n) {
+          float z = zero[0];
+#pragma unroll
+          for (int k = 1; k < NT; ++k) z = k == n ? zero[k] : z;
+          z += xor_lane_f<16>(z);
+          z += xor_lane_f<32>(z);
           const int col = min(col0 + 16 * n + lm, cols - 1);
-          slow.sum_keys((int64_t)(rq.row0 + col / g.group) * g.ldq + (head * g.group + col % g.group) * D, pos0 + col / g.group,
-                        t0 + wave, last);
-          if (l < 16) {
+          const int64_t query = (int64_t)(rq.row0 + col / g.group) * g.ldq + (head * g.group + col % g.group) * D;
+          const bool again = z != 0.0f && slow.finite(query);
+          if (!__any(again)) continue;
+          slow.sum_keys(query, pos0 + col / g.group, t0 + wave, last);
+          if (again && l < 16) {
             lds_m[wave][n][l] = slow.ref;
             lds_l[wave][n][l] = slow.sum;
           }
 #pragma unroll
           for (int k = 0; k < NT; ++k) {
-            if (k != n) continue;
+            if (k != n || !again) continue;
             ref[k] = slow.ref;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[k][d] = slow.o[d * 64 + l];

@@ -237,3 +237,24 @@ def test_rows_that_do_not_see_infinities_and_nan(dev, types, d, length):
                     k = cache.k[0].copy()
                     w = np.exp((k[:-1, 0].astype(np.float64) @ part[2, h].astype(np.float64)) / math.sqrt(d))
                     np.testing.assert_allclose(sees[h], (w @ cache.v[0][:-1, 0]) / w.sum(), rtol=0, atol=1e-4)
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_queries_that_are_not_numbers(dev, types, bad):
+    """A row whose query holds a NaN or an infinity is NaN in that head alone, whatever lies beside it."""
+    rng = np.random.default_rng(21)
+    lengths, rows = [700, 33], [3, 2]
+    cache = po.Cache(rng, lengths, 2, 64, 16, TYPES[types][1])
+    q = queries(rng, rows, 4, 64, types)
+    wrong = q.copy()
+    wrong[1, 2, 7], wrong[3, 0, 63] = bad, bad
+    cache.v_cache[cache.table[0, 699 // 16], 1, 3, 699 % 16] = 0x7FC0 if TYPES[types][1] else math.nan  # row 2's own value
+    got = run(dev, wrong, cache, lengths, rows, 4, types)
+    assert np.isnan(got[1, 2]).all() and np.isnan(got[3, 0]).all() and np.isnan(got[2, 2:, 3]).all()
+    for b, at in ((0, 0), (1, 3)):
+        want, bound = po.attention(q[at:at + rows[b]], cache.k[b], cache.v[b], lengths[b], scale=1.0 / math.sqrt(64))
+        off = np.abs(got[at:at + rows[b]] - want)
+        fine = np.isfinite(got[at:at + rows[b]])
+        assert (off[fine] <= bound[fine]).all()
+    assert np.isnan(got).sum() == 64 + 64 + 2
