@@ -159,9 +159,13 @@ __global__ __launch_bounds__(kThreads) void k_verify(VerifyArgs g, int slices) {
       const f4v nv = load4<BF16>(row, next, g.V);
       f4v nd = nv;
       if (less) nd = load4<BF16>(other, next, g.V);
-      uint64_t w[4];
-      weights(v, d, id, w);
-      const uint64_t all = wave_scan_mass((w[0] + w[1]) + (w[2] + w[3]));
+      uint64_t all = 0;
+      // Groups of which nothing is kept are left out (a row's one id, or its infinities, are not told by the border).
+      if (target.flags || __any(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= target.border_v)) {
+        uint64_t w[4];
+        weights(v, d, id, w);
+        all = wave_scan_mass((w[0] + w[1]) + (w[2] + w[3]));
+      }
       if (lane == 63) shared_store(&seg[s], all);
       v = nv;
       d = nd;

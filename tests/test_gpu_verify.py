@@ -209,3 +209,28 @@ def test_many_requests(dev):
     got = run(dev, logits, cu, drafts, u, u_draw, settings, small)
     want = oracle(logits, cu, drafts, u, u_draw, settings, small)
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]) and got[2] == 0
+
+
+@pytest.mark.parametrize("v, requests, most, drafted", [(5000, 150, 7, True), (5000, 150, 7, False), (33000, 70, 6, True),
+                                                         (200, 24, 90, True), (300, 900, 4, False)])
+def test_more_rows_than_run_at_once(dev, v, requests, most, drafted):
+    """Many workgroups a compute unit, one after the other; some drafts and numbers out of range among them, and requests of
+    more than 64 rows."""
+    rng = np.random.default_rng(v + most)
+    counts = rng.integers(0, most + 1, size=requests)
+    counts[rng.integers(0, requests)] = most
+    cu, logits, small, u, u_draw = case(rng, v, counts, 0.35)
+    settings = mixed(rng, requests)
+    if most > 64:
+        settings, small, u = (None,) * 4, logits + np.float32(0.01) * small, 0.9 * u  # long runs of accepted drafts
+    drafts = drawn(rng, small, cu, settings)
+    odd = rng.random(len(u)) < 0.02
+    drafts[odd] = rng.choice([-1, v, v + 7], size=int(odd.sum()))
+    u = u.copy()
+    u[rng.random(len(u)) < 0.02] = 1.0
+    for _ in range(2):  # the workspace as the last call left it
+        got = run(dev, logits, cu, drafts, u, u_draw, settings, small if drafted else None, max_rows=most)
+        want = oracle(logits, cu, drafts, u, u_draw, settings, small if drafted else None)
+        assert np.array_equal(got[1], want[1])
+        assert np.array_equal(got[0], want[0]) and got[2] == 1
+    assert want[1].max() > (3 if drafted else 0)
