@@ -141,6 +141,10 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
   constexpr int NW = T / 64, NJ = IDS / (4 * T);  // slots of four ids per thread
   static_assert(NJ * 4 * T == IDS && T >= kList && kBins % T == 0, "whole slots");
   __shared__ __attribute__((aligned(16))) SampleLds<T, IDS> L;
+  // The ids of a bin that a list is too short for, where the row itself is not at hand: from then on they are what is
+  // looked at (verify_drafts, us without | with them: 100 requests of 100003 ids 162 | 132, 4 of 131072 129 | 90).
+  constexpr int CROWD = KEPT && IDS == 0 ? 4096 : 0;
+  __shared__ uint64_t crowded[CROWD ? CROWD : 1];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t row = blockIdx.x;
   int64_t set = row;  // of the settings
@@ -510,9 +514,15 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
       int first = 0, last = 0, shift = -1;  // shift: of a part's number
       uint64_t lo = 0, hi = ~0ull;          // pairs looked at
       above = 0;
+      int crowd = 0;  // ids in `crowded`
 #pragma unroll 1
       for (;;) {
-        if (shift >= 0) {
+        if (CROWD > 0 && crowd > 0) {
+          for (int i = t; i < crowd; i += T) {
+            const uint64_t p = crowded[i];
+            if (p >= lo && p <= hi) lds_add(&L.hist[(hi - p) >> shift], stage == BORDER_P ? mass_of(pair_logit(p)) : (uint64_t)1);
+          }
+        } else if (shift >= 0) {
           each([&](int, int i, f4v v) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -551,7 +561,14 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
         }
         need -= f.before;
         above += f.before;
-        if (last >= 0) {
+        if (CROWD > 0 && crowd > 0) {
+          for (int i = t; i < crowd; i += T) {
+            const uint64_t p = crowded[i];
+            if (p < lo || p > hi) continue;
+            const uint32_t at = lds_add(&L.listed, 1u);
+            if (at < (uint32_t)kList) L.entry[at] = p;
+          }
+        } else if (last >= 0) {
           const float least = least_of(last), most = first ? most_of(first) : INFINITY;
           each([&](int, int i, f4v v) {
             bool in[4];
@@ -566,6 +583,7 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
               if (b < first || b > last || p < lo || p > hi || p < pair_of(border_v, (uint32_t)border_id)) continue;
               const uint32_t at = lds_add(&L.listed, 1u);
               if (at < (uint32_t)kList) L.entry[at] = p;
+              if (CROWD > 0 && shift < 0 && at < (uint32_t)CROWD) crowded[at] = p;
               if (shift < 0 && stage >= BORDER_K) {  // the range of all, should they be too many
                 __hip_atomic_fetch_min(&L.lo, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                 __hip_atomic_fetch_max(&L.hi, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -578,6 +596,7 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
         if (shift < 0) {
           lo = L.lo;
           hi = L.hi;
+          if (CROWD > 0 && L.listed <= (uint32_t)CROWD) crowd = (int)L.listed;
         }
         shift = max(0, 64 - 11 - __builtin_clzll((hi - lo) | 1));  // kBins parts of [lo, hi]
       }

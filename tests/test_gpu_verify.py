@@ -234,3 +234,20 @@ def test_more_rows_than_run_at_once(dev, v, requests, most, drafted):
         assert np.array_equal(got[1], want[1])
         assert np.array_equal(got[0], want[0]) and got[2] == 1
     assert want[1].max() > (3 if drafted else 0)
+
+
+@pytest.mark.parametrize("v", [3000, 32000, 40001, 131072])
+def test_equal_logits(dev, v):
+    """Few distinct logits: borders inside long runs of equal ones, bins of more ids than a list holds."""
+    rng = np.random.default_rng(v)
+    counts = [3, 1, 4, 2, 3, 5]
+    cu, logits, small, u, u_draw = case(rng, v, counts, 0.7)
+    logits, small = np.round(logits), np.round(small)
+    logits[2], logits[3, ::2] = 1.0, -np.inf
+    logits[5, 7], small[6, 9] = np.nan, -np.inf
+    settings = (np.array([1, 0.7, 1.3, 0.9, 1, 0.5], np.float32), np.array([0, 0, 0, 700, 0, 0]),
+                np.array([0.9, 0.5, 1, 0.7, 0.99, 1], np.float32), np.array([0, 0, 0.02, 0, 0.1, 0], np.float32))
+    drafts = drawn(rng, small, cu, settings)
+    got = run(dev, logits, cu, drafts, u, u_draw, settings, small)
+    want = oracle(logits, cu, drafts, u, u_draw, settings, small)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0]) and got[2] == 0
