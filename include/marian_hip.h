@@ -567,7 +567,7 @@ int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t l
  * weights and sums are fp32, products exact.  The order of the sums, and with it a result's
  * last bits, depends on the call's sizes and on the lengths of all its requests; the same
  * call gives the same bits.  q is fp32, or
- * bfloat16 with q_bf16 != 0 (then the cache must be too); ldq a multiple of 8, ldo of 4.
+ * bfloat16 with q_bf16 != 0; ldq a multiple of 8, ldo of 4.
  * max_rows (at most 64) and max_keys (at most 2^27) bound every request's rows and length:
  * they choose the split.  A request past them, or whose rows are not within rows, sets *err
  * (device int, may be NULL) to 1 and its rows are left as they were, as are rows that

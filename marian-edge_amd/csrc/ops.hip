@@ -600,7 +600,6 @@ const char* paged_attention_sizes(PagedAttnArgs& g, int64_t requests, int64_t ma
   if (kv_heads <= 0 || kv_heads > kMaxKvHeads || heads <= 0 || heads > kMaxKvHeads || heads % kv_heads)
     return "heads is a multiple of kv_heads, both at most 128";
   if (head_dim != 48 && head_dim != 64 && head_dim != 128) return "head_dim is 48, 64 or 128";
-  if (q_bf16 && !cache_bf16) return "bfloat16 queries need a bfloat16 cache";
   g.q_bf16 = q_bf16 ? 1 : 0;
   g.cache_bf16 = cache_bf16 ? 1 : 0;
   g.requests = (int)requests;

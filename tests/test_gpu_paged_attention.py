@@ -19,7 +19,7 @@ def dev(pkg):
     return d
 
 
-TYPES = {"f32": (False, False), "mixed": (False, True), "bf16": (True, True)}  # (queries, cache) in bfloat16
+TYPES = {"f32": (False, False), "mixed": (False, True), "bf16": (True, True), "wide": (True, False)}  # (queries, cache) in bfloat16
 
 
 def run(dev, q, cache, lengths, rows, heads, types, window=0, sinks=0, scale=None, max_rows=None, max_keys=None, ldq=None,

@@ -87,7 +87,6 @@ def attention_args(**change):
     (dict(ldo=508), "out of range"), (dict(ldq=516), "out of range"), (dict(ldo=514), "out of range"),
     (dict(ldq=1 << 30), "out of range"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
-    (dict(bf16=1, cache16=0), "bfloat16 cache"),
     (dict(q=at(0) + 8), "16-byte"), (dict(out=at(6) + 4), "16-byte"), (dict(kc=at(1) + 8), "16-byte"), (dict(vc=at(2) + 2), "16-byte"),
     (dict(ws=at(7) + 8), "16-byte"),
     (dict(out=at(0)), "overlaps"), (dict(out=at(1) + 1024), "overlaps"), (dict(out=at(3)), "overlaps"), (dict(ws=at(2)), "overlaps"),
@@ -135,12 +134,12 @@ def test_workspace_sizes(pkg, lib):
     n = C.c_size_t(0)
     size = lib.marian_hip_paged_attention_workspace
     assert size(1, 1, 64, 8, 8, 64, 1, 1, 0, 0, C.byref(n)) == pkg._lib.OK and n.value == 0  # one piece
-    for q16, c16 in ((0, 0), (0, 1), (1, 1)):
+    for q16, c16 in ((0, 0), (0, 1), (1, 1), (1, 0)):
         assert size(1, 1, 100000, 8, 8, 64, q16, c16, 0, 0, C.byref(n)) == pkg._lib.OK and n.value > 8 * 64 * 4
         assert size(1, 1, 100000, 8, 8, 64, q16, c16, 100, 4, C.byref(n)) == pkg._lib.OK and n.value == 0  # a short window
     assert size(1, 1, 100000, 8, 8, 64, 1, 1, 0, 0, None) == pkg._lib.ERR_INVALID_INPUT
     for bad in ((-1, 1, 64, 8, 8, 64, 1, 1, 0, 0), (1, 65, 64, 8, 8, 64, 1, 1, 0, 0), (1, 1, 64, 8, 3, 64, 1, 1, 0, 0),
-                (1, 1, 64, 8, 8, 65, 1, 1, 0, 0), (1, 1, 64, 8, 8, 64, 1, 1, -1, 0), (1, 1, 64, 8, 8, 64, 1, 0, 0, 0)):
+                (1, 1, 64, 8, 8, 65, 1, 1, 0, 0), (1, 1, 64, 8, 8, 64, 1, 1, -1, 0)):
         assert size(*bad, C.byref(n)) == pkg._lib.ERR_INVALID_INPUT
     of_rows = lib.marian_hip_verify_drafts_workspace
     assert of_rows(10, 3, 1000, 0, C.byref(n)) == pkg._lib.OK
