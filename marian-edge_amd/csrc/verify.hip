@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void k_verify(VerifyArgs g, int slices) {
   // ---- the last workgroup: the group, and its id ----
   uint64_t total;
 #pragma unroll 1
-  for (;;) {
+  for (bool again = false;; again = true) {
     uint64_t mine = 0;
     for (int s = t; s < segs; s += kThreads) mine += shared_load(&seg[s]);
     mine = wave_scan_mass(mine);
@@ -192,8 +192,8 @@ __global__ __launch_bounds__(kThreads) void k_verify(VerifyArgs g, int slices) {
     total = 0;
 #pragma unroll
     for (int w = 0; w < kVerifyWaves; ++w) total += sums[w];
-    if (total) break;
-    // p is nowhere over q (they are equal but for rounding): from p.
+    if (total || again) break;
+    // p is nowhere over q (they are equal but for rounding): from p, whose sum is not 0.
     less = false;
     without = -1;
     __syncthreads();
