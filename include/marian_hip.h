@@ -571,7 +571,8 @@ int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t l
  * max_rows (at most 64) and max_keys (at most 2^27) bound every request's rows and length:
  * they choose the split.  A request past them, or whose rows are not within rows, sets *err
  * (device int, may be NULL) to 1 and its rows are left as they were, as are rows that
- * are no request's; a page out of range that a row sees sets *err, its keys count as unseen.
+ * are no request's; a page out of range that a row sees sets *err, its keys count as unseen (a
+ * row that sees no others gets zeros).
  * heads a multiple of kv_heads, up to 128; head_dim 48, 64 or 128; scale positive.
  * q, out, the caches and workspace must be 16-byte aligned.  workspace: device memory of
  * marian_hip_paged_attention_workspace bytes that no other call uses meanwhile, or

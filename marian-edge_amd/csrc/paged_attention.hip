@@ -5,7 +5,8 @@
 // with j > p - window or j < sinks:
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q k_j).
 // One pass over the keys keeps, per query, a reference m close to the largest score so far, l = sum w_j e^-m and the sum
-// of w_j e^-m v_j; parts of the keys join by rescaling each to the largest m.
+// of w_j e^-m v_j; parts of the keys join by rescaling each to the largest m.  m is -inf only where no key has been seen: a
+// seen one, whatever its score, makes it kSeen at least (scores of -inf alone give 0 / 0, no key at all gives 0).
 #include "device_common.h"
 #include "kernels.h"
 #include "mass.h"
@@ -30,6 +31,7 @@ constexpr int split_cost() {
 }
 // Scores (in octaves) may pass the reference by so much before the sums are rescaled: weights up to 2^8.
 constexpr float kSlack = 8.0f;
+constexpr float kSeen = -0x1.fffffep127f;  // the lowest finite value
 
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef int v2i __attribute__((ext_vector_type(2)));
@@ -403,8 +405,7 @@ struct Slow {
         score += xor_lane_f<32>(score);
         score *= g.scale_log2e;
         if (!there || key > pos || (g.window > 0 && key <= pos - g.window && key >= g.sinks)) continue;
-        const float to = score > ref ? score : ref;
-        const float by = to > -INFINITY ? exp2_fast(ref - to) : 1.0f, w = exp2_fast(score - (to > -INFINITY ? to : 0.0f));
+        const float to = fmaxf(fmaxf(score, kSeen), ref), by = exp2_fast(ref - to), w = exp2_fast(score - to);
         ref = to;
         sum = sum * by + w;
 #pragma unroll 2
@@ -516,6 +517,7 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
 
     Tile<D, CB16> x;
     int it = t0 + wave;
+    bool saw = false;  // a tile that every row sees whole
     int page_k = 0, page_v = 0, next_k = 0, next_v = 0;
     auto load_k = [&](int tile, int page) {
       const int key = tile * kTileKeys + 8 * (m >> 2) + (m & 3);
@@ -553,24 +555,25 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
                          (g.window <= 0 || key0 > span.last_pos - g.window || key0 + kTileKeys <= g.sinks);
       const bool bad = !in_range(page);
       if (!whole || __any(bad)) {
-        uint32_t some = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = kg + i;
-          const bool any = key <= span.last_pos && (g.window <= 0 || key > span.first_pos - g.window || key < g.sinks);
-          some |= any ? 1u << i : 0u;
-        }
+        // Which of the lane's eight keys are seen by rows from position `low` to `high`.
+        auto first_of = [](int n) { return (1u << min(max(n, 0), 8)) - 1; };
+        auto seen = [&](int low, int high) {
+          const uint32_t out = g.window > 0 ? first_of(low - g.window + 1 - kg) & ~first_of(g.sinks - kg) : 0u;
+          return first_of(high + 1 - kg) & ~out;
+        };
+        uint32_t some = seen(span.first_pos, span.last_pos);
         if (bad && some && g.err) *g.err = 1;
         if (bad) some = 0;
         x.keep_v(some);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          const uint32_t see = some & seen(pos[n], pos[n]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = kg + i;
-            const bool see = (some >> i & 1) && key <= pos[n] && (g.window <= 0 || key > pos[n] - g.window || key < g.sinks);
-            s[n][i >> 2][i & 3] = see ? s[n][i >> 2][i & 3] : -INFINITY;
-          }
+          for (int i = 0; i < 8; ++i) s[n][i >> 2][i & 3] = see >> i & 1 ? s[n][i >> 2][i & 3] : -INFINITY;
+          if (see) ref[n] = fmaxf(ref[n], kSeen);  // as long as it is kSeen the column's lanes may differ: all sums are 0
+        }
+      } else {
+        saw = true;
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -602,6 +605,9 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
     const int lm = l & 15, lg = l >> 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      ref[n] = fmaxf(ref[n], saw ? kSeen : -INFINITY);
+      ref[n] = fmaxf(ref[n], xor_lane_f<16>(ref[n]));
+      ref[n] = fmaxf(ref[n], xor_lane_f<32>(ref[n]));
       sum[n] += xor_lane_f<16>(sum[n]);
       sum[n] += xor_lane_f<32>(sum[n]);
       if (l < 16) {
@@ -674,15 +680,13 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
       __syncthreads();
       const int col = col0 + 16 * n + lm;
       const int i = col / g.group, hq = head * g.group + col % g.group;
-      // A row that sees no key gives zeros; one whose weights are all zero what the formula gives, 0 / 0.
-      const bool sees = pos0 + i >= 0;
       for (int d = wave; d < DT; d += kWaves) {
         f4v v = *(const f4v*)&lds_o[0][(d * 64 + l) * 4];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) v += *(const f4v*)&lds_o[w][(d * 64 + l) * 4];
         if (col >= cols) continue;
         if (alone) {
-          v = sees ? v / total : f4v{0, 0, 0, 0};
+          v = top > -INFINITY ? v / total : f4v{0, 0, 0, 0};
           *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 16 * d + 4 * lg) = v;
         } else {
           const int64_t at = part * (16 * NT) + 16 * n + lm;
@@ -722,9 +726,8 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(PagedAttnArgs g, int lg
   const float2* ml = (const float2*)g.part_ml;
   const int quad = lane % QUADS, row = lane / QUADS;
   f4v v = {0, 0, 0, 0};
-  float sum = 0.0f;
+  float sum = 0.0f, top = -INFINITY;
   if (col_in < cols) {
-    float top = -INFINITY;
     for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[place(p)].x);
     top = wave_max(top);
     const float base = top > -INFINITY ? top : 0.0f;
@@ -762,7 +765,7 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(PagedAttnArgs g, int lg
   if (col_in < cols && lane < QUADS) {
     const int col = qt * 16 * NT + col_in, i = col / g.group, hq = head * g.group + col % g.group;
     *(f4v*)(g.out + (int64_t)(rq.row0 + i) * g.ldo + hq * D + 4 * quad) =
-        rq.len - rq.n + i >= 0 ? v / sum : f4v{0, 0, 0, 0};
+        top > -INFINITY ? v / sum : f4v{0, 0, 0, 0};
   }
 }
 
