@@ -562,11 +562,14 @@ int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t l
  * keys are in the cache already) and sees the keys j <= p; with window > 0 those with
  * j > p - window or j < sinks.  Query head h reads key head h / (heads / kv_heads).
  *   out[row, h] = sum_j softmax_j(scale q k_j) v_j   (fp32, [rows, heads * head_dim])
- * A row that sees no key (p < 0) gets zeros.  Keys and values that a row does not see do
- * not change its result, whatever they hold; pages that no row sees are not read.  Scores,
+ * A row that sees no key (p < 0) gets zeros.  Keys and values that a row does not see, and
+ * the queries of other rows and heads, do not change its result by a bit; but where 32 keys (from
+ * a multiple of 32 on) hold some that the row sees and some that only other rows do, infinities
+ * and NaN among the latter's values may change its last bits: the row's sums are then
+ * formed in another order.  Pages that no row sees are not read.  Scores,
  * weights and sums are fp32, products exact.  The order of the sums, and with it a result's
- * last bits, depends on the call's sizes and on the lengths of all its requests; the same
- * call gives the same bits.  q is fp32, or
+ * last bits, depends on the call's sizes and on the lengths and rows of all its requests; the
+ * same call gives the same bits.  q is fp32, or
  * bfloat16 with q_bf16 != 0; ldq a multiple of 8, ldo of 4.
  * max_rows (at most 64) and max_keys (at most 2^27) bound every request's rows and length:
  * they choose the split.  A request past them, or whose rows are not within rows, sets *err

@@ -582,7 +582,7 @@ __global__ __launch_bounds__(kThreads, (waves_a_simd<D, CB16, QP, NT>())) void k
         if (__any(top > ref[n] + kSlack)) {
           top = fmaxf(top, xor_lane_f<16>(top));
           top = fmaxf(top, xor_lane_f<32>(top));
-          const float to = fmaxf(ref[n], top);
+          const float to = top > ref[n] + kSlack ? top : ref[n];  // each column by its own scores, whatever the others'
           const float by = to > -INFINITY ? exp2_fast(ref[n] - to) : 1.0f;
           ref[n] = to;
           sum[n] *= by;
