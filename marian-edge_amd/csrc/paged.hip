@@ -336,7 +336,8 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs g) {
     }
   }
   const bool mine = lane >= 8 && lane < 8 + kAppendRows && slot >= 0;
-  const uint32_t next = (uint32_t)__ballot(slot >= 0 && lane < 31 && __shfl_down(slot, 1) == slot + 1);
+  const int after = __shfl_down(slot, 1);  // by every lane: what one gives that is masked off is not defined
+  const uint32_t next = (uint32_t)__ballot(slot >= 0 && lane < 31 && after == slot + 1);
   const int first = lane - (slot & 7);  // lane of the group's first row
   const bool grouped = first >= 0 && lane < 32 && (next >> (first & 31) & 0x7F) == 0x7F;
   uint32_t groups = (uint32_t)__ballot(mine && grouped && first == lane);
