@@ -177,11 +177,10 @@ def paged_plan(lengths, new_tokens, page_size: int, block_table, pages_held, fre
                pages_held_out, free_count_out, cu_rows, served, slot_of_row=None, request_of_row=None, position_of_row=None,
                row_cap=None, err=None, stream=None) -> None:
     """marian_hip_paged_plan: pages, slots and rows of a step.  lengths_out, pages_held_out and free_count_out may be
-    the inputs.  row_cap: the most rows of the step (the length of the row maps that are given)."""
+    the inputs.  row_cap: the most rows of the step (the length of the shortest row map that is given)."""
     requests, max_blocks = block_table.shape
     if row_cap is None:
-        maps = slot_of_row or request_of_row or position_of_row
-        row_cap = maps.shape[0] if maps else 0
+        row_cap = min([m.shape[0] for m in (slot_of_row, request_of_row, position_of_row) if m is not None] or [0])
     _lib.check(_lib.load().marian_hip_paged_plan(
         lengths.ptr, new_tokens.ptr, pages_held.ptr, requests, int(page_size), block_table.ptr, max_blocks, free_pages.ptr,
         free_count.ptr, free_pages.shape[0], lengths_out.ptr, pages_held_out.ptr, free_count_out.ptr, cu_rows.ptr,
