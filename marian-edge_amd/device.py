@@ -190,8 +190,11 @@ def paged_plan(lengths, new_tokens, page_size: int, block_table, pages_held, fre
 def paged_append(k, v, slot_of_row, k_cache, v_cache, ldk=None, ldv=None, bf16: bool = False, cache_bf16: bool = False,
                  err=None, stream=None) -> None:
     """marian_hip_paged_append: rows k and v into their slots of k_cache [pages, kv_heads, page_size, head_dim] and
-    v_cache [pages, kv_heads, head_dim, page_size]; bf16: of the rows."""
+    v_cache [pages, kv_heads, head_dim, page_size]; bf16: of the rows.  k and v have a row for every slot, also for the
+    negative ones at the end of a map that paged_plan has filled up."""
     pages, kv_heads, page_size, head_dim = k_cache.shape
+    if min(k.shape[0], v.shape[0]) < slot_of_row.shape[0]:
+        raise ValueError("paged_append: k or v has fewer rows than slot_of_row")
     _lib.check(_lib.load().marian_hip_paged_append(
         k.ptr, ldk or k.shape[1], v.ptr, ldv or v.shape[1], int(bf16), slot_of_row.ptr, slot_of_row.shape[0], kv_heads,
         head_dim, k_cache.ptr, v_cache.ptr, int(cache_bf16), pages, page_size, _p(err), stream), "paged_append")

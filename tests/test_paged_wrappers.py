@@ -35,3 +35,18 @@ def test_plan_writes_no_more_rows_than_the_shortest_map_has(calls, slot, request
     device.paged_plan(*state, **maps)
     device.paged_plan(*state, row_cap=3, **maps)
     assert [a[17] for _, a in made] == [cap, 3]
+
+
+@pytest.mark.parametrize("k, v, slots, refused", [(8, 8, 8, False), (9, 8, 8, False), (8, 9, 8, False), (7, 8, 8, True), (8, 7, 8, True),
+                                                  (0, 0, 0, False), (0, 0, 1, True)])
+def test_append_needs_a_row_for_every_slot(calls, k, v, slots, refused):
+    """Rows are read before their slots are known."""
+    device, made = calls
+    call = lambda: device.paged_append(Buf(k, 128), Buf(v, 128), Buf(slots), Buf(30, 2, 16, 64), Buf(30, 2, 64, 16))  # noqa: E731
+    if refused:
+        with pytest.raises(ValueError, match="fewer rows"):
+            call()
+        assert not made
+    else:
+        call()
+        assert made[0][1][6] == slots
