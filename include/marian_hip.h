@@ -518,7 +518,9 @@ int marian_hip_q8_linear_lora_workspace(int64_t M, int64_t K, int64_t max_rank, 
  * in order.  The rows of a step are packed: request b's are [cu_rows[b], cu_rows[b + 1]).
  * A step is paged_plan, paged_append and paged_attention in every layer, then
  * sample_logits or verify_drafts; the next step's lengths are lengths_out, less what
- * verify_drafts rejected (lengths may shrink between steps: the pages stay). */
+ * verify_drafts rejected (lengths may shrink between steps: the pages stay); no call here takes
+ * that off, it is the caller's to do.  paged_attention takes at most 64 rows a request: longer
+ * prompts come in chunks of so many. */
 
 /* Pages, slots and rows of a step.  Request b has lengths[b] tokens, held by the first
  * pages_held[b] entries of its table row, and brings new_tokens[b] rows; a negative
@@ -527,8 +529,10 @@ int marian_hip_q8_linear_lora_workspace(int64_t M, int64_t K, int64_t max_rank, 
  * requests are served in order, up to the first that needs more pages than there are,
  * more table entries than max_blocks or more rows than are left of row_cap: that one and
  * those after it get no rows and keep what they had, and *served tells how many came
- * before it (requests: all; a scheduler asks again once pages are back).  Pages are taken
- * from the top of the stack, a request's in order.
+ * before it (requests: all; a scheduler asks again once pages are back).  A request that can
+ * never be served (longer than max_blocks pages, more rows than row_cap, counts out of range)
+ * stops those after it at every step: *served names it, and the caller ends it, cuts its
+ * rows or moves it.  Pages are taken from the top of the stack, a request's in order.
  * lengths_out, pages_held_out and free_count_out (each may be the input that it follows)
  * hold the state after the step, cu_rows [requests + 1] the rows; for r below
  * cu_rows[requests], slot_of_row[r], request_of_row[r] and position_of_row[r] (each [row_cap]
@@ -566,11 +570,11 @@ int marian_hip_paged_append(const void* k, int64_t ldk, const void* v, int64_t l
  * the queries of other rows and heads, do not change its result by a bit; but where 32 keys (from
  * a multiple of 32 on) hold some that the row sees and some that only other rows do, infinities
  * and NaN among the latter's values may change its last bits: the row's sums are then
- * formed in another order.  Pages that no row sees are not read.  Scores,
- * weights and sums are fp32, products exact.  The order of the sums, and with it a result's
- * last bits, depends on the call's sizes and on the lengths and rows of all its requests; the
- * same call gives the same bits.  q is fp32, or
- * bfloat16 with q_bf16 != 0; ldq a multiple of 8, ldo of 4.
+ * formed in another order.  Caches are read by such 32 keys at a time: a page that lies in
+ * none of which some row sees a part is not read.  Scores, weights and sums are fp32, products
+ * exact.  The order of the sums, and with it a result's last bits, depends on the call's sizes
+ * and on the lengths and rows of all its requests; the same call gives the same bits.  q is
+ * fp32, or bfloat16 with q_bf16 != 0; ldq a multiple of 8, ldo of 4.
  * max_rows (at most 64) and max_keys (at most 2^27) bound every request's rows and length:
  * they choose the split.  A request past them, or whose rows are not within rows, sets *err
  * (device int, may be NULL) to 1 and its rows are left as they were, as are rows that

@@ -18,13 +18,17 @@ namespace {
 
 constexpr int kTileKeys = 32;  // keys a wave takes at once
 constexpr int kWaves = 4;
-constexpr int kMinTiles = 2 * kWaves;  // of a share
+// Least tiles of a share (us, 4 | 8 | 16 | 32: 1 request of 4000 keys of 8 heads of 64 13.5 | 14.2 | 15.3 | 17.7, 8 of up to 4000
+// of 8 heads of 128 with 6 rows of 4 heads each 28.0 | 31.3 | 26.9 | 34.6; calls whose shares are longer all the same).
+constexpr int kMinTiles = 2 * kWaves;
 // What splitting sequences costs (another beginning and end in every workgroup, a second launch, 7 to 10 us), as tiles
 // that one workgroup works on meanwhile: 0.11 us for 8 KB of keys and values.  us, unsplit | split, 8 key heads of 64, bf16:
 // 1 request of 1024 keys 9.5 | 12.1, of 2048 13.6 | 12.4, of 4000 22.5 | 13.2; 64 ragged ones of up to 1024 17.7 | 21.5, of up
 // to 2048 29.6 | 33.2; 24 of up to 16000 121 | 85; with 6 rows of 4 heads of 128 each, up to 8192 keys, 289 | 211.
 constexpr int kSplitCost = 64;
-constexpr int kRate = 64;  // workgroups that read as fast as the whole chip does
+// Workgroups that read as fast as the whole chip does (32, 64 and 128 within 1 % of each other from 1 to 300 requests, but for
+// 128 of up to 3000 keys of one head of 64: 24.1, 24.1 and 22.3 us).
+constexpr int kRate = 64;
 template <int D, bool CB16, int NT>
 constexpr int split_cost() {
   return kSplitCost * 8 / (D / 8 * (CB16 ? 1 : 2)) / NT;
@@ -83,8 +87,10 @@ __device__ __forceinline__ void split3(float a, float b, int& hi, int& mid, int&
 __device__ __forceinline__ f4v mfma32(v4i a, v4i b, f4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
 }
-// An operand of half a product: four values a lane, the other four zero.  (The product of 16 keys' own instruction, in turns
-// with the one of 32 on the same sums, gave wrong scores: head_dim 48, fp32 queries.)
+// An operand of half a product: four values a lane, the other four zero.  The instruction for 16 summed values is not
+// taken: right behind one of 32 on the same sums it adds to what they were before, and the compiler puts no wait
+// between the two (six in turns: all 256 sums wrong; with a wait for loads between them, none).  Sums that one kind of
+// instruction alone adds to are passed on in order.
 __device__ __forceinline__ v4i half(v2i a) { return v4i{a[0], a[1], 0, 0}; }
 
 // The operands of one tile, in the order of the matrix instructions' lanes.  A wave's lane is (m, g) = (lane % 16,
@@ -271,6 +277,8 @@ constexpr int waves_a_simd() {
 
 // A sequence is what one query tile and key head of a request see.  Work is counted in its tiles and kBegin more for its
 // beginning and end, in the order request, query tile, head.
+// us with 2 | 4 | 8 | 16: 61 ragged requests of up to 4001 keys 93.5 | 89.3 | 89.2 | 92.7, 64 of up to 8192 with 6 rows 213 | 211 |
+// 211 | 218, 24 of up to 16000 86.5 | 86.1 | 85.2 | 85.5.
 constexpr int kBegin = 8;
 template <int NT>
 __device__ __forceinline__ int64_t request_tiles(const PagedAttnArgs& g, const Request& r, int& longest) {
@@ -359,7 +367,8 @@ __device__ __forceinline__ Share share_of(const PagedAttnArgs& g, int worker, in
 }
 
 // One column's keys one after the other, a wave's lanes (m, g): the column of query m, dimensions d % 4 == g of the score
-// and 16 d + 4 g .. 4 g + 3 of the sums, which are kept in `o` (LDS).
+// and 16 d + 4 g .. 4 g + 3 of the sums, which are kept in `o` (LDS).  One key after the other, each a trip to memory: one NaN among
+// the values that a call's rows see takes 131000 keys from 103 us to 2.6 ms, 2000 keys of 8 heads of 64 from 15 us to 1.0 ms.
 template <int D, bool CB16>
 struct Slow {
   const PagedAttnArgs& g;
@@ -806,7 +815,7 @@ Plan plan_of(const PagedAttnArgs& g) {
 
 template <int D, bool CB16, int QP, int NT>
 hipError_t launch(const PagedAttnArgs& g, hipStream_t s) {
-  // At most 2^23 workgroups: 8192 requests, 64 rows each, 128 heads.
+  // At most 2^21 workgroups: 8192 requests of 256 sequences (64 rows of 128 heads, 32 columns each).
   const int64_t sequences = (int64_t)g.requests * g.qtiles * g.kv_heads;
   hipLaunchKernelGGL((k_paged_attention<D, CB16, QP, NT>), dim3((unsigned)(g.whole ? sequences : std::max<int64_t>(sequences, g.workers))),
                      dim3(kThreads), 0, s, g);
