@@ -550,14 +550,15 @@ struct RowKept {
 };
 // Records of a verification's rows: target rows 0 .. rows - 1 in kept[0 ..), and with draft_logits the draft row of
 // target row r (row draft_row[r], or r, of draft_logits) in kept[rows + r].  Settings are per request, request b's rows
-// cu[b] .. cu[b + 1).  Rows that nothing is drawn from (no request's; of the drafts a request's last) are left out.
+// cu[b] .. cu[b + 1), at most max_rows.  Rows that nothing is drawn from (no request's, or one's that cannot be taken; of the
+// drafts a request's last) are left out.
 struct KeptArgs : SampleArgs {
   const int32_t* cu = nullptr;
   int requests = 0;
   const void* draft_logits = nullptr;
   int64_t ld_draft = 0;
   const int32_t* draft_row = nullptr;
-  int draft_rows = 0;
+  int draft_rows = 0, max_rows = 0;  // max_rows: of a request
   const int32_t* drafts = nullptr;
   RowKept* kept = nullptr;
   int32_t* done = nullptr;  // [requests], set to 0
@@ -571,7 +572,6 @@ hipError_t launch_kept(const KeptArgs& g, hipStream_t s);
 struct VerifyArgs : KeptArgs {
   const float* u_draw = nullptr;
   uint64_t* seg = nullptr;  // [requests, groups of 256 ids]
-  int max_rows = 0;  // of a request
   int32_t* accepted = nullptr;
 };
 size_t verify_bytes(int64_t rows, int64_t requests, int64_t V, bool drafted);

@@ -154,8 +154,10 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
     wg_lds_barrier();
     int last = 0;
     for (int b = t; b < g.requests; b += T) {
-      const int end = g.cu[b + 1];
-      if (g.cu[b] <= r && r < end) {
+      const int begin = g.cu[b], end = g.cu[b + 1];
+      if (row == 0) g.done[b] = 0;
+      // Of requests whose rows can be taken: another's may lie over them.
+      if (begin >= 0 && begin <= r && r < end && end <= g.rows && end - begin <= g.max_rows) {
         L.found = b;
         L.best = end - 1;
       }
@@ -164,7 +166,6 @@ __global__ __launch_bounds__(T) void k_sample(std::conditional_t<KEPT, KeptArgs,
     set = __builtin_amdgcn_readfirstlane(L.found);
     last = __builtin_amdgcn_readfirstlane(L.best);
     if (set < 0) return;  // no request's
-    if (t == 0 && row < g.rows && r == g.cu[set]) g.done[set] = 0;
     if (row >= g.rows && r == last) return;  // nothing was drafted after a request's last row
     wg_lds_barrier();  // found and best are used again
   }
